@@ -26,7 +26,11 @@ ext = cpp_extension.CUDAExtension(
     sources=sources,
     extra_compile_args={
         "cxx": ["-O3", "-std=c++17"],
-        "nvcc": ["-O3", "-std=c++17", "--offload-arch=gfx950"],
+        # no packed-fp32 instructions: some of their forms have given wrong
+        # results on this hardware, and -O3 makes them from scalar code
+        "nvcc": ["-O3", "-std=c++17", "--offload-arch=gfx950",
+                 "-Xclang", "-target-feature", "-Xclang",
+                 "-packed-fp32-ops"],
     },
 )
 
