@@ -1,0 +1,667 @@
+// Attention inside documents that lie one behind the other, and its
+// gradients.
+//
+//   s_ij = scale q_i . k_j - slope_h |i - j|     i, j of the same document
+//   p_ij = exp(s_ij) / sum_j exp(s_ij)           o_i = sum_j p_ij v_j
+//   dv_j = sum_i p_ij do_i                       D_i = do_i . o_i
+//   ds_ij = p_ij (do_i . v_j - D_i)
+//   dq_i = scale sum_j ds_ij k_j                 dk_j = scale sum_i ds_ij q_i
+//
+// Documents are given by their borders (cu_seqlens); a tile begins where its
+// document does, so no tile holds two of them, what a document holds (NaN
+// too) never reaches another, and only a document's last tile has a mask.
+// Tokens in front of the first border and behind the last get zeros.
+//
+// Every product runs on 32x32x16 matrix instructions with the transposed
+// result: in S^T = K Q^T a lane holds one query, so the softmax of a row is
+// its lane's own but for one exchange with lane ^ 32, and the registers of
+// P^T are at once operand B of O^T = V^T P^T (mfma_tile.h).  The gradient of
+// keys and values takes S = Q K^T instead, a lane holding one key.  P is
+// rounded to the inputs' type for the second product, as its other operand
+// is; maxima, sums and all accumulators are fp32.
+//
+// No atomics: dq comes from a pass over keys, dk and dv from a pass over
+// queries, each with its own recomputation of P (two products of seven).
+#include <torch/extension.h>
+#include <ATen/cuda/CUDAContext.h>
+
+#include <cmath>
+#include <limits>
+
+#include "mfma_tile.h"
+
+namespace dlx {
+
+namespace {
+
+constexpr int kKeys = 64;             // rows of an LDS tile
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ const uint4 g_zero16 = {0, 0, 0, 0};
+
+struct View {                         // [tokens, heads, dim]
+  uint16_t* p;
+  long token, head;                   // strides, in elements
+};
+
+struct AttnArgs {
+  View q, k, v, o, dout, dq, dk, dv;
+  float* lse;                         // [heads, tokens], base 2
+  float* delta;                       // [heads, tokens]
+  const int* cu;
+  const float* slopes;                // [heads] or none
+  int docs, tokens, heads, group, dim;
+  float scale;
+};
+
+// Border e of the documents with what lies in front of and behind them:
+// 0, cu[0], .., cu[docs], tokens.  Clamped, so that no border, whatever the
+// caller's array holds, leads out of the tokens.
+DLX_DEV int border(const AttnArgs& a, int e) {
+  if (e == 0) return 0;
+  if (e == a.docs + 2) return a.tokens;
+  const int c = a.cu[e - 1];
+  return c < 0 ? 0 : c > a.tokens ? a.tokens : c;
+}
+
+struct Tile {
+  int start, len, row0;               // document, first row of the tile in it
+  bool doc;                           // false: in no document
+};
+
+// Tile t of ROWS rows.  Document e's tiles are numbered from
+// border(e) / ROWS + e, which leaves each at least as many as it has rows
+// for; the tiles it does not need are empty (row0 >= len).
+template <int ROWS> DLX_DEV Tile find_tile(const AttnArgs& a, int t) {
+  const int lane = threadIdx.x & (kWave - 1);
+  int lo = 0, n = a.docs + 2;         // the document is one of lo..lo+n-1
+  while (n > 1) {
+    const int step = (n + kWave - 1) / kWave;
+    const int e = lo + lane * step;
+    const bool at = lane * step < n && border(a, e) / ROWS + e <= t;
+    int c = __popcll(__ballot(at));
+    c = c < 1 ? 1 : c;
+    const int left = n - (c - 1) * step;
+    lo += (c - 1) * step;
+    n = left < step ? left : step;
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  Tile x;
+  x.start = border(a, lo);
+  x.len = border(a, lo + 1) - x.start;
+  x.row0 = (t - (x.start / ROWS + lo)) * ROWS;
+  x.doc = lo > 0 && lo <= a.docs;
+  if (x.row0 < 0) x.row0 = x.len < 0 ? 0 : x.len;
+  x.start = __builtin_amdgcn_readfirstlane(x.start);
+  x.len = __builtin_amdgcn_readfirstlane(x.len);
+  x.row0 = __builtin_amdgcn_readfirstlane(x.row0);
+  return x;
+}
+
+// Rows row0.. of a document into an LDS tile; rows behind its end repeat the
+// last one, chunks behind the head's width are zero.
+template <int DP, int NT>
+DLX_DEV void load_tile(uint16_t* lds, const uint16_t* base, long stride,
+                       int row0, int len, int dim) {
+  constexpr int CH = DP / 8;
+#pragma unroll
+  for (int u = 0; u < kKeys * CH / NT; ++u) {
+    const int f = u * NT + threadIdx.x;
+    const int row = f / CH;
+    const int chunk = (f % CH) ^ (row & 7);
+    const int r = row0 + row < len ? row0 + row : len - 1;
+    const void* src = base + r * stride + chunk * 8;
+    if (chunk * 8 >= dim) src = &g_zero16;
+    copy16_to_lds(src, lds + f * 8);
+  }
+}
+
+// Operand B of a wave's 32 rows, from memory.
+template <int DP>
+DLX_DEV void load_rows(s16x8* f, const uint16_t* row, int dim, int lane) {
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) {
+    const int c = (s * 2 + (lane >> 5)) * 8;
+    f[s] = c < dim ? *reinterpret_cast<const s16x8*>(row + c) : s16x8{};
+  }
+}
+
+// A result C[d][row] to row `row`: four d at a time.
+template <typename T, int DP>
+DLX_DEV void store_rows(uint16_t* row, const f32x16* acc, float by, int dim,
+                        int lane) {
+#pragma unroll
+  for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = b * 32 + g * 8 + (lane >> 5) * 4;
+      uint2 x;
+      x.x = pack2<T>(acc[b][g * 4] * by, acc[b][g * 4 + 1] * by);
+      x.y = pack2<T>(acc[b][g * 4 + 2] * by, acc[b][g * 4 + 3] * by);
+      if (d < dim) *reinterpret_cast<uint2*>(row + d) = x;
+    }
+}
+
+template <int DP>
+DLX_DEV void zero_rows(const View& v, long token, int head, int dim, int lane) {
+  uint16_t* row = v.p + token * v.token + head * v.head;
+  for (int c = (lane >> 5) * 8; c < dim; c += 16)
+    *reinterpret_cast<s16x8*>(row + c) = s16x8{};
+}
+
+// register i of a result: its row of 32
+DLX_DEV constexpr int reg_row(int i) { return 8 * (i >> 2) + (i & 3); }
+
+// ---------------------------------------------------------------------------
+// forward: a wave owns 32 queries, a block NW waves; keys and values pass in
+// tiles of 64, the next one on its way while this one is worked on.
+// ---------------------------------------------------------------------------
+
+template <typename T, int DP, int NW, bool BIAS>
+__global__ __launch_bounds__(NW * 64) void doc_attn_fwd_kernel(AttnArgs a) {
+  constexpr int NT = NW * 64, ROWS = NW * 32, TS = kKeys * DP;
+  __shared__ __attribute__((aligned(16))) uint16_t lds[4 * TS];
+
+  const int tiles = gridDim.x / a.heads;
+  const int bid = xcd_block(blockIdx.x, gridDim.x);
+  const int head = bid / tiles;
+  const Tile tl = find_tile<ROWS>(a, bid - head * tiles);
+  if (tl.row0 >= tl.len) return;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wid = threadIdx.x / kWave;
+  const int half = lane >> 5;
+  const int qpos = tl.row0 + wid * 32 + (lane & 31);
+  const bool real = qpos < tl.len;
+  if (!tl.doc) {
+    if (real) zero_rows<DP>(a.o, tl.start + qpos, head, a.dim, lane);
+    return;
+  }
+  const int kvh = head / a.group;
+  const uint16_t* kb = a.k.p + tl.start * a.k.token + kvh * a.k.head;
+  const uint16_t* vb = a.v.p + tl.start * a.v.token + kvh * a.v.head;
+  const long token = tl.start + (real ? qpos : tl.len - 1);
+
+  const int nt = (tl.len + kKeys - 1) / kKeys;
+  load_tile<DP, NT>(lds, kb, a.k.token, 0, tl.len, a.dim);
+  load_tile<DP, NT>(lds + TS, vb, a.v.token, 0, tl.len, a.dim);
+  s16x8 qf[DP / 16];
+  load_rows<DP>(qf, a.q.p + token * a.q.token + head * a.q.head, a.dim, lane);
+
+  const float sc = a.scale * kLog2e;
+  const float sl = BIAS ? a.slopes[head] * kLog2e : 0.f;
+  float m = -INFINITY, l = 0.f;
+  f32x16 acc[DP / 32] = {};
+
+  for (int t = 0; t < nt; ++t) {
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    const uint16_t* lk = lds + (t & 1) * 2 * TS;
+    const uint16_t* lv = lk + TS;
+    if (t + 1 < nt) {
+      uint16_t* nx = lds + ((t + 1) & 1) * 2 * TS;
+      load_tile<DP, NT>(nx, kb, a.k.token, (t + 1) * kKeys, tl.len, a.dim);
+      load_tile<DP, NT>(nx + TS, vb, a.v.token, (t + 1) * kKeys, tl.len, a.dim);
+    }
+    f32x16 s[2] = {};
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int st = 0; st < DP / 16; ++st)
+        s[b] = mfma32<T>(row_frag<DP>(lk, b * 32, st, lane), qf[st], s[b]);
+
+    const int k0 = t * kKeys + half * 4;      // key of register 0 of block 0
+    if (BIAS) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const float d0 = (float)(k0 + b * 32 - qpos);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          s[b][i] = s[b][i] * sc - sl * fabsf(d0 + (float)reg_row(i));
+      }
+    }
+    if ((t + 1) * kKeys > tl.len) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (k0 + b * 32 + reg_row(i) >= tl.len) s[b][i] = -INFINITY;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[b][i]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+    if (!BIAS) mx *= sc;
+    if (__ballot(mx > m)) {
+      const float mn = fmaxf(m, mx);
+      const float by = mn == -INFINITY ? 1.f : exp2f(m - mn);
+      m = mn;
+      l *= by;
+#pragma unroll
+      for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[b][i] *= by;
+    }
+    const float ms = m == -INFINITY ? 0.f : m;   // a row of -inf so far
+    float p[2][16];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        p[b][i] = __builtin_amdgcn_exp2f(BIAS ? s[b][i] - ms
+                                              : s[b][i] * sc - ms);
+        l += p[b][i];
+      }
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        const s16x8 pf = pack_step<T>(&p[b][st * 8]);
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+          acc[db] = mfma32<T>(
+              tr_frag<DP>(lv, b * 32 + st * 16, db * 32, lane), pf, acc[db]);
+      }
+  }
+  l += __shfl_xor(l, 32, kWave);
+  if (!real) return;
+  store_rows<T, DP>(a.o.p + token * a.o.token + head * a.o.head, acc, 1.f / l,
+                    a.dim, lane);
+  if (a.lse && half == 0)
+    a.lse[(long)head * a.tokens + token] = m + log2f(l);
+}
+
+// ---------------------------------------------------------------------------
+// gradient of the queries: the forward's walk over the keys, a third product.
+// Also writes delta, which the next kernel reads.
+// ---------------------------------------------------------------------------
+
+template <typename T, int DP, int NW, bool BIAS>
+__global__ __launch_bounds__(NW * 64) void doc_attn_dq_kernel(AttnArgs a) {
+  constexpr int NT = NW * 64, ROWS = NW * 32, TS = kKeys * DP;
+  __shared__ __attribute__((aligned(16))) uint16_t lds[4 * TS];
+
+  const int tiles = gridDim.x / a.heads;
+  const int bid = xcd_block(blockIdx.x, gridDim.x);
+  const int head = bid / tiles;
+  const Tile tl = find_tile<ROWS>(a, bid - head * tiles);
+  if (tl.row0 >= tl.len) return;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wid = threadIdx.x / kWave;
+  const int half = lane >> 5;
+  const int qpos = tl.row0 + wid * 32 + (lane & 31);
+  const bool real = qpos < tl.len;
+  if (!tl.doc) {
+    if (real) zero_rows<DP>(a.dq, tl.start + qpos, head, a.dim, lane);
+    return;
+  }
+  const int kvh = head / a.group;
+  const uint16_t* kb = a.k.p + tl.start * a.k.token + kvh * a.k.head;
+  const uint16_t* vb = a.v.p + tl.start * a.v.token + kvh * a.v.head;
+  const long token = tl.start + (real ? qpos : tl.len - 1);
+
+  const int nt = (tl.len + kKeys - 1) / kKeys;
+  load_tile<DP, NT>(lds, kb, a.k.token, 0, tl.len, a.dim);
+  load_tile<DP, NT>(lds + TS, vb, a.v.token, 0, tl.len, a.dim);
+  s16x8 qf[DP / 16], gf[DP / 16];
+  load_rows<DP>(qf, a.q.p + token * a.q.token + head * a.q.head, a.dim, lane);
+  load_rows<DP>(gf, a.dout.p + token * a.dout.token + head * a.dout.head,
+                a.dim, lane);
+  float delta = 0.f;
+  {
+    s16x8 of[DP / 16];
+    load_rows<DP>(of, a.o.p + token * a.o.token + head * a.o.head, a.dim, lane);
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        delta += to_f32<T>(T{(uint16_t)gf[s][e]}) *
+                 to_f32<T>(T{(uint16_t)of[s][e]});
+    delta += __shfl_xor(delta, 32, kWave);
+  }
+  if (real && half == 0) a.delta[(long)head * a.tokens + token] = delta;
+  const float lse = a.lse[(long)head * a.tokens + token];
+  const float sc = a.scale * kLog2e;
+  const float sl = BIAS ? a.slopes[head] * kLog2e : 0.f;
+  f32x16 acc[DP / 32] = {};
+
+  for (int t = 0; t < nt; ++t) {
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    const uint16_t* lk = lds + (t & 1) * 2 * TS;
+    const uint16_t* lv = lk + TS;
+    if (t + 1 < nt) {
+      uint16_t* nx = lds + ((t + 1) & 1) * 2 * TS;
+      load_tile<DP, NT>(nx, kb, a.k.token, (t + 1) * kKeys, tl.len, a.dim);
+      load_tile<DP, NT>(nx + TS, vb, a.v.token, (t + 1) * kKeys, tl.len, a.dim);
+    }
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      f32x16 s = {}, dp = {};
+#pragma unroll
+      for (int st = 0; st < DP / 16; ++st)
+        s = mfma32<T>(row_frag<DP>(lk, b * 32, st, lane), qf[st], s);
+#pragma unroll
+      for (int st = 0; st < DP / 16; ++st)
+        dp = mfma32<T>(row_frag<DP>(lv, b * 32, st, lane), gf[st], dp);
+      const int k0 = t * kKeys + b * 32 + half * 4;
+      const float d0 = (float)(k0 - qpos);
+      float ds[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float x = s[i] * sc - lse;
+        if (BIAS) x -= sl * fabsf(d0 + (float)reg_row(i));
+        ds[i] = __builtin_amdgcn_exp2f(x) * (dp[i] - delta);
+      }
+      if ((t + 1) * kKeys > tl.len) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (k0 + reg_row(i) >= tl.len) ds[i] = 0.f;
+      }
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        const s16x8 df = pack_step<T>(&ds[st * 8]);
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+          acc[db] = mfma32<T>(
+              tr_frag<DP>(lk, b * 32 + st * 16, db * 32, lane), df, acc[db]);
+      }
+    }
+  }
+  if (real)
+    store_rows<T, DP>(a.dq.p + token * a.dq.token + head * a.dq.head, acc,
+                      a.scale, a.dim, lane);
+}
+
+// ---------------------------------------------------------------------------
+// gradients of keys and values: a wave owns 32 keys of one key head; the
+// queries of every head that shares it pass in tiles of 64.
+// ---------------------------------------------------------------------------
+
+template <typename T, int DP, int NW, bool BIAS>
+__global__ __launch_bounds__(NW * 64) void doc_attn_dkv_kernel(AttnArgs a) {
+  constexpr int NT = NW * 64, ROWS = NW * 32, TS = kKeys * DP;
+  __shared__ __attribute__((aligned(16))) uint16_t lds[4 * TS];
+  __shared__ __attribute__((aligned(16))) float stat[2][2][kKeys];
+
+  const int kv_heads = a.heads / a.group;
+  const int tiles = gridDim.x / kv_heads;
+  const int bid = xcd_block(blockIdx.x, gridDim.x);
+  const int kvh = bid / tiles;
+  const Tile tl = find_tile<ROWS>(a, bid - kvh * tiles);
+  if (tl.row0 >= tl.len) return;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wid = threadIdx.x / kWave;
+  const int half = lane >> 5;
+  const int kpos = tl.row0 + wid * 32 + (lane & 31);
+  const bool real = kpos < tl.len;
+  if (!tl.doc) {
+    if (real) {
+      zero_rows<DP>(a.dk, tl.start + kpos, kvh, a.dim, lane);
+      zero_rows<DP>(a.dv, tl.start + kpos, kvh, a.dim, lane);
+    }
+    return;
+  }
+  const long token = tl.start + (real ? kpos : tl.len - 1);
+  const int nt = (tl.len + kKeys - 1) / kKeys;
+  const int all = nt * a.group;
+
+  // tile n of the walk: head kvh * group + n / nt, rows (n % nt) * 64..
+  auto stage = [&](int n) {
+    const int head = kvh * a.group + n / nt;
+    const int row0 = (n % nt) * kKeys;
+    uint16_t* at = lds + (n & 1) * 2 * TS;
+    load_tile<DP, NT>(at, a.q.p + tl.start * a.q.token + head * a.q.head,
+                      a.q.token, row0, tl.len, a.dim);
+    load_tile<DP, NT>(at + TS,
+                      a.dout.p + tl.start * a.dout.token + head * a.dout.head,
+                      a.dout.token, row0, tl.len, a.dim);
+    if (threadIdx.x < kKeys) {
+      // a query behind the document's end: exp2(x - inf) is 0
+      const int r = row0 + threadIdx.x;
+      const long i = (long)head * a.tokens + tl.start + r;
+      stat[n & 1][0][threadIdx.x] = r < tl.len ? a.lse[i] : INFINITY;
+      stat[n & 1][1][threadIdx.x] = r < tl.len ? a.delta[i] : 0.f;
+    }
+  };
+  stage(0);
+  s16x8 kf[DP / 16], vf[DP / 16];
+  load_rows<DP>(kf, a.k.p + token * a.k.token + kvh * a.k.head, a.dim, lane);
+  load_rows<DP>(vf, a.v.p + token * a.v.token + kvh * a.v.head, a.dim, lane);
+  const float sc = a.scale * kLog2e;
+  f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
+
+  for (int n = 0; n < all; ++n) {
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (n + 1 < all) stage(n + 1);
+    const uint16_t* lq = lds + (n & 1) * 2 * TS;
+    const uint16_t* lg = lq + TS;
+    const float sl =
+        BIAS ? a.slopes[kvh * a.group + n / nt] * kLog2e : 0.f;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      f32x16 s = {}, dp = {};
+#pragma unroll
+      for (int st = 0; st < DP / 16; ++st)
+        s = mfma32<T>(row_frag<DP>(lq, b * 32, st, lane), kf[st], s);
+#pragma unroll
+      for (int st = 0; st < DP / 16; ++st)
+        dp = mfma32<T>(row_frag<DP>(lg, b * 32, st, lane), vf[st], dp);
+      const int q0 = b * 32 + half * 4;
+      const float d0 = (float)((n % nt) * kKeys + q0 - kpos);
+      float p[16], ds[16];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const F32x4 ls =
+            *reinterpret_cast<const F32x4*>(&stat[n & 1][0][q0 + g * 8]);
+        const F32x4 de =
+            *reinterpret_cast<const F32x4*>(&stat[n & 1][1][q0 + g * 8]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = g * 4 + e;
+          float x = s[i] * sc - ls.v[e];
+          if (BIAS) x -= sl * fabsf(d0 + (float)reg_row(i));
+          p[i] = __builtin_amdgcn_exp2f(x);
+          ds[i] = p[i] * (dp[i] - de.v[e]);
+        }
+      }
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        const s16x8 pf = pack_step<T>(&p[st * 8]);
+        const s16x8 df = pack_step<T>(&ds[st * 8]);
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db) {
+          dv[db] = mfma32<T>(
+              tr_frag<DP>(lg, b * 32 + st * 16, db * 32, lane), pf, dv[db]);
+          dk[db] = mfma32<T>(
+              tr_frag<DP>(lq, b * 32 + st * 16, db * 32, lane), df, dk[db]);
+        }
+      }
+    }
+  }
+  if (!real) return;
+  store_rows<T, DP>(a.dk.p + token * a.dk.token + kvh * a.dk.head, dk, a.scale,
+                    a.dim, lane);
+  store_rows<T, DP>(a.dv.p + token * a.dv.token + kvh * a.dv.head, dv, 1.f,
+                    a.dim, lane);
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+
+// 16-byte rows at any stride: what the kernels' loads take.
+bool loadable(const at::Tensor& t) {
+  return t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
+         t.stride(0) >= 0 && t.stride(1) >= 0 &&
+         reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+}
+
+at::Tensor rows(const at::Tensor& t) {
+  return loadable(t) ? t : t.contiguous();
+}
+
+View view(const at::Tensor& t) {
+  return View{static_cast<uint16_t*>(t.data_ptr()), t.stride(0), t.stride(1)};
+}
+
+void check_inputs(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                  const at::Tensor& cu, const c10::optional<at::Tensor>& slopes,
+                  double scale) {
+  TORCH_CHECK(q.dim() == 3 && k.dim() == 3 && v.dim() == 3,
+              "document_attention: q, k and v are [tokens, heads, dim]");
+  TORCH_CHECK(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf,
+              "document_attention: bf16 or fp16 only, got ", q.scalar_type());
+  TORCH_CHECK(k.scalar_type() == q.scalar_type() &&
+                  v.scalar_type() == q.scalar_type(),
+              "document_attention: q, k and v differ in type");
+  TORCH_CHECK(k.sizes() == v.sizes() && k.size(0) == q.size(0) &&
+                  k.size(2) == q.size(2),
+              "document_attention: q/k/v shape mismatch");
+  TORCH_CHECK(k.size(1) > 0 && q.size(1) % k.size(1) == 0,
+              "document_attention: query heads have to be a multiple of key "
+              "heads");
+  TORCH_CHECK(q.size(2) % 8 == 0 && q.size(2) >= 8 && q.size(2) <= 128,
+              "document_attention: the head's width has to be a multiple of 8 "
+              "up to 128, got ", q.size(2));
+  TORCH_CHECK(q.size(0) < (1l << 30),
+              "document_attention: too many tokens");
+  TORCH_CHECK(cu.dim() == 1 && cu.numel() >= 1 &&
+                  cu.scalar_type() == at::kInt && cu.is_contiguous(),
+              "document_attention: cu_seqlens is a contiguous int32 vector");
+  TORCH_CHECK(k.device() == q.device() && v.device() == q.device() &&
+                  cu.device() == q.device(),
+              "document_attention: inputs on different devices");
+  if (slopes)
+    TORCH_CHECK(slopes->scalar_type() == at::kFloat && slopes->dim() == 1 &&
+                    slopes->size(0) == q.size(1) && slopes->is_contiguous() &&
+                    slopes->device() == q.device(),
+                "document_attention: slopes is a float32 vector, one a head");
+  TORCH_CHECK(std::isfinite(scale) && scale > 0,
+              "document_attention: scale has to be positive and finite");
+}
+
+void fill(AttnArgs& a, const at::Tensor& q, const at::Tensor& k,
+          const at::Tensor& v, const at::Tensor& cu,
+          const c10::optional<at::Tensor>& slopes, double scale) {
+  a.q = view(q);
+  a.k = view(k);
+  a.v = view(v);
+  a.cu = cu.data_ptr<int>();
+  a.slopes = slopes ? slopes->data_ptr<float>() : nullptr;
+  a.docs = (int)cu.numel() - 1;
+  a.tokens = (int)q.size(0);
+  a.heads = (int)q.size(1);
+  a.group = (int)(q.size(1) / k.size(1));
+  a.dim = (int)q.size(2);
+  a.scale = (float)scale;
+}
+
+unsigned blocks_of(const AttnArgs& a, int rows_, int heads) {
+  const long n = ((long)a.tokens / rows_ + a.docs + 2) * heads;
+  TORCH_CHECK(n <= std::numeric_limits<int>::max(),
+              "document_attention: too many tokens or documents");
+  return (unsigned)n;
+}
+
+enum { kFwd, kDq, kDkv };
+
+template <typename T, int DP, int NW, bool BIAS>
+void launch_one(int which, const AttnArgs& a, hipStream_t s) {
+  const unsigned b =
+      blocks_of(a, NW * 32, which == kDkv ? a.heads / a.group : a.heads);
+  if (which == kFwd)
+    doc_attn_fwd_kernel<T, DP, NW, BIAS><<<b, NW * 64, 0, s>>>(a);
+  else if (which == kDq)
+    doc_attn_dq_kernel<T, DP, NW, BIAS><<<b, NW * 64, 0, s>>>(a);
+  else
+    doc_attn_dkv_kernel<T, DP, NW, BIAS><<<b, NW * 64, 0, s>>>(a);
+}
+
+template <typename T, int DP>
+void launch_tile(int which, const AttnArgs& a, hipStream_t s) {
+  if (a.slopes)
+    launch_one<T, DP, 4, true>(which, a, s);
+  else
+    launch_one<T, DP, 4, false>(which, a, s);
+}
+
+void launch(int which, const AttnArgs& a, at::ScalarType t, hipStream_t s) {
+  if (t == at::kBFloat16) {
+    if (a.dim <= 64) launch_tile<BF16, 64>(which, a, s);
+    else launch_tile<BF16, 128>(which, a, s);
+  } else {
+    if (a.dim <= 64) launch_tile<FP16, 64>(which, a, s);
+    else launch_tile<FP16, 128>(which, a, s);
+  }
+}
+
+}  // namespace
+
+// q [T,H,D], k and v [T,Hkv,D] (rows at any stride), cu [docs+1] int32
+// -> (o [T,H,D], lse [H,T] fp32, base 2; empty without need_lse)
+std::tuple<at::Tensor, at::Tensor> doc_attn_fwd_impl(
+    const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
+    const at::Tensor& cu, const c10::optional<at::Tensor>& slopes, double scale,
+    bool need_lse) {
+  check_inputs(q_in, k_in, v_in, cu, slopes, scale);
+  const c10::DeviceGuard guard(q_in.device());
+  const auto q = rows(q_in), k = rows(k_in), v = rows(v_in);
+  auto o = at::empty(q.sizes(), q.options());
+  auto lse = at::empty({need_lse ? q.size(1) : 0, need_lse ? q.size(0) : 0},
+                       q.options().dtype(at::kFloat));
+  if (q.numel() == 0) return {o, lse};
+  AttnArgs a{};
+  fill(a, q, k, v, cu, slopes, scale);
+  a.o = view(o);
+  a.lse = need_lse ? lse.data_ptr<float>() : nullptr;
+  launch(kFwd, a, q.scalar_type(), at::cuda::getCurrentCUDAStream());
+  return {o, lse};
+}
+
+// dq, dk, dv: written whole, rows at any stride
+void doc_attn_bwd_impl(const at::Tensor& dout_in, const at::Tensor& q_in,
+                       const at::Tensor& k_in, const at::Tensor& v_in,
+                       const at::Tensor& o, const at::Tensor& lse,
+                       const at::Tensor& cu,
+                       const c10::optional<at::Tensor>& slopes, double scale,
+                       at::Tensor dq, at::Tensor dk, at::Tensor dv) {
+  check_inputs(q_in, k_in, v_in, cu, slopes, scale);
+  const c10::DeviceGuard guard(q_in.device());
+  TORCH_CHECK(dout_in.sizes() == q_in.sizes() &&
+                  dout_in.scalar_type() == q_in.scalar_type() &&
+                  dout_in.device() == q_in.device(),
+              "document_attention: the gradient differs from the output");
+  TORCH_CHECK(o.sizes() == q_in.sizes() && o.scalar_type() == q_in.scalar_type()
+                  && loadable(o) && lse.numel() == q_in.size(0) * q_in.size(1)
+                  && lse.scalar_type() == at::kFloat && lse.is_contiguous(),
+              "document_attention: o and lse are not the forward's");
+  TORCH_CHECK(dq.sizes() == q_in.sizes() && dk.sizes() == k_in.sizes() &&
+                  dv.sizes() == k_in.sizes() && loadable(dq) && loadable(dk) &&
+                  loadable(dv) && dq.scalar_type() == q_in.scalar_type() &&
+                  dk.scalar_type() == q_in.scalar_type() &&
+                  dv.scalar_type() == q_in.scalar_type() &&
+                  dq.device() == q_in.device() &&
+                  dk.device() == q_in.device() && dv.device() == q_in.device(),
+              "document_attention: dq, dk, dv do not fit q, k, v");
+  if (q_in.numel() == 0) return;
+  const auto q = rows(q_in), k = rows(k_in), v = rows(v_in);
+  const auto dout = rows(dout_in);
+  auto delta = at::empty({q.size(1), q.size(0)}, lse.options());
+  AttnArgs a{};
+  fill(a, q, k, v, cu, slopes, scale);
+  a.o = view(o);
+  a.dout = view(dout);
+  a.dq = view(dq);
+  a.dk = view(dk);
+  a.dv = view(dv);
+  a.lse = lse.data_ptr<float>();
+  a.delta = delta.data_ptr<float>();
+  const auto s = at::cuda::getCurrentCUDAStream();
+  launch(kDq, a, q.scalar_type(), s);
+  launch(kDkv, a, q.scalar_type(), s);
+}
+
+}  // namespace dlx

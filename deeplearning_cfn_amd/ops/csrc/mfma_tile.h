@@ -1,0 +1,109 @@
+// Matrix-instruction tiles of 16-bit elements, shared by document attention
+// and Newton-Schulz.
+//
+// v_mfma_f32_32x32x16, lane l of the 64, h = l >> 5:
+//   A[m][k]: m = l & 31, k = 8h + e            (e = 0..7, one 16-byte read)
+//   B[k][n]: n = l & 31, k = 8h + e
+//   C[m][n]: n = l & 31, m = 8 (i >> 2) + 4h + (i & 3)      (i = 0..15)
+// The order of k is free as long as A and B agree.  Taking it as
+//   k(e) = 8 (e >> 2) + 4h + (e & 3)
+// makes registers 8a..8a+7 of a result C the operand B of step a of a next
+// product whose k is C's m: a product's result feeds the next one without
+// leaving its lane.  The next product's A, read across its rows, is then two
+// transposing reads of four rows each (tr_frag).
+//
+// LDS tiles are rows of DP elements in chunks of 8, chunk c of row r stored
+// at place c ^ (r & 7): reads of 32 rows at one chunk (row_frag) and of 8
+// rows at 4 chunks (tr_frag) both touch every bank evenly.
+#pragma once
+
+#include "seq_common.h"
+
+namespace dlx {
+
+using f32x16 = __attribute__((ext_vector_type(16))) float;
+using s16x8 = __attribute__((ext_vector_type(8))) short;
+using s16x4 = __attribute__((ext_vector_type(4))) short;
+using bf16v4_t = __attribute__((ext_vector_type(4))) __bf16;
+using bf16v8_t = __attribute__((ext_vector_type(8))) __bf16;
+using f16v8_t = __attribute__((ext_vector_type(8))) _Float16;
+using bf16v2_t = __attribute__((ext_vector_type(2))) __bf16;
+using f16v2_t = __attribute__((ext_vector_type(2))) _Float16;
+using f32v2_t = __attribute__((ext_vector_type(2))) float;
+using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
+
+typedef __attribute__((address_space(3))) uint32_t lds_word_t;
+typedef const __attribute__((address_space(1))) uint32_t glb_word_t;
+typedef __attribute__((address_space(3))) bf16v4_t lds_tr_t;
+
+template <typename T> DLX_DEV f32x16 mfma32(s16x8 a, s16x8 b, f32x16 c);
+template <> DLX_DEV f32x16 mfma32<BF16>(s16x8 a, s16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+      __builtin_bit_cast(bf16v8_t, a), __builtin_bit_cast(bf16v8_t, b), c, 0, 0,
+      0);
+}
+template <> DLX_DEV f32x16 mfma32<FP16>(s16x8 a, s16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(
+      __builtin_bit_cast(f16v8_t, a), __builtin_bit_cast(f16v8_t, b), c, 0, 0,
+      0);
+}
+
+// two fp32 to two 16-bit, round to nearest even
+template <typename T> DLX_DEV uint32_t pack2(float a, float b);
+template <> DLX_DEV uint32_t pack2<BF16>(float a, float b) {
+  return __builtin_bit_cast(
+      uint32_t, __builtin_convertvector(f32v2_t{a, b}, bf16v2_t));
+}
+template <> DLX_DEV uint32_t pack2<FP16>(float a, float b) {
+  return __builtin_bit_cast(
+      uint32_t, __builtin_convertvector(f32v2_t{a, b}, f16v2_t));
+}
+
+// registers 8a..8a+7 of a result as the next product's operand B
+template <typename T> DLX_DEV s16x8 pack_step(const float* p) {
+  return __builtin_bit_cast(
+      s16x8, u32x4{pack2<T>(p[0], p[1]), pack2<T>(p[2], p[3]),
+                   pack2<T>(p[4], p[5]), pack2<T>(p[6], p[7])});
+}
+
+template <int DP> DLX_DEV int tile_at(int row, int chunk) {
+  return row * DP + ((chunk ^ (row & 7)) << 3);
+}
+
+// operand A or B of step `step`: rows row0.. along m or n, k along the row
+template <int DP>
+DLX_DEV s16x8 row_frag(const uint16_t* tile, int row0, int step, int lane) {
+  return *reinterpret_cast<const s16x8*>(
+      tile + tile_at<DP>(row0 + (lane & 31), step * 2 + (lane >> 5)));
+}
+
+// operand A (or B) whose m (n) runs along the tile's rows, columns col0..31,
+// and whose k runs over its rows row0..row0+15 in the order of pack_step
+template <int DP>
+DLX_DEV s16x8 tr_frag(const uint16_t* tile, int row0, int col0, int lane) {
+  const int col = col0 + (lane & 16) + ((lane & 3) << 2);
+  const int row = row0 + ((lane >> 5) << 2) + ((lane & 15) >> 2);
+  auto* lo = (lds_tr_t*)(tile + tile_at<DP>(row, col >> 3) + (col & 7));
+  auto* hi = (lds_tr_t*)(tile + tile_at<DP>(row + 8, col >> 3) + (col & 7));
+  const s16x4 a = __builtin_bit_cast(
+      s16x4, __builtin_amdgcn_ds_read_tr16_b64_v4bf16(lo));
+  const s16x4 b = __builtin_bit_cast(
+      s16x4, __builtin_amdgcn_ds_read_tr16_b64_v4bf16(hi));
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// 16 bytes a lane from memory to LDS, lanes one behind the other there
+DLX_DEV void copy16_to_lds(const void* src, uint16_t* dst) {
+  __builtin_amdgcn_global_load_lds((glb_word_t*)src, (lds_word_t*)dst, 16, 0,
+                                   0);
+}
+
+// The blocks of one stretch of the grid onto one XCD (blocks go round the
+// eight XCDs by number), so that neighbours share its L2.
+DLX_DEV int xcd_block(int bid, int blocks) {
+  const int q = blocks / 8, r = blocks % 8;
+  const int xcd = bid % 8, idx = bid / 8;
+  return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + idx;
+}
+
+}  // namespace dlx

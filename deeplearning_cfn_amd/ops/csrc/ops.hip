@@ -135,6 +135,29 @@ bn_fwd_train_res_presum_impl(
     at::Tensor& rmean, at::Tensor& rvar, double momentum, double eps,
     const at::Tensor& res, const at::Tensor& sums);
 
+// embedding.hip
+at::Tensor embed_sum_fwd_impl(at::TensorList ids, at::TensorList tables,
+                              at::ArrayRef<double> scales);
+std::vector<at::Tensor> embed_sum_bwd_impl(const at::Tensor& dy,
+                                           at::TensorList ids,
+                                           at::IntArrayRef rows,
+                                           at::ArrayRef<double> scales);
+
+// doc_attention.hip
+std::tuple<at::Tensor, at::Tensor> doc_attn_fwd_impl(
+    const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+    const at::Tensor& cu, const c10::optional<at::Tensor>& slopes,
+    double scale, bool need_lse);
+void doc_attn_bwd_impl(const at::Tensor& dout, const at::Tensor& q,
+                       const at::Tensor& k, const at::Tensor& v,
+                       const at::Tensor& o, const at::Tensor& lse,
+                       const at::Tensor& cu,
+                       const c10::optional<at::Tensor>& slopes, double scale,
+                       at::Tensor dq, at::Tensor dk, at::Tensor dv);
+
+// newton_schulz.hip
+at::Tensor newton_schulz_impl(const at::Tensor& g, int64_t steps, double eps);
+
 namespace {
 
 hipStream_t cur_stream() { return at::cuda::getCurrentCUDAStream(); }
@@ -306,6 +329,11 @@ TORCH_LIBRARY(dlx_hip, m) {
   m.def("gelu_bwd(Tensor g, Tensor x) -> Tensor");
   m.def("attn_fwd(Tensor q, Tensor k, Tensor v, float scale) -> (Tensor, Tensor)");
   m.def("attn_bwd(Tensor grad, Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, float scale) -> (Tensor, Tensor, Tensor)");
+  m.def("embed_sum_fwd(Tensor[] ids, Tensor[] tables, float[] scales) -> Tensor");
+  m.def("embed_sum_bwd(Tensor dy, Tensor[] ids, int[] rows, float[] scales) -> Tensor[]");
+  m.def("doc_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor cu, Tensor? slopes, float scale, bool need_lse) -> (Tensor, Tensor)");
+  m.def("doc_attn_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, Tensor cu, Tensor? slopes, float scale, Tensor(a!) dq, Tensor(b!) dk, Tensor(c!) dv) -> ()");
+  m.def("newton_schulz(Tensor g, int steps, float eps) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(dlx_hip, CUDA, m) {
@@ -349,4 +377,9 @@ TORCH_LIBRARY_IMPL(dlx_hip, CUDA, m) {
   m.impl("gelu_bwd", dlx::gelu_bwd_impl);
   m.impl("attn_fwd", dlx::attn_fwd_impl);
   m.impl("attn_bwd", dlx::attn_bwd_impl);
+  m.impl("embed_sum_fwd", dlx::embed_sum_fwd_impl);
+  m.impl("embed_sum_bwd", dlx::embed_sum_bwd_impl);
+  m.impl("doc_attn_fwd", dlx::doc_attn_fwd_impl);
+  m.impl("doc_attn_bwd", dlx::doc_attn_bwd_impl);
+  m.impl("newton_schulz", dlx::newton_schulz_impl);
 }

@@ -7,10 +7,12 @@ implementation of the same op), the HIP path is the production one.
 
 from __future__ import annotations
 
-from typing import Optional
+import math
+from typing import Optional, Sequence
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import native, native_available
 
@@ -624,3 +626,263 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     s = (q @ k.transpose(-1, -2)) * scale
     p = torch.softmax(s.float(), dim=-1).to(q.dtype)
     return p @ v
+
+
+# ---------------------------------------------------------------------------
+# embedding lookup: scaled sum of tables' rows, gradient by sorted tokens
+# (embedding.hip)
+# ---------------------------------------------------------------------------
+
+class _EmbeddingSum(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, scales, *tables):
+        ctx.ids, ctx.scales = ids, scales
+        ctx.rows = [w.shape[0] for w in tables]
+        y = native().embed_sum_fwd(ids, tables, scales)
+        return y.view(*ids[0].shape, tables[0].shape[1])
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        want = [i for i in range(len(ctx.rows)) if ctx.needs_input_grad[2 + i]]
+        grads = [None] * len(ctx.rows)
+        if want:
+            got = native().embed_sum_bwd(
+                grad.reshape(-1, grad.shape[-1]), [ctx.ids[i] for i in want],
+                [ctx.rows[i] for i in want], [ctx.scales[i] for i in want])
+            for i, g in zip(want, got):
+                grads[i] = g
+        return (None, None, *grads)
+
+
+def embedding_sum(ids: Sequence[torch.Tensor], tables: Sequence[torch.Tensor],
+                  scales: Optional[Sequence[float]] = None) -> torch.Tensor:
+    """``sum_j scales[j] * tables[j][ids[j]]`` for one to four tables.
+
+    ``ids``: int32 or int64 tensors of one shape; ``tables``: [rows_j, width]
+    of one type (bf16, fp16, fp32).  The sum is taken in fp32 and rounded
+    once.  A table's gradient adds its tokens in their order in fp32, so it
+    is the same from run to run.  On the GPU an id outside its table gives a
+    row of NaN and takes no part in the gradient (on the CPU it raises).
+    """
+    ids, tables = list(ids), list(tables)
+    scales = [1.0] * len(tables) if scales is None else [float(c)
+                                                         for c in scales]
+    if not 1 <= len(tables) <= 4:
+        raise ValueError(f"embedding_sum: 1 to 4 tables, got {len(tables)}")
+    if len(ids) != len(tables) or len(scales) != len(tables):
+        raise ValueError("embedding_sum: as many ids and scales as tables")
+    w0 = tables[0]
+    for i, w in zip(ids, tables):
+        if i.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"embedding_sum: ids are int32 or int64, got "
+                             f"{i.dtype}")
+        if i.shape != ids[0].shape:
+            raise ValueError("embedding_sum: the ids differ in shape")
+        if w.dim() != 2 or w.shape[1] != w0.shape[1] or w.dtype != w0.dtype:
+            raise ValueError("embedding_sum: tables are [rows, width], of one "
+                             "width and type")
+        if i.device != w0.device or w.device != w0.device:
+            raise ValueError("embedding_sum: ids and tables are on different "
+                             "devices")
+    if _use_native(w0) and w0.dtype in (torch.bfloat16, torch.float16,
+                                        torch.float32):
+        return _EmbeddingSum.apply(ids, scales, *tables)
+    acc = sum(F.embedding(i, w).float() * c
+              for i, w, c in zip(ids, tables, scales))
+    return acc.to(w0.dtype)
+
+
+def embedding(ids: torch.Tensor, weight: torch.Tensor,
+              scale: float = 1.0) -> torch.Tensor:
+    """``scale * weight[ids]``: ``embedding_sum`` of one table."""
+    return embedding_sum([ids], [weight], [scale])
+
+
+# ---------------------------------------------------------------------------
+# attention inside packed documents (doc_attention.hip)
+# ---------------------------------------------------------------------------
+
+class _DocAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, cu, slopes, scale):
+        o, lse = native().doc_attn_fwd(q, k, v, cu, slopes, scale,
+                                       any(ctx.needs_input_grad))
+        ctx.save_for_backward(q, k, v, o, lse, cu, slopes)
+        ctx.scale = scale
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        q, k, v, o, lse, cu, slopes = ctx.saved_tensors
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device)
+                      for t in (q, k, v))
+        native().doc_attn_bwd(grad, q, k, v, o, lse, cu, slopes, ctx.scale,
+                              dq, dk, dv)
+        return dq, dk, dv, None, None, None
+
+
+class _DocAttentionQKV(torch.autograd.Function):
+    """The same on one projection's output: its gradient is written in place
+    of the projection's, with no slices to put together."""
+
+    @staticmethod
+    def forward(ctx, qkv, cu, slopes, scale):
+        q, k, v = qkv.unbind(1)
+        o, lse = native().doc_attn_fwd(q, k, v, cu, slopes, scale,
+                                       any(ctx.needs_input_grad))
+        ctx.save_for_backward(qkv, o, lse, cu, slopes)
+        ctx.scale = scale
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        qkv, o, lse, cu, slopes = ctx.saved_tensors
+        d = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+        native().doc_attn_bwd(grad, *qkv.unbind(1), o, lse, cu, slopes,
+                              ctx.scale, *d.unbind(1))
+        return d, None, None, None
+
+
+def _doc_attention_args(name, q, k, cu, scale, slopes):
+    if cu.dim() != 1 or cu.numel() < 1 or cu.dtype not in (torch.int32,
+                                                           torch.int64):
+        raise ValueError(f"{name}: cu_seqlens is a vector of int32 or int64")
+    if k.shape[1] < 1 or q.shape[1] % k.shape[1]:
+        raise ValueError(f"{name}: query heads have to be a multiple of key "
+                         f"heads, got {q.shape[1]} and {k.shape[1]}")
+    if cu.device != q.device:
+        raise ValueError(f"{name}: cu_seqlens is on another device")
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    if not (math.isfinite(scale) and scale > 0):
+        raise ValueError(f"{name}: scale has to be positive and finite")
+    if slopes is not None:
+        if slopes.requires_grad:
+            raise ValueError(f"{name}: slopes are constants, they get no "
+                             "gradient")
+        if slopes.shape != (q.shape[1],) or slopes.device != q.device:
+            raise ValueError(f"{name}: slopes has one number a query head, "
+                             "on the same device")
+        slopes = slopes.float().contiguous()
+    return cu.to(torch.int32).contiguous(), scale, slopes
+
+
+def _doc_attention_native(t: torch.Tensor) -> bool:
+    return (_use_native(t) and t.dtype in (torch.bfloat16, torch.float16)
+            and t.shape[-1] % 8 == 0 and 8 <= t.shape[-1] <= 128)
+
+
+def _doc_attention_composed(q, k, v, cu, scale, slopes):
+    """A document at a time in fp32; reads the borders on the host."""
+    ends = cu.clamp(0, q.shape[0]).tolist()
+    group = q.shape[1] // k.shape[1]
+    parts, at = [], 0
+    for a, b in zip(ends[:-1], ends[1:]):
+        if a > at:
+            parts.append(q.new_zeros(a - at, *q.shape[1:]))
+        if b > a:
+            qd, kd, vd = (t[a:b].float().transpose(0, 1) for t in (q, k, v))
+            kd, vd = (t.repeat_interleave(group, 0) for t in (kd, vd))
+            s = (qd @ kd.transpose(1, 2).contiguous()) * scale
+            if slopes is not None:
+                i = torch.arange(b - a, device=q.device, dtype=torch.float32)
+                s = s - slopes[:, None, None] * (i[:, None] - i).abs()
+            parts.append((torch.softmax(s, -1) @ vd).transpose(0, 1)
+                         .to(q.dtype))
+        at = max(at, b)
+    if at < q.shape[0] or not parts:
+        parts.append(q.new_zeros(q.shape[0] - at, *q.shape[1:]))
+    return torch.cat(parts)
+
+
+def document_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                       cu_seqlens: torch.Tensor,
+                       scale: Optional[float] = None,
+                       slopes: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention inside documents that lie one behind the other.
+
+    ``q`` [tokens, heads, dim], ``k`` and ``v`` [tokens, kv_heads, dim] (heads
+    a multiple of kv_heads; neighbouring query heads share one).
+    ``cu_seqlens`` [documents + 1]: document i is the tokens from
+    ``cu_seqlens[i]`` to ``cu_seqlens[i + 1]``, in rising order; empty ones
+    are allowed.  Tokens in no document get zeros, and zero gradients.
+    ``scale`` (default dim ** -0.5) is positive.  ``slopes`` [heads] takes
+    ``slopes[h] * |i - j|`` off the scores; it gets no gradient.
+
+    Fused CDNA4 kernels for bf16 and fp16 with dim a multiple of 8 up to 128;
+    anything else runs document by document in torch, in fp32.
+    """
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or \
+            k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+        raise ValueError(
+            "document_attention: q is [tokens, heads, dim], k and v "
+            f"[tokens, kv_heads, dim], got {tuple(q.shape)}, "
+            f"{tuple(k.shape)}, {tuple(v.shape)}")
+    if not q.dtype == k.dtype == v.dtype:
+        raise ValueError("document_attention: q, k and v differ in type")
+    cu, scale, slopes = _doc_attention_args("document_attention", q, k,
+                                            cu_seqlens, scale, slopes)
+    if _doc_attention_native(q):
+        return _DocAttention.apply(q, k, v, cu, slopes, scale)
+    return _doc_attention_composed(q, k, v, cu, scale, slopes)
+
+
+def document_attention_qkv(qkv: torch.Tensor, cu_seqlens: torch.Tensor,
+                           scale: Optional[float] = None,
+                           slopes: Optional[torch.Tensor] = None
+                           ) -> torch.Tensor:
+    """``document_attention`` of one projection's output [tokens, 3, heads,
+    dim]; its gradient comes in the same layout."""
+    if qkv.dim() != 4 or qkv.shape[1] != 3:
+        raise ValueError("document_attention_qkv: [tokens, 3, heads, dim] "
+                         f"expected, got {tuple(qkv.shape)}")
+    q, k, v = qkv.unbind(1)
+    cu, scale, slopes = _doc_attention_args("document_attention_qkv", q, k,
+                                            cu_seqlens, scale, slopes)
+    if _doc_attention_native(qkv):
+        return _DocAttentionQKV.apply(qkv, cu, slopes, scale)
+    return _doc_attention_composed(q, k, v, cu, scale, slopes)
+
+
+# ---------------------------------------------------------------------------
+# Newton-Schulz orthogonalisation (the Muon update; newton_schulz.hip)
+# ---------------------------------------------------------------------------
+
+NS_COEFFS = (3.4445, -4.7750, 2.0315)
+
+
+def newton_schulz(g: torch.Tensor, steps: int = 5,
+                  eps: float = 1e-7) -> torch.Tensor:
+    """Orthogonalises each matrix of ``g`` [..., rows, cols] by ``steps``
+    products ``X <- a X + (b A + c A A) X``, ``A = X X^T``, from
+    ``X = g / (|g| + eps)``; the result, in bf16, has singular values near 1.
+
+    ``g`` is fp32, bf16 or fp16.  Matrices of a batch share their launches.
+    The products take fp16 operands with fp32 sums; X itself is carried in 22
+    bits.  A zero matrix stays zero.  Gives no gradient.
+    """
+    if g.dim() < 2 or not g.is_floating_point():
+        raise ValueError("newton_schulz: a floating [..., rows, cols] "
+                         f"expected, got {tuple(g.shape)} {g.dtype}")
+    if not 1 <= steps <= 100:
+        raise ValueError(f"newton_schulz: 1 to 100 steps, got {steps}")
+    if not (math.isfinite(eps) and eps >= 0):
+        raise ValueError("newton_schulz: eps has to be finite and not "
+                         "negative")
+    g = g.detach()
+    x = g.reshape(-1, *g.shape[-2:])
+    if _use_native(g) and g.dtype in (torch.float32, torch.bfloat16,
+                                      torch.float16):
+        return native().newton_schulz(x, steps, eps).view(g.shape)
+    a, b, c = NS_COEFFS
+    tall = x.shape[1] > x.shape[2]
+    x = (x.transpose(1, 2) if tall else x).float().contiguous()
+    norm = x.double().square().sum((1, 2), keepdim=True).sqrt() + eps
+    x = (x / norm).float()
+    for _ in range(steps):
+        s = x @ x.transpose(1, 2).contiguous()
+        x = a * x + (b * s + c * (s @ s)) @ x
+    x = x.transpose(1, 2) if tall else x
+    return x.to(torch.bfloat16).reshape(g.shape)
