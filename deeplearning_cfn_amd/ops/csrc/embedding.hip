@@ -9,14 +9,18 @@
 //
 // The gradient sorts the tokens by id and sums each row's tokens in that
 // order, so every bit is the same from run to run (no float atomics).
-//   1. embed_sort: a block owns a range of ids and looks at ALL tokens; the
-//      tokens with smaller ids, counted on the way, are the place where its
-//      own begin, so no block waits for another and one launch sorts.  It
-//      reads the ids once a block (from L2), which costs less than the
-//      launches of a many-pass sort up to about a hundred thousand tokens.
-//   2. embed_grad: a wave sums a row of few tokens; a row of kHeavy or more
-//      (a mask token, a segment) is cut into pieces, a block each, and the
-//      piece that ends last adds them up in their order.
+//   1. Tokens into buckets, id % G (frequent ids are neighbours in a
+//      vocabulary, so this spreads them): embed_count counts each of up to
+//      64 chunks of the tokens, embed_scatter turns the counts into places
+//      and puts every token into its bucket.
+//   2. embed_order sorts a bucket by the rest of the id, id / G, a block each.
+//   3. embed_grad: a wave sums some rows of few tokens; a row of kHeavy or
+//      more (a mask token, a segment) is cut into pieces, a block each.
+//   4. embed_join adds up the pieces of a row, in their order.  (One block
+//      of the third launch could, the last to finish; but the fence it needs
+//      writes back its XCD's whole L2: 81 us instead of 41 for 16384 tokens
+//      of 768 in three tables.)
+// An id's "place" below is its number in that order, (id % G) * own + id / G.
 //
 // An id outside its table reads nothing: its output row is NaN, and it
 // takes no part in the gradient.
@@ -34,11 +38,14 @@ namespace {
 constexpr int kMaxTables = 4;
 constexpr int kSortThreads = 1024;
 constexpr int kSortWaves = kSortThreads / kWave;
-constexpr int kMaxOwn = 2048;     // ids a sort block owns: 128 KiB of counts
-constexpr int kHeavy = 64;        // tokens from which a row is cut in pieces
-constexpr int kSlotUnit = 32;     // sorted positions to a piece's slot
-constexpr int kMinPiece = 128;    // tokens of a piece
+constexpr int kChunks = 64;       // chunks of the tokens, at most
+constexpr int kMaxSplit = 11;     // log2 of the buckets, and of a bucket's ids
+constexpr int kMaxOwn = 1 << kMaxSplit;
+constexpr int kHeavy = 32;        // tokens from which a row is cut in pieces
+constexpr int kSlotUnit = 16;     // sorted positions to a piece's slot
+constexpr int kPiece = 128;       // tokens of a piece, at least
 constexpr int kMaxPieces = 256;   // pieces of a row
+constexpr int kLightRows = 4;     // rows of few tokens to a wave
 
 struct LookupTable {
   const void* ids;
@@ -56,6 +63,13 @@ struct LookupArgs {
 DLX_DEV long read_id(const void* ids, int ids64, long i) {
   return ids64 ? static_cast<const int64_t*>(ids)[i]
                : static_cast<const int32_t*>(ids)[i];
+}
+
+// An id as 32 bits without a sign; all ones where it fits no table.
+DLX_DEV uint32_t read_id32(const void* ids, int ids64, long i) {
+  if (!ids64) return static_cast<const uint32_t*>(ids)[i];
+  const uint2 x = static_cast<const uint2*>(ids)[i];
+  return x.y ? 0xffffffffu : x.x;
 }
 
 // Four vectors of a token's row a thread, `tokens` tokens a block.
@@ -94,75 +108,227 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(
 struct GradTable {
   const void* ids;
   void* out;            // [rows, width]
+  int* count;           // [buckets, kChunks] tokens
+  int* start;           // [buckets + 1] sorted position where one begins
+  int2* loose;          // [n] tokens in buckets, with id / G
   int* order;           // [n] token of each sorted position
-  int* first;           // [rows + 1] sorted position where a row begins
-  int* slot_row;        // [slots] row of a piece, -1: none
-  int* done;            // [slots] pieces of a row that are summed
+  int* first;           // [places + 1] sorted position where a place begins
+  int* slot_row;        // [slots] place of a piece, -1: none
+  int* join_row;        // [joins] place whose pieces are added up, -1: none
   float* part;          // [slots, width]
   float scale;
   int ids64;
   int rows;
-  int own;              // ids a sort block owns
-  int sort0;            // first sort block
+  int own;              // ids of a bucket
+  int lg;               // log2 of the buckets, G
+  int bucket0;          // first block of embed_order
   int light0;           // first block of rows of few tokens
 };
 
 struct GradArgs {
   GradTable t[kMaxTables];
   int n;
-  int slots;            // a table
+  int slots, joins;     // a table
 };
+
+DLX_DEV int place_id(const GradTable& t, int place) {
+  const int b = place / t.own;
+  return b + ((place - b * t.own) << t.lg);
+}
 
 DLX_DEV int piece_tokens(int count) {
   int p = (count + kMaxPieces - 1) / kMaxPieces;
-  return p < kMinPiece ? kMinPiece : p;
+  return p < kPiece ? kPiece : p;
 }
 
-// LDS: counts [wave][own], then 2 * kSortWaves scratch ints.
-__global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(
-    GradArgs a, int n) {
+// The lanes of `any` whose number is mine.  The first two numbers are looked
+// for one by one (a frequent id fills a bucket nearly alone), the others bit
+// by bit.
+DLX_DEV uint64_t peers(int r, uint64_t any, int bits) {
+  uint64_t same = 0, left = any;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    if (!left) return same;
+    const int f = __ffsll((unsigned long long)left) - 1;
+    const bool me = r == __builtin_amdgcn_readlane(r, f);
+    const uint64_t m = __ballot(me) & any;
+    if (me) same = m;
+    left &= ~m;
+  }
+  if (!left) return same;
+  uint64_t rest = left;
+  for (int b = 0; b < bits; ++b) {
+    const uint64_t one = __ballot((r >> b) & 1);
+    rest &= (r >> b) & 1 ? one : ~one;
+  }
+  const uint64_t bit = 1ull << (threadIdx.x & (kWave - 1));
+  return left & bit ? rest : same;
+}
+
+// Block (c, j): the tokens of chunk c in each bucket of table j.
+__global__ __launch_bounds__(kSortThreads) void embed_count_kernel(
+    GradArgs a, int n, int chunk) {
+  __shared__ int h[kMaxOwn];
+  const GradTable& tb = a.t[blockIdx.y];
+  const int g = 1 << tb.lg;
+  for (int i = threadIdx.x; i < g; i += kSortThreads) h[i] = 0;
+  __syncthreads();
+  const int i0 = blockIdx.x * chunk;
+  const int i1 = n - i0 < chunk ? n : i0 + chunk;
+  for (int i = i0 + threadIdx.x; i < i1; i += kSortThreads) {
+    const uint32_t id = read_id32(tb.ids, tb.ids64, i);
+    if (id < (uint32_t)tb.rows) atomicAdd(h + (id & (g - 1)), 1);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < g; i += kSortThreads)
+    tb.count[i * kChunks + blockIdx.x] = h[i];
+}
+
+// Exclusive sum over a block of kSortThreads; scratch: kSortWaves ints.
+DLX_DEV int block_scan(int x, int* scratch) {
+  const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
+  int s = x;
+  for (int off = 1; off < kWave; off <<= 1) {
+    const int up = __shfl_up(s, off, kWave);
+    if (lane >= off) s += up;
+  }
+  if (lane == kWave - 1) scratch[w] = s;
+  __syncthreads();
+  int base = s - x;
+  for (int i = 0; i < w; ++i) base += scratch[i];
+  __syncthreads();
+  return base;
+}
+
+// Block (c, j): the tokens of chunk c into table j's buckets.
+// LDS: counts [wave][bucket], then scratch.
+__global__ __launch_bounds__(kSortThreads) void embed_scatter_kernel(
+    GradArgs a, int n, int chunk, int chunks) {
+  extern __shared__ int lds[];
+  const GradTable& tb = a.t[blockIdx.y];
+  const int g = 1 << tb.lg, bits = tb.lg;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  volatile int* cnt = lds + w * g;
+  int* scratch = lds + kSortWaves * g;
+  const int me = blockIdx.x;
+  for (int i = threadIdx.x; i < kSortWaves * g; i += kSortThreads) lds[i] = 0;
+  __syncthreads();
+
+  const int i0 = me * chunk;
+  const int i1 = n - i0 < chunk ? n : i0 + chunk;
+  for (int i = i0 + w * kWave; i < i1; i += kSortThreads) {
+    const uint32_t id =
+        i + lane < i1 ? read_id32(tb.ids, tb.ids64, i + lane) : 0xffffffffu;
+    const bool in = id < (uint32_t)tb.rows;
+    const int r = in ? (int)(id & (g - 1)) : 0;
+    const uint64_t same = peers(r, __ballot(in), bits);
+    if (in && !(same & ((1ull << lane) - 1))) cnt[r] = cnt[r] + __popcll(same);
+  }
+  __syncthreads();
+
+  // two buckets a thread: all chunks' tokens, and those of chunks before me
+  constexpr int PER = kMaxOwn / kSortThreads;
+  int total[PER], before[PER], sum = 0;
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    const int r = threadIdx.x * PER + u;
+    total[u] = before[u] = 0;
+    if (r < g) {
+      const int4* p = reinterpret_cast<const int4*>(tb.count + r * kChunks);
+      for (int c = 0; c < chunks; c += 4) {
+        const int4 x = p[c / 4];
+        const int y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (c + e < chunks) total[u] += y[e];
+          if (c + e < me) before[u] += y[e];
+        }
+      }
+    }
+    sum += total[u];
+  }
+  int base = block_scan(sum, scratch);
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    const int r = threadIdx.x * PER + u;
+    if (r < g) {
+      if (me == 0) tb.start[r] = base;
+      int at = base + before[u];
+      for (int i = 0; i < kSortWaves; ++i) {
+        const int c = lds[i * g + r];
+        lds[i * g + r] = at;
+        at += c;
+      }
+      if (me == 0 && r == g - 1) tb.start[g] = base + total[u];
+    }
+    base += total[u];
+  }
+  __syncthreads();
+
+  for (int i = i0 + w * kWave; i < i1; i += kSortThreads) {
+    const uint32_t id =
+        i + lane < i1 ? read_id32(tb.ids, tb.ids64, i + lane) : 0xffffffffu;
+    const bool in = id < (uint32_t)tb.rows;
+    const int r = in ? (int)(id & (g - 1)) : 0;
+    const uint64_t same = peers(r, __ballot(in), bits);
+    if (in) {
+      const uint64_t first = same & ((1ull << lane) - 1);
+      const int at = cnt[r];
+      tb.loose[at + __popcll(first)] = make_int2(i + lane, (int)(id >> bits));
+      if (!first) cnt[r] = at + __popcll(same);
+    }
+  }
+}
+
+DLX_DEV int2 loose_at(const GradTable& t, int i, int end) {
+  int2 x = t.loose[i < end ? i : end - 1];
+  if (i >= end) x.y = -1;
+  return x;
+}
+
+// A bucket's tokens by id / G.  LDS: counts [wave][own], then scratch.
+__global__ __launch_bounds__(kSortThreads) void embed_order_kernel(GradArgs a) {
   extern __shared__ int lds[];
   int j = 0;
-  while (j + 1 < a.n && (int)blockIdx.x >= a.t[j + 1].sort0) ++j;
+  while (j + 1 < a.n && (int)blockIdx.x >= a.t[j + 1].bucket0) ++j;
   const GradTable& tb = a.t[j];
   const int own = tb.own;
-  const int lo = ((int)blockIdx.x - tb.sort0) * own;
-  const int hi = lo + own < tb.rows ? lo + own : tb.rows;
+  const int me = (int)blockIdx.x - tb.bucket0;
+  const int lo = me * own;
+  const bool top = me == (1 << tb.lg) - 1;
   const int lane = threadIdx.x & (kWave - 1);
-  const int w = threadIdx.x / kWave;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   volatile int* cnt = lds + w * own;
   int* scratch = lds + kSortWaves * own;
-
   for (int i = threadIdx.x; i < kSortWaves * own; i += kSortThreads)
     lds[i] = 0;
   __syncthreads();
 
-  // a wave's own stretch of the tokens, in whole steps of 64
-  const int seg = (n + kSortThreads - 1) / kSortThreads * kWave;
-  const int s0 = w * seg;
-  const int s1 = s0 + seg < n ? s0 + seg : n;
-  int less = 0;
+  const int start = __builtin_amdgcn_readfirstlane(tb.start[me]);
+  const int end = __builtin_amdgcn_readfirstlane(tb.start[me + 1]);
+  // a wave's own stretch; U times 64 tokens of it on their way
   constexpr int U = 4;
-  for (int i0 = s0; i0 < s1; i0 += U * kWave) {
-    long id[U];
+  const int seg = (end - start + kSortThreads - 1) / kSortThreads * kWave;
+  const int s0 = start + w * seg < end ? start + w * seg : end;
+  const int s1 = s0 + seg < end ? s0 + seg : end;
+  const int bits = own > 1 ? 32 - __clz(own - 1) : 0;
+  for (int i = s0; i < s1; i += U * kWave) {
+    int2 x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = loose_at(tb, i + u * kWave + lane, s1);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * kWave + lane;
-      id[u] = i < s1 ? read_id(tb.ids, tb.ids64, i) : -1;
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      less += __popcll(__ballot(id[u] >= 0 && id[u] < lo));
-      if (id[u] >= lo && id[u] < hi)
-        atomicAdd(lds + w * own + (int)(id[u] - lo), 1);
+      const int r = x[u].y;
+      const uint64_t any = __ballot(r >= 0);
+      if (!any) break;
+      const uint64_t same = peers(r, any, bits);
+      if (r >= 0 && !(same & ((1ull << lane) - 1)))
+        cnt[r] = cnt[r] + __popcll(same);
     }
   }
-  if (lane == 0) scratch[w] = less;
   __syncthreads();
-  int start = 0;
-  for (int i = 0; i < kSortWaves; ++i) start += scratch[i];
 
-  // exclusive scan over (row, wave); two rows a thread
   constexpr int PER = kMaxOwn / kSortThreads;
   int mine[PER], sum = 0;
 #pragma unroll
@@ -173,36 +339,29 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(
       for (int i = 0; i < kSortWaves; ++i) mine[u] += lds[i * own + r];
     sum += mine[u];
   }
-  int scan = sum;
-  for (int off = 1; off < kWave; off <<= 1) {
-    const int up = __shfl_up(scan, off, kWave);
-    if (lane >= off) scan += up;
-  }
-  if (lane == kWave - 1) scratch[kSortWaves + w] = scan;
-  __syncthreads();
-  int base = start + scan - sum, end = start;
-  for (int i = 0; i < kSortWaves; ++i) {
-    if (i < w) base += scratch[kSortWaves + i];
-    end += scratch[kSortWaves + i];
-  }
-  const int z0 = start / kSlotUnit;
-  const int z1 = hi == tb.rows ? a.slots : end / kSlotUnit;
-  for (int i = z0 + threadIdx.x; i < z1; i += kSortThreads) {
+  int base = start + block_scan(sum, scratch);
+  // this block's pieces' slots: those that begin between its borders
+  const int z1 = top ? a.slots : end / kSlotUnit;
+  for (int i = start / kSlotUnit + threadIdx.x; i < z1; i += kSortThreads)
     tb.slot_row[i] = -1;
-    tb.done[i] = 0;
-  }
+  // a row of more than one piece owns the first multiple of kPiece in it
+  const int y1 = top ? a.joins : (end + kPiece - 1) / kPiece;
+  for (int i = (start + kPiece - 1) / kPiece + threadIdx.x; i < y1;
+       i += kSortThreads)
+    tb.join_row[i] = -1;
   __syncthreads();
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
     const int r = threadIdx.x * PER + u;
-    if (r < own && lo + r < hi) {
+    if (r < own) {
       tb.first[lo + r] = base;
       if (mine[u] >= kHeavy) {
-        // count / 32 slots lie inside the row, its pieces are fewer
+        // count / 16 slots lie inside the row, its pieces are fewer
         const int p = piece_tokens(mine[u]);
         const int k1 = (mine[u] + p - 1) / p;
         for (int k = 0; k < k1; ++k)
           tb.slot_row[base / kSlotUnit + k] = lo + r;
+        if (k1 > 1) tb.join_row[(base + kPiece - 1) / kPiece] = lo + r;
       }
       int at = base;
       for (int i = 0; i < kSortWaves; ++i) {
@@ -213,100 +372,137 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(
       base += mine[u];
     }
   }
-  if (hi == tb.rows && threadIdx.x == 0) tb.first[tb.rows] = end;
+  if (top && threadIdx.x == 0) tb.first[lo + own] = end;
   __syncthreads();
 
-  // again over the tokens: lanes of the same id take their places in order
-  for (int i0 = s0; i0 < s1; i0 += U * kWave) {
-    long id[U];
+  for (int i = s0; i < s1; i += U * kWave) {
+    int2 x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = loose_at(tb, i + u * kWave + lane, s1);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * kWave + lane;
-      id[u] = i < s1 ? read_id(tb.ids, tb.ids64, i) : -1;
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool in = id[u] >= lo && id[u] < hi;
-      const int r = in ? (int)(id[u] - lo) : -1;
-      uint64_t left = __ballot(in);
-      while (left) {
-        const int f = __ffsll((unsigned long long)left) - 1;
-        const int rf = __shfl(r, f, kWave);
-        const uint64_t same = __ballot(r == rf);
-        const int at = cnt[rf];
-        if (r == rf)
-          tb.order[at + __popcll(same & ((1ull << lane) - 1))] =
-              i0 + u * kWave + lane;
-        if (lane == f) cnt[rf] = at + __popcll(same);
-        left &= ~same;
+      const int r = x[u].y;
+      const uint64_t any = __ballot(r >= 0);
+      if (!any) break;
+      const uint64_t same = peers(r, any, bits);
+      if (r >= 0) {
+        const uint64_t first = same & ((1ull << lane) - 1);
+        const int at = cnt[r];
+        tb.order[at + __popcll(first)] = x[u].x;
+        if (!first) cnt[r] = at + __popcll(same);
       }
     }
   }
 }
 
-// The sum of tokens order[p0..p1) of dy, columns c..c+VEC.  p1 - p0 <= 64 a
-// turn: a lane holds one token's number and hands it to the others.
+constexpr int kFlight = 8;          // rows on their way at a time
+
+// The sum of tokens order[p0..p1), VEC columns at `from` in token 0.  64
+// tokens a turn: a lane holds one token's number and hands it to the others.
 template <typename T, int VEC>
-DLX_DEV void sum_tokens(const T* __restrict__ dy, const int* __restrict__ order,
-                        int p0, int p1, int width, int c, bool on, int lane,
-                        float* acc) {
+DLX_DEV void sum_tokens(const T* __restrict__ from,
+                        const int* __restrict__ order, int p0, int p1,
+                        int width, int lane, float* acc) {
 #pragma unroll
   for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
   for (int q = p0; q < p1; q += kWave) {
     const int m = p1 - q < kWave ? p1 - q : kWave;
     const int tok = lane < m ? order[q + lane] : 0;
-    int k = 0;
-    for (; k + 8 <= m; k += 8) {
-      float x[8][VEC];
+    for (int k = 0; k < m; k += kFlight) {
+      Pack<T, VEC> x[kFlight];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const long t = __builtin_amdgcn_readlane(tok, k + u);
-        if (on) load_vec<T, VEC>(dy + t * width + c, x[u]);
+      for (int u = 0; u < kFlight; ++u) {
+        const long t =
+            __builtin_amdgcn_readlane(tok, k + u < m ? k + u : m - 1);
+        x[u] = *reinterpret_cast<const Pack<T, VEC>*>(from + t * width);
       }
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
+      for (int u = 0; u < kFlight; ++u)
+        if (k + u < m) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) acc[i] += x[u][i];
-    }
-    for (; k < m; ++k) {
-      float x[VEC];
-      const long t = __builtin_amdgcn_readlane(tok, k);
-      if (on) load_vec<T, VEC>(dy + t * width + c, x);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) acc[i] += x[i];
+          for (int i = 0; i < VEC; ++i) acc[i] += to_f32<T>(x[u].v[i]);
+        }
     }
   }
 }
 
 // Blocks [0, n * slots): pieces of rows of many tokens (they take longest,
-// so they begin first); the rest: four rows of few tokens each.
+// so they begin first); the rest: kLightRows rows of few tokens a wave.
+// Columns: blockIdx.y * cols and on, VEC a lane, cols <= 64 * VEC.
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void embed_grad_kernel(
-    GradArgs a, const T* __restrict__ dy, int width) {
+    GradArgs a, const T* __restrict__ dy, int width, int cols) {
   __shared__ float red[4][kWave * VEC];
-  __shared__ int last;
   const int lane = threadIdx.x & (kWave - 1);
-  const int w = threadIdx.x / kWave;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int nslots = a.n * a.slots;
-  const int step = kWave * VEC;
+  const int c0 = blockIdx.y * cols;
+  const int c = c0 + lane * VEC;
+  const bool on = lane * VEC < cols && c < width;
+  // lanes without columns load the first ones: a load under a condition
+  // would be waited for before the next one is sent
+  const T* from = dy + (on ? c : c0);
 
   if ((int)blockIdx.x >= nslots) {
     const int b = (int)blockIdx.x - nslots;
     int j = 0;
     while (j + 1 < a.n && b >= a.t[j + 1].light0) ++j;
     const GradTable& tb = a.t[j];
-    const int r = (b - tb.light0) * 4 + w;
-    if (r >= tb.rows) return;
-    const int p0 = tb.first[r], p1 = tb.first[r + 1];
-    if (p1 - p0 >= kHeavy) return;
-    T* out = static_cast<T*>(tb.out) + (long)r * width;
-    for (int c0 = 0; c0 < width; c0 += step) {
-      const int c = c0 + lane * VEC;
-      float acc[VEC];
-      sum_tokens<T, VEC>(dy, tb.order, p0, p1, width, c, c < width, lane, acc);
+    const int r0 = ((b - tb.light0) * 4 + w) * kLightRows;
+    const int places = tb.own << tb.lg;
+    if (r0 >= places) return;
+    const int nr = places - r0 < kLightRows ? places - r0 : kLightRows;
+    // lane i: where place r0 + i begins (lane nr: where the last one ends)
+    const int begin = tb.first[r0 + (lane < nr ? lane : nr)];
+    int r = 0;
+    while (r < nr) {
+      int p = __builtin_amdgcn_readlane(begin, r);
+      int e = __builtin_amdgcn_readlane(begin, r + 1);
+      if (e - p >= kHeavy) {
+        ++r;
+        continue;
+      }
+      // the rows up to the next heavy one: their tokens are neighbours
+      int r1 = r + 1, p1 = e;
+      while (r1 < nr) {
+        const int n = __builtin_amdgcn_readlane(begin, r1 + 1);
+        if (n - p1 >= kHeavy) break;
+        p1 = n;
+        ++r1;
+      }
+      float acc[VEC] = {};
+      auto store = [&]() {
+        const int id = place_id(tb, r0 + r);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) acc[i] *= tb.scale;
-      if (c < width) store_vec<T, VEC>(out + c, acc);
+        for (int i = 0; i < VEC; ++i) acc[i] *= tb.scale;
+        if (on && id < tb.rows)
+          store_vec<T, VEC>(static_cast<T*>(tb.out) + (long)id * width + c, acc);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
+        ++r;
+        if (r < r1) e = __builtin_amdgcn_readlane(begin, r + 1);
+      };
+      for (; p < p1; p += kWave) {
+        const int m = p1 - p < kWave ? p1 - p : kWave;
+        const int tok = lane < m ? tb.order[p + lane] : 0;
+        for (int k = 0; k < m; k += kFlight) {
+          Pack<T, VEC> x[kFlight];
+#pragma unroll
+          for (int u = 0; u < kFlight; ++u) {
+            const long t =
+                __builtin_amdgcn_readlane(tok, k + u < m ? k + u : m - 1);
+            x[u] = *reinterpret_cast<const Pack<T, VEC>*>(from + t * width);
+          }
+#pragma unroll
+          for (int u = 0; u < kFlight; ++u)
+            if (k + u < m) {
+              while (e <= p + k + u) store();
+#pragma unroll
+              for (int i = 0; i < VEC; ++i) acc[i] += to_f32<T>(x[u].v[i]);
+            }
+        }
+      }
+      while (r < r1) store();
     }
     return;
   }
@@ -314,87 +510,63 @@ __global__ __launch_bounds__(256) void embed_grad_kernel(
   const int j = (int)blockIdx.x / a.slots;
   const int slot = (int)blockIdx.x - j * a.slots;
   const GradTable& tb = a.t[j];
-  const int r = tb.slot_row[slot];
+  const int r = __builtin_amdgcn_readfirstlane(tb.slot_row[slot]);
+  if (r < 0) return;
+  const int p0 = __builtin_amdgcn_readfirstlane(tb.first[r]);
+  const int p1 = __builtin_amdgcn_readfirstlane(tb.first[r + 1]);
+  const int piece = piece_tokens(p1 - p0);
+  const int pieces = (p1 - p0 + piece - 1) / piece;
+  const int k = slot - p0 / kSlotUnit;
+  const int q0 = p0 + k * piece;
+  const int q1 = q0 + piece < p1 ? q0 + piece : p1;
+  const int per = (q1 - q0 + 3) / 4;               // a wave's tokens
+  const int w0 = __builtin_amdgcn_readfirstlane(q0 + w * per < q1 ? q0 + w * per
+                                                                  : q1);
+  const int w1 = w0 + per < q1 ? w0 + per : q1;
+  float acc[VEC];
+  sum_tokens<T, VEC>(from, tb.order, w0, w1, width, lane, acc);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) red[w][lane * VEC + i] = acc[i];
+  __syncthreads();
+  for (int i = threadIdx.x; i < cols && c0 + i < width; i += 256) {
+    const float x = (red[0][i] + red[1][i]) + (red[2][i] + red[3][i]);
+    if (pieces == 1)
+      static_cast<T*>(tb.out)[(long)place_id(tb, r) * width + c0 + i] =
+          from_f32<T>(x * tb.scale);
+    else
+      tb.part[(long)slot * width + c0 + i] = x;
+  }
+}
+
+// Rows of more than one piece: the pieces' sums, in their order.  A block
+// takes 64 columns, a wave a quarter of the pieces.
+template <typename T>
+__global__ __launch_bounds__(256) void embed_join_kernel(GradArgs a,
+                                                         int width) {
+  __shared__ float red[4][kWave];
+  const GradTable& tb = a.t[blockIdx.y];
+  const int r = tb.join_row[blockIdx.x];
   if (r < 0) return;
   const int p0 = tb.first[r], p1 = tb.first[r + 1];
   const int piece = piece_tokens(p1 - p0);
   const int pieces = (p1 - p0 + piece - 1) / piece;
-  const int slot0 = p0 / kSlotUnit;
-  const int k = slot - slot0;
-  const int q0 = p0 + k * piece;
-  const int q1 = q0 + piece < p1 ? q0 + piece : p1;
-  const int per = (q1 - q0 + 3) / 4;               // a wave's tokens
-  const int w0 = q0 + w * per < q1 ? q0 + w * per : q1;
-  const int w1 = w0 + per < q1 ? w0 + per : q1;
-  T* out = static_cast<T*>(tb.out) + (long)r * width;
-
-  for (int c0 = 0; c0 < width; c0 += step) {
-    const int c = c0 + lane * VEC;
-    float acc[VEC];
-    sum_tokens<T, VEC>(dy, tb.order, w0, w1, width, c, c < width, lane, acc);
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) red[w][lane * VEC + i] = acc[i];
-    __syncthreads();
-    if (w == 0 && c < width) {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        acc[i] = (red[0][lane * VEC + i] + red[1][lane * VEC + i]) +
-                 (red[2][lane * VEC + i] + red[3][lane * VEC + i]);
-      if (pieces == 1) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) acc[i] *= tb.scale;
-        store_vec<T, VEC>(out + c, acc);
-      } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i)
-          tb.part[(long)slot * width + c + i] = acc[i];
-      }
-    }
-    __syncthreads();
+  const int lane = threadIdx.x & (kWave - 1);
+  const int w = threadIdx.x / kWave;
+  const int c = blockIdx.z * kWave + lane;
+  const int per = (pieces + 3) / 4;
+  const int k1 = (w + 1) * per < pieces ? (w + 1) * per : pieces;
+  const float* part = tb.part + (long)(p0 / kSlotUnit) * width;
+  float x = 0.f;
+  if (c < width) {
+#pragma unroll 8
+    for (int k = w * per; k < k1; ++k) x += part[(long)k * width + c];
   }
-  if (pieces == 1) return;
-
-  // The piece that ends last adds all of them, in their order.  Every
-  // thread's stores are made visible before the count goes up, and the
-  // count is seen before the other pieces are read.
-  __threadfence();
+  red[w][lane] = x;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    const int before = __hip_atomic_fetch_add(
-        tb.done + slot0, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
-    last = before == pieces - 1;
-  }
-  __syncthreads();
-  if (!last) return;
-  __threadfence();
-  const int kp = (pieces + 3) / 4;
-  const int k0 = w * kp < pieces ? w * kp : pieces;
-  const int k1 = k0 + kp < pieces ? k0 + kp : pieces;
-  for (int c0 = 0; c0 < width; c0 += step) {
-    const int c = c0 + lane * VEC;
-    float acc[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
-    if (c < width) {
-#pragma unroll 4
-      for (int q = k0; q < k1; ++q)
-#pragma unroll
-        for (int i = 0; i < VEC; ++i)
-          acc[i] += tb.part[(long)(slot0 + q) * width + c + i];
-    }
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) red[w][lane * VEC + i] = acc[i];
-    __syncthreads();
-    if (w == 0 && c < width) {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        acc[i] = ((red[0][lane * VEC + i] + red[1][lane * VEC + i]) +
-                  (red[2][lane * VEC + i] + red[3][lane * VEC + i])) *
-                 tb.scale;
-      store_vec<T, VEC>(out + c, acc);
-    }
-    __syncthreads();
-  }
+  if (w == 0 && c < width)
+    static_cast<T*>(tb.out)[(long)place_id(tb, r) * width + c] = from_f32<T>(
+        ((red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane])) *
+        tb.scale);
 }
 
 void check_ids(const at::Tensor& ids, const at::Tensor& like, int64_t n) {
@@ -433,8 +605,17 @@ void launch_fwd(const LookupArgs& a, at::Tensor& y, long n, int width,
 template <typename T, int VEC>
 void launch_grad(const GradArgs& a, const at::Tensor& dy, int width,
                  unsigned blocks, hipStream_t s) {
-  embed_grad_kernel<T, VEC><<<blocks, 256, 0, s>>>(
-      a, static_cast<const T*>(dy.data_ptr()), width);
+  // even shares of the columns: 768 in two of 384, not 512 and 256
+  const int most = kWave * VEC;
+  const int parts = (width + most - 1) / most;
+  const int cols = ((width + parts - 1) / parts + VEC - 1) / VEC * VEC;
+  embed_grad_kernel<T, VEC><<<dim3(blocks, (unsigned)parts), 256, 0, s>>>(
+      a, static_cast<const T*>(dy.data_ptr()), width, cols);
+  // a row has more than one piece only among more tokens than that
+  if (dy.size(0) > kPiece)
+    embed_join_kernel<T><<<dim3((unsigned)a.joins, (unsigned)a.n,
+                                (unsigned)((width + kWave - 1) / kWave)),
+                           256, 0, s>>>(a, width);
 }
 
 }  // namespace
@@ -452,7 +633,7 @@ at::Tensor embed_sum_fwd_impl(at::TensorList ids_in, at::TensorList tables_in,
   TORCH_CHECK(w0.dim() == 2, "embedding: a table is [rows, width]");
   const c10::DeviceGuard guard(w0.device());
   const long n = ids_in[0].numel(), width = w0.size(1);
-  TORCH_CHECK(width <= (1 << 24), "embedding: a row is too wide");
+  TORCH_CHECK(width <= (1 << 22), "embedding: a row is too wide");
   std::vector<at::Tensor> hold;
   LookupArgs a{};
   a.n = (int)nt;
@@ -508,45 +689,51 @@ std::vector<at::Tensor> embed_sum_bwd_impl(const at::Tensor& dy_in,
   const c10::DeviceGuard guard(dy_in.device());
   const auto dy = dy_in.contiguous();
   const long n = dy.size(0), width = dy.size(1);
-  TORCH_CHECK(width <= (1 << 24) && n <= (1 << 30),
+  TORCH_CHECK(width <= (1 << 22) && n <= (1 << 30),
               "embedding: the gradient is too large");
   const long slots = n / kSlotUnit + 1;
   std::vector<at::Tensor> hold, out;
   GradArgs a{};
   a.n = (int)nt;
+  const long joins = n / kPiece + 1;
   a.slots = (int)slots;
+  a.joins = (int)joins;
   const auto ints = dy.options().dtype(at::kInt);
-  long sort_blocks = 0, light_blocks = 0;
-  int own_most = 1;
+  long buckets = 0, light_blocks = 0, most = 1;
   for (size_t j = 0; j < nt; ++j) {
     check_ids(ids_in[j], dy, n);
-    TORCH_CHECK(rows[j] >= 0 && rows[j] < (1ll << 31) - 8,
+    TORCH_CHECK(rows[j] >= 0 && rows[j] < (1l << (2 * kMaxSplit)),
                 "embedding: a table has too many rows");
     out.push_back(at::empty({rows[j], width}, dy.options()));
     GradTable& t = a.t[j];
     t.rows = (int)rows[j];
-    // a block a CU; more where a block's counts would not fit its LDS
-    long blocks = rows[j] < 256 ? std::max<long>(rows[j], 1) : 256;
-    long own = (rows[j] + blocks - 1) / blocks;
-    if (own > kMaxOwn) own = kMaxOwn;
-    if (own < 1) own = 1;
-    blocks = std::max<long>((rows[j] + own - 1) / own, 1);
-    own_most = std::max(own_most, (int)own);
+    // 256 buckets, more where a bucket's counts would not fit a block's LDS
+    int lg = 0;
+    while ((1l << lg) < rows[j] && (lg < 8 || (rows[j] >> lg) >= kMaxOwn)) ++lg;
+    const long own = std::max<long>((rows[j] + (1l << lg) - 1) >> lg, 1);
+    const long places = own << lg;
+    most = std::max(most, std::max(own, 1l << lg));
     t.own = (int)own;
-    t.sort0 = (int)sort_blocks;
-    sort_blocks += blocks;
+    t.lg = lg;
+    t.bucket0 = (int)buckets;
+    buckets += 1l << lg;
     t.light0 = (int)light_blocks;
-    light_blocks += (rows[j] + 3) / 4;
+    light_blocks += (places + 4 * kLightRows - 1) / (4 * kLightRows);
     hold.push_back(ids_in[j].contiguous());
     t.ids = hold.back().data_ptr();
     t.ids64 = hold.back().scalar_type() == at::kLong;
     t.scale = (float)scales[j];
     t.out = out.back().data_ptr();
-    hold.push_back(at::empty({n + rows[j] + 1 + 2 * slots}, ints));
-    t.order = hold.back().data_ptr<int>();
-    t.first = t.order + n;
-    t.slot_row = t.first + rows[j] + 1;
-    t.done = t.slot_row + slots;
+    const long g = 1l << lg;
+    hold.push_back(at::empty(
+        {g * kChunks + 3 * n + g + 1 + places + 1 + slots + joins}, ints));
+    t.count = hold.back().data_ptr<int>();     // first: read 16 bytes at a time
+    t.loose = reinterpret_cast<int2*>(t.count + g * kChunks);
+    t.order = t.count + g * kChunks + 2 * n;
+    t.start = t.order + n;
+    t.first = t.start + g + 1;
+    t.slot_row = t.first + places + 1;
+    t.join_row = t.slot_row + slots;
     hold.push_back(at::empty({slots * width}, dy.options().dtype(at::kFloat)));
     t.part = hold.back().data_ptr<float>();
   }
@@ -559,9 +746,16 @@ std::vector<at::Tensor> embed_sum_bwd_impl(const at::Tensor& dy_in,
   TORCH_CHECK(blocks <= std::numeric_limits<int>::max(),
               "embedding: the tables are too large");
   auto s = at::cuda::getCurrentCUDAStream();
-  const size_t lds =
-      ((size_t)kSortWaves * own_most + 2 * kSortWaves) * sizeof(int);
-  embed_sort_kernel<<<(unsigned)sort_blocks, kSortThreads, lds, s>>>(a, (int)n);
+  const size_t lds = ((size_t)kSortWaves * (most + 1)) * sizeof(int);
+  const long chunk = std::max<long>(
+      kSortThreads, (n + kChunks - 1) / kChunks + kSortThreads - 1) /
+      kSortThreads * kSortThreads;
+  const long chunks = (n + chunk - 1) / chunk;
+  const dim3 by_chunk((unsigned)chunks, (unsigned)nt);
+  embed_count_kernel<<<by_chunk, kSortThreads, 0, s>>>(a, (int)n, (int)chunk);
+  embed_scatter_kernel<<<by_chunk, kSortThreads, lds, s>>>(
+      a, (int)n, (int)chunk, (int)chunks);
+  embed_order_kernel<<<(unsigned)buckets, kSortThreads, lds, s>>>(a);
   const bool vec = aligned16(dy.data_ptr());
   switch (dy.scalar_type()) {
     case at::kBFloat16:

@@ -155,6 +155,17 @@ void doc_attn_bwd_impl(const at::Tensor& dout, const at::Tensor& q,
                        const c10::optional<at::Tensor>& slopes, double scale,
                        at::Tensor dq, at::Tensor dk, at::Tensor dv);
 
+// seq_autograd.hip
+at::Tensor embedding_sum(at::TensorList ids, at::TensorList tables,
+                         at::ArrayRef<double> scales);
+at::Tensor doc_attention(const at::Tensor& q, const at::Tensor& k,
+                         const at::Tensor& v, const at::Tensor& cu,
+                         const c10::optional<at::Tensor>& slopes,
+                         double scale);
+at::Tensor doc_attention_qkv(const at::Tensor& qkv, const at::Tensor& cu,
+                             const c10::optional<at::Tensor>& slopes,
+                             double scale);
+
 // newton_schulz.hip
 at::Tensor newton_schulz_impl(const at::Tensor& g, int64_t steps, double eps);
 
@@ -333,6 +344,9 @@ TORCH_LIBRARY(dlx_hip, m) {
   m.def("embed_sum_bwd(Tensor dy, Tensor[] ids, int[] rows, float[] scales) -> Tensor[]");
   m.def("doc_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor cu, Tensor? slopes, float scale, bool need_lse) -> (Tensor, Tensor)");
   m.def("doc_attn_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, Tensor cu, Tensor? slopes, float scale, Tensor(a!) dq, Tensor(b!) dk, Tensor(c!) dv) -> ()");
+  m.def("embedding_sum(Tensor[] ids, Tensor[] tables, float[] scales) -> Tensor");
+  m.def("doc_attention(Tensor q, Tensor k, Tensor v, Tensor cu, Tensor? slopes, float scale) -> Tensor");
+  m.def("doc_attention_qkv(Tensor qkv, Tensor cu, Tensor? slopes, float scale) -> Tensor");
   m.def("newton_schulz(Tensor g, int steps, float eps) -> Tensor");
 }
 
@@ -382,4 +396,17 @@ TORCH_LIBRARY_IMPL(dlx_hip, CUDA, m) {
   m.impl("doc_attn_fwd", dlx::doc_attn_fwd_impl);
   m.impl("doc_attn_bwd", dlx::doc_attn_bwd_impl);
   m.impl("newton_schulz", dlx::newton_schulz_impl);
+}
+
+TORCH_LIBRARY_IMPL(dlx_hip, AutogradCUDA, m) {
+  m.impl("embedding_sum", dlx::embedding_sum);
+  m.impl("doc_attention", dlx::doc_attention);
+  m.impl("doc_attention_qkv", dlx::doc_attention_qkv);
+}
+
+// without a graph (inference mode)
+TORCH_LIBRARY_IMPL(dlx_hip, CUDA, m) {
+  m.impl("embedding_sum", dlx::embedding_sum);
+  m.impl("doc_attention", dlx::doc_attention);
+  m.impl("doc_attention_qkv", dlx::doc_attention_qkv);
 }

@@ -1,0 +1,193 @@
+// Gradients of the embedding lookup and of document attention as nodes of
+// torch's graph in C++.
+//
+// A training step runs these once a layer, next to kernels of 10 to 100 us;
+// a node written in Python adds about 60 us of host time to a forward and
+// backward pass (the interpreter lock changes hands between threads), one in
+// C++ about 20.
+//
+// The gradients have no gradient of their own: asking for a graph of them
+// (create_graph) raises.  Saved inputs are checked for changes in place.
+#include <torch/extension.h>
+#include <torch/csrc/autograd/custom_function.h>
+
+namespace dlx {
+
+at::Tensor embed_sum_fwd_impl(at::TensorList ids, at::TensorList tables,
+                              at::ArrayRef<double> scales);
+std::vector<at::Tensor> embed_sum_bwd_impl(const at::Tensor& dy,
+                                           at::TensorList ids,
+                                           at::IntArrayRef rows,
+                                           at::ArrayRef<double> scales);
+std::tuple<at::Tensor, at::Tensor> doc_attn_fwd_impl(
+    const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+    const at::Tensor& cu, const c10::optional<at::Tensor>& slopes,
+    double scale, bool need_lse);
+void doc_attn_bwd_impl(const at::Tensor& dout, const at::Tensor& q,
+                       const at::Tensor& k, const at::Tensor& v,
+                       const at::Tensor& o, const at::Tensor& lse,
+                       const at::Tensor& cu,
+                       const c10::optional<at::Tensor>& slopes, double scale,
+                       at::Tensor dq, at::Tensor dk, at::Tensor dv);
+
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::Function;
+using torch::autograd::tensor_list;
+
+void refuse_graph(const char* name) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), name,
+              ": its gradient has no gradient (create_graph)");
+}
+
+at::Tensor lookup(at::TensorList ids, at::TensorList tables,
+                  at::ArrayRef<double> scales) {
+  auto y = embed_sum_fwd_impl(ids, tables, scales);
+  auto shape = ids[0].sizes().vec();
+  shape.push_back(tables[0].size(1));
+  return y.view(shape);
+}
+
+struct EmbeddingSum : Function<EmbeddingSum> {
+  static at::Tensor forward(AutogradContext* ctx, at::TensorList tables,
+                            at::TensorList ids, std::vector<double> scales) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    ctx->save_for_backward(ids.vec());
+    std::vector<int64_t> rows;
+    for (const auto& w : tables) rows.push_back(w.size(0));
+    ctx->saved_data["rows"] = rows;
+    ctx->saved_data["scales"] = scales;
+    return lookup(ids, tables, scales);
+  }
+
+  static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+    refuse_graph("embedding_sum");
+    const auto ids = ctx->get_saved_variables();
+    const auto rows = ctx->saved_data["rows"].toIntVector();
+    const auto scales = ctx->saved_data["scales"].toDoubleVector();
+    const size_t n = ids.size();
+    tensor_list out(2 * n + 1);       // tables, ids, scales
+    std::vector<at::Tensor> want;
+    std::vector<int64_t> want_rows;
+    std::vector<double> want_scales;
+    for (size_t i = 0; i < n; ++i)
+      if (ctx->needs_input_grad(i)) {
+        want.push_back(ids[i]);
+        want_rows.push_back(rows[i]);
+        want_scales.push_back(scales[i]);
+      }
+    if (want.empty() || !grads[0].defined()) return out;
+    const auto got =
+        embed_sum_bwd_impl(grads[0].reshape({-1, grads[0].size(-1)}), want,
+                           want_rows, want_scales);
+    for (size_t i = 0, k = 0; i < n; ++i)
+      if (ctx->needs_input_grad(i)) out[i] = got[k++];
+    return out;
+  }
+};
+
+struct DocAttention : Function<DocAttention> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& q,
+                            const at::Tensor& k, const at::Tensor& v,
+                            const at::Tensor& cu,
+                            const c10::optional<at::Tensor>& slopes,
+                            double scale) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [o, lse] = doc_attn_fwd_impl(q, k, v, cu, slopes, scale, true);
+    ctx->save_for_backward(
+        {q, k, v, o, lse, cu, slopes ? *slopes : at::Tensor()});
+    ctx->saved_data["scale"] = scale;
+    return o;
+  }
+
+  static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+    refuse_graph("document_attention");
+    tensor_list out(6);
+    if (!grads[0].defined()) return out;
+    const auto s = ctx->get_saved_variables();
+    for (int i = 0; i < 3; ++i) out[i] = at::empty(s[i].sizes(), s[i].options());
+    c10::optional<at::Tensor> slopes;
+    if (s[6].defined()) slopes = s[6];
+    doc_attn_bwd_impl(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], slopes,
+                      ctx->saved_data["scale"].toDouble(), out[0], out[1],
+                      out[2]);
+    return out;
+  }
+};
+
+// The same on one projection's output [tokens, 3, heads, dim]: the gradient
+// is written in its layout.
+struct DocAttentionQKV : Function<DocAttentionQKV> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& qkv,
+                            const at::Tensor& cu,
+                            const c10::optional<at::Tensor>& slopes,
+                            double scale) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [o, lse] =
+        doc_attn_fwd_impl(qkv.select(1, 0), qkv.select(1, 1), qkv.select(1, 2),
+                          cu, slopes, scale, true);
+    ctx->save_for_backward({qkv, o, lse, cu, slopes ? *slopes : at::Tensor()});
+    ctx->saved_data["scale"] = scale;
+    return o;
+  }
+
+  static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+    refuse_graph("document_attention_qkv");
+    tensor_list out(4);
+    if (!grads[0].defined()) return out;
+    const auto s = ctx->get_saved_variables();
+    const auto& qkv = s[0];
+    out[0] = at::empty(qkv.sizes(), qkv.options());
+    c10::optional<at::Tensor> slopes;
+    if (s[4].defined()) slopes = s[4];
+    doc_attn_bwd_impl(grads[0], qkv.select(1, 0), qkv.select(1, 1),
+                      qkv.select(1, 2), s[1], s[2], s[3], slopes,
+                      ctx->saved_data["scale"].toDouble(), out[0].select(1, 0),
+                      out[0].select(1, 1), out[0].select(1, 2));
+    return out;
+  }
+};
+
+bool wants_grad(at::TensorList ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const auto& t : ts)
+    if (t.requires_grad()) return true;
+  return false;
+}
+
+}  // namespace
+
+// ids of one shape, tables [rows, width] -> [*shape, width]
+at::Tensor embedding_sum(at::TensorList ids, at::TensorList tables,
+                         at::ArrayRef<double> scales) {
+  TORCH_CHECK(!ids.empty() && !tables.empty(), "embedding_sum: no tables");
+  if (wants_grad(tables))
+    return EmbeddingSum::apply(tables, ids, scales.vec());
+  at::AutoDispatchBelowADInplaceOrView below;
+  return lookup(ids, tables, scales);
+}
+
+at::Tensor doc_attention(const at::Tensor& q, const at::Tensor& k,
+                         const at::Tensor& v, const at::Tensor& cu,
+                         const c10::optional<at::Tensor>& slopes,
+                         double scale) {
+  if (wants_grad({q, k, v}))
+    return DocAttention::apply(q, k, v, cu, slopes, scale);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return std::get<0>(doc_attn_fwd_impl(q, k, v, cu, slopes, scale, false));
+}
+
+at::Tensor doc_attention_qkv(const at::Tensor& qkv, const at::Tensor& cu,
+                             const c10::optional<at::Tensor>& slopes,
+                             double scale) {
+  TORCH_CHECK(qkv.dim() == 4 && qkv.size(1) == 3,
+              "document_attention_qkv: [tokens, 3, heads, dim] expected");
+  if (wants_grad({qkv})) return DocAttentionQKV::apply(qkv, cu, slopes, scale);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return std::get<0>(doc_attn_fwd_impl(qkv.select(1, 0), qkv.select(1, 1),
+                                       qkv.select(1, 2), cu, slopes, scale,
+                                       false));
+}
+
+}  // namespace dlx

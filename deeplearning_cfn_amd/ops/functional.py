@@ -12,7 +12,6 @@ from typing import Optional, Sequence
 
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from . import native, native_available
 
@@ -633,28 +632,6 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 # (embedding.hip)
 # ---------------------------------------------------------------------------
 
-class _EmbeddingSum(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, ids, scales, *tables):
-        ctx.ids, ctx.scales = ids, scales
-        ctx.rows = [w.shape[0] for w in tables]
-        y = native().embed_sum_fwd(ids, tables, scales)
-        return y.view(*ids[0].shape, tables[0].shape[1])
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        want = [i for i in range(len(ctx.rows)) if ctx.needs_input_grad[2 + i]]
-        grads = [None] * len(ctx.rows)
-        if want:
-            got = native().embed_sum_bwd(
-                grad.reshape(-1, grad.shape[-1]), [ctx.ids[i] for i in want],
-                [ctx.rows[i] for i in want], [ctx.scales[i] for i in want])
-            for i, g in zip(want, got):
-                grads[i] = g
-        return (None, None, *grads)
-
-
 def embedding_sum(ids: Sequence[torch.Tensor], tables: Sequence[torch.Tensor],
                   scales: Optional[Sequence[float]] = None) -> torch.Tensor:
     """``sum_j scales[j] * tables[j][ids[j]]`` for one to four tables.
@@ -687,7 +664,7 @@ def embedding_sum(ids: Sequence[torch.Tensor], tables: Sequence[torch.Tensor],
                              "devices")
     if _use_native(w0) and w0.dtype in (torch.bfloat16, torch.float16,
                                         torch.float32):
-        return _EmbeddingSum.apply(ids, scales, *tables)
+        return native().embedding_sum(ids, tables, scales)
     acc = sum(F.embedding(i, w).float() * c
               for i, w, c in zip(ids, tables, scales))
     return acc.to(w0.dtype)
@@ -702,49 +679,6 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor,
 # ---------------------------------------------------------------------------
 # attention inside packed documents (doc_attention.hip)
 # ---------------------------------------------------------------------------
-
-class _DocAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, cu, slopes, scale):
-        o, lse = native().doc_attn_fwd(q, k, v, cu, slopes, scale,
-                                       any(ctx.needs_input_grad))
-        ctx.save_for_backward(q, k, v, o, lse, cu, slopes)
-        ctx.scale = scale
-        return o
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        q, k, v, o, lse, cu, slopes = ctx.saved_tensors
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device)
-                      for t in (q, k, v))
-        native().doc_attn_bwd(grad, q, k, v, o, lse, cu, slopes, ctx.scale,
-                              dq, dk, dv)
-        return dq, dk, dv, None, None, None
-
-
-class _DocAttentionQKV(torch.autograd.Function):
-    """The same on one projection's output: its gradient is written in place
-    of the projection's, with no slices to put together."""
-
-    @staticmethod
-    def forward(ctx, qkv, cu, slopes, scale):
-        q, k, v = qkv.unbind(1)
-        o, lse = native().doc_attn_fwd(q, k, v, cu, slopes, scale,
-                                       any(ctx.needs_input_grad))
-        ctx.save_for_backward(qkv, o, lse, cu, slopes)
-        ctx.scale = scale
-        return o
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        qkv, o, lse, cu, slopes = ctx.saved_tensors
-        d = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-        native().doc_attn_bwd(grad, *qkv.unbind(1), o, lse, cu, slopes,
-                              ctx.scale, *d.unbind(1))
-        return d, None, None, None
-
 
 def _doc_attention_args(name, q, k, cu, scale, slopes):
     if cu.dim() != 1 or cu.numel() < 1 or cu.dtype not in (torch.int32,
@@ -825,7 +759,7 @@ def document_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     cu, scale, slopes = _doc_attention_args("document_attention", q, k,
                                             cu_seqlens, scale, slopes)
     if _doc_attention_native(q):
-        return _DocAttention.apply(q, k, v, cu, slopes, scale)
+        return native().doc_attention(q, k, v, cu, slopes, scale)
     return _doc_attention_composed(q, k, v, cu, scale, slopes)
 
 
@@ -842,7 +776,7 @@ def document_attention_qkv(qkv: torch.Tensor, cu_seqlens: torch.Tensor,
     cu, scale, slopes = _doc_attention_args("document_attention_qkv", q, k,
                                             cu_seqlens, scale, slopes)
     if _doc_attention_native(qkv):
-        return _DocAttentionQKV.apply(qkv, cu, slopes, scale)
+        return native().doc_attention_qkv(qkv, cu, slopes, scale)
     return _doc_attention_composed(q, k, v, cu, scale, slopes)
 
 
