@@ -36,6 +36,7 @@ namespace {
 
 constexpr int kKeys = 64;             // rows of an LDS tile
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLazy = 8.f;          // P stays under 2^8
 
 __device__ const uint4 g_zero16 = {0, 0, 0, 0};
 
@@ -108,7 +109,7 @@ DLX_DEV void load_tile(uint16_t* lds, const uint16_t* base, long stride,
   for (int u = 0; u < kKeys * CH / NT; ++u) {
     const int f = u * NT + threadIdx.x;
     const int row = f / CH;
-    const int chunk = (f % CH) ^ (row & 7);
+    const int chunk = (f % CH) ^ swizzle<DP>(row);
     const int r = row0 + row < len ? row0 + row : len - 1;
     const void* src = base + r * stride + chunk * 8;
     if (chunk * 8 >= dim) src = &g_zero16;
@@ -152,13 +153,33 @@ DLX_DEV void zero_rows(const View& v, long token, int head, int dim, int lane) {
 // register i of a result: its row of 32
 DLX_DEV constexpr int reg_row(int i) { return 8 * (i >> 2) + (i & 3); }
 
+// What a block of scores begins at: -sl |key - query|, keys k0 + .., queries
+// wave_row ..+31, shift = 4 * (lane >> 5) - query.  Where the block lies on
+// one side of the diagonal the sign is known, and a register takes one fma.
+DLX_DEV f32x16 bias(float sl, int k0, int wave_row, int shift) {
+  f32x16 s;
+  const float d0 = (float)(k0 + shift);
+  if (k0 >= wave_row + 31) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      s[i] = fmaf(-sl, (float)reg_row(i), -sl * d0);
+  } else if (k0 + 31 <= wave_row) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = fmaf(sl, (float)reg_row(i), sl * d0);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = -sl * fabsf(d0 + (float)reg_row(i));
+  }
+  return s;
+}
+
 // ---------------------------------------------------------------------------
 // forward: a wave owns 32 queries, a block NW waves; keys and values pass in
 // tiles of 64, the next one on its way while this one is worked on.
 // ---------------------------------------------------------------------------
 
 template <typename T, int DP, int NW, bool BIAS>
-__global__ __launch_bounds__(NW * 64) void doc_attn_fwd_kernel(AttnArgs a) {
+__global__ __launch_bounds__(NW * 64, 2) void doc_attn_fwd_kernel(AttnArgs a) {
   constexpr int NT = NW * 64, ROWS = NW * 32, TS = kKeys * DP;
   __shared__ __attribute__((aligned(16))) uint16_t lds[4 * TS];
 
@@ -168,9 +189,10 @@ __global__ __launch_bounds__(NW * 64) void doc_attn_fwd_kernel(AttnArgs a) {
   const Tile tl = find_tile<ROWS>(a, bid - head * tiles);
   if (tl.row0 >= tl.len) return;
   const int lane = threadIdx.x & (kWave - 1);
-  const int wid = threadIdx.x / kWave;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int half = lane >> 5;
-  const int qpos = tl.row0 + wid * 32 + (lane & 31);
+  const int wave_row = tl.row0 + wid * 32;
+  const int qpos = wave_row + (lane & 31);
   const bool real = qpos < tl.len;
   if (!tl.doc) {
     if (real) zero_rows<DP>(a.o, tl.start + qpos, head, a.dim, lane);
@@ -187,39 +209,34 @@ __global__ __launch_bounds__(NW * 64) void doc_attn_fwd_kernel(AttnArgs a) {
   s16x8 qf[DP / 16];
   load_rows<DP>(qf, a.q.p + token * a.q.token + head * a.q.head, a.dim, lane);
 
+  const Frags<DP> fr(lane);
   const float sc = a.scale * kLog2e;
-  const float sl = BIAS ? a.slopes[head] * kLog2e : 0.f;
-  float m = -INFINITY, l = 0.f;
+  const float sl = BIAS ? a.slopes[head] / a.scale : 0.f;
+  // m: what the row's exponents are taken next to; it follows the row's
+  // maximum only when that is past it by 2^kLazy, which spares the products
+  // their rescaling in nearly every tile.  ms: m, or 0 in a row of -inf.
+  float m = -INFINITY, ms = 0.f, l = 0.f;
   f32x16 acc[DP / 32] = {};
 
-  for (int t = 0; t < nt; ++t) {
+  auto body = [&](int t, const uint16_t* lk, uint16_t* nx) {
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    const uint16_t* lk = lds + (t & 1) * 2 * TS;
     const uint16_t* lv = lk + TS;
     if (t + 1 < nt) {
-      uint16_t* nx = lds + ((t + 1) & 1) * 2 * TS;
       load_tile<DP, NT>(nx, kb, a.k.token, (t + 1) * kKeys, tl.len, a.dim);
       load_tile<DP, NT>(nx + TS, vb, a.v.token, (t + 1) * kKeys, tl.len, a.dim);
     }
-    f32x16 s[2] = {};
+    f32x16 s[2];
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < 2; ++b) {
+      s[b] = BIAS ? bias(sl, t * kKeys + b * 32, wave_row, half * 4 - qpos)
+                  : f32x16{};
 #pragma unroll
       for (int st = 0; st < DP / 16; ++st)
-        s[b] = mfma32<T>(row_frag<DP>(lk, b * 32, st, lane), qf[st], s[b]);
-
-    const int k0 = t * kKeys + half * 4;      // key of register 0 of block 0
-    if (BIAS) {
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const float d0 = (float)(k0 + b * 32 - qpos);
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          s[b][i] = s[b][i] * sc - sl * fabsf(d0 + (float)reg_row(i));
-      }
+        s[b] = mfma32<T>(fr.row(lk, b * 32, st), qf[st], s[b]);
     }
     if ((t + 1) * kKeys > tl.len) {
+      const int k0 = t * kKeys + half * 4;
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -231,38 +248,40 @@ __global__ __launch_bounds__(NW * 64) void doc_attn_fwd_kernel(AttnArgs a) {
     for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[b][i]);
-    mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
-    if (!BIAS) mx *= sc;
-    if (__ballot(mx > m)) {
+    mx *= sc;
+    if (__ballot(mx > m + kLazy)) {
+      mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
       const float mn = fmaxf(m, mx);
-      const float by = mn == -INFINITY ? 1.f : exp2f(m - mn);
+      const float by =
+          mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       m = mn;
+      ms = m == -INFINITY ? 0.f : m;
       l *= by;
 #pragma unroll
       for (int b = 0; b < DP / 32; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[b][i] *= by;
     }
-    const float ms = m == -INFINITY ? 0.f : m;   // a row of -inf so far
-    float p[2][16];
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        p[b][i] = __builtin_amdgcn_exp2f(BIAS ? s[b][i] - ms
-                                              : s[b][i] * sc - ms);
-        l += p[b][i];
-      }
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
-        const s16x8 pf = pack_step<T>(&p[b][st * 8]);
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          p[e] = __builtin_amdgcn_exp2f(s[b][st * 8 + e] * sc - ms);
+          l += p[e];
+        }
+        const s16x8 pf = pack_step<T>(p);
 #pragma unroll
         for (int db = 0; db < DP / 32; ++db)
-          acc[db] = mfma32<T>(
-              tr_frag<DP>(lv, b * 32 + st * 16, db * 32, lane), pf, acc[db]);
+          acc[db] = mfma32<T>(fr.tr(lv, b * 32 + st * 16, db), pf, acc[db]);
       }
+  };
+  // two tiles a turn, so that each half of LDS has its own addresses
+  for (int t = 0; t < nt; t += 2) {
+    body(t, lds, lds + 2 * TS);
+    if (t + 1 < nt) body(t + 1, lds + 2 * TS, lds);
   }
   l += __shfl_xor(l, 32, kWave);
   if (!real) return;
@@ -278,7 +297,7 @@ __global__ __launch_bounds__(NW * 64) void doc_attn_fwd_kernel(AttnArgs a) {
 // ---------------------------------------------------------------------------
 
 template <typename T, int DP, int NW, bool BIAS>
-__global__ __launch_bounds__(NW * 64) void doc_attn_dq_kernel(AttnArgs a) {
+__global__ __launch_bounds__(NW * 64, 2) void doc_attn_dq_kernel(AttnArgs a) {
   constexpr int NT = NW * 64, ROWS = NW * 32, TS = kKeys * DP;
   __shared__ __attribute__((aligned(16))) uint16_t lds[4 * TS];
 
@@ -288,9 +307,10 @@ __global__ __launch_bounds__(NW * 64) void doc_attn_dq_kernel(AttnArgs a) {
   const Tile tl = find_tile<ROWS>(a, bid - head * tiles);
   if (tl.row0 >= tl.len) return;
   const int lane = threadIdx.x & (kWave - 1);
-  const int wid = threadIdx.x / kWave;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int half = lane >> 5;
-  const int qpos = tl.row0 + wid * 32 + (lane & 31);
+  const int wave_row = tl.row0 + wid * 32;
+  const int qpos = wave_row + (lane & 31);
   const bool real = qpos < tl.len;
   if (!tl.doc) {
     if (real) zero_rows<DP>(a.dq, tl.start + qpos, head, a.dim, lane);
@@ -322,39 +342,39 @@ __global__ __launch_bounds__(NW * 64) void doc_attn_dq_kernel(AttnArgs a) {
   }
   if (real && half == 0) a.delta[(long)head * a.tokens + token] = delta;
   const float lse = a.lse[(long)head * a.tokens + token];
+  const Frags<DP> fr(lane);
   const float sc = a.scale * kLog2e;
-  const float sl = BIAS ? a.slopes[head] * kLog2e : 0.f;
+  const float sl = BIAS ? a.slopes[head] / a.scale : 0.f;
   f32x16 acc[DP / 32] = {};
+  f32x16 less;                        // what dP begins at: dP - D for nothing
+#pragma unroll
+  for (int i = 0; i < 16; ++i) less[i] = -delta;
 
-  for (int t = 0; t < nt; ++t) {
+  auto body = [&](int t, const uint16_t* lk, uint16_t* nx) {
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    const uint16_t* lk = lds + (t & 1) * 2 * TS;
     const uint16_t* lv = lk + TS;
     if (t + 1 < nt) {
-      uint16_t* nx = lds + ((t + 1) & 1) * 2 * TS;
       load_tile<DP, NT>(nx, kb, a.k.token, (t + 1) * kKeys, tl.len, a.dim);
       load_tile<DP, NT>(nx + TS, vb, a.v.token, (t + 1) * kKeys, tl.len, a.dim);
     }
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      f32x16 s = {}, dp = {};
+      f32x16 s = BIAS ? bias(sl, t * kKeys + b * 32, wave_row, half * 4 - qpos)
+                      : f32x16{};
+      f32x16 dp = less;
 #pragma unroll
       for (int st = 0; st < DP / 16; ++st)
-        s = mfma32<T>(row_frag<DP>(lk, b * 32, st, lane), qf[st], s);
+        s = mfma32<T>(fr.row(lk, b * 32, st), qf[st], s);
 #pragma unroll
       for (int st = 0; st < DP / 16; ++st)
-        dp = mfma32<T>(row_frag<DP>(lv, b * 32, st, lane), gf[st], dp);
-      const int k0 = t * kKeys + b * 32 + half * 4;
-      const float d0 = (float)(k0 - qpos);
+        dp = mfma32<T>(fr.row(lv, b * 32, st), gf[st], dp);
       float ds[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float x = s[i] * sc - lse;
-        if (BIAS) x -= sl * fabsf(d0 + (float)reg_row(i));
-        ds[i] = __builtin_amdgcn_exp2f(x) * (dp[i] - delta);
-      }
+      for (int i = 0; i < 16; ++i)
+        ds[i] = __builtin_amdgcn_exp2f(s[i] * sc - lse) * dp[i];
       if ((t + 1) * kKeys > tl.len) {
+        const int k0 = t * kKeys + b * 32 + half * 4;
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (k0 + reg_row(i) >= tl.len) ds[i] = 0.f;
@@ -364,10 +384,13 @@ __global__ __launch_bounds__(NW * 64) void doc_attn_dq_kernel(AttnArgs a) {
         const s16x8 df = pack_step<T>(&ds[st * 8]);
 #pragma unroll
         for (int db = 0; db < DP / 32; ++db)
-          acc[db] = mfma32<T>(
-              tr_frag<DP>(lk, b * 32 + st * 16, db * 32, lane), df, acc[db]);
+          acc[db] = mfma32<T>(fr.tr(lk, b * 32 + st * 16, db), df, acc[db]);
       }
     }
+  };
+  for (int t = 0; t < nt; t += 2) {
+    body(t, lds, lds + 2 * TS);
+    if (t + 1 < nt) body(t + 1, lds + 2 * TS, lds);
   }
   if (real)
     store_rows<T, DP>(a.dq.p + token * a.dq.token + head * a.dq.head, acc,
@@ -380,7 +403,7 @@ __global__ __launch_bounds__(NW * 64) void doc_attn_dq_kernel(AttnArgs a) {
 // ---------------------------------------------------------------------------
 
 template <typename T, int DP, int NW, bool BIAS>
-__global__ __launch_bounds__(NW * 64) void doc_attn_dkv_kernel(AttnArgs a) {
+__global__ __launch_bounds__(NW * 64, 2) void doc_attn_dkv_kernel(AttnArgs a) {
   constexpr int NT = NW * 64, ROWS = NW * 32, TS = kKeys * DP;
   __shared__ __attribute__((aligned(16))) uint16_t lds[4 * TS];
   __shared__ __attribute__((aligned(16))) float stat[2][2][kKeys];
@@ -407,6 +430,8 @@ __global__ __launch_bounds__(NW * 64) void doc_attn_dkv_kernel(AttnArgs a) {
   const int nt = (tl.len + kKeys - 1) / kKeys;
   const int all = nt * a.group;
 
+  const float sc = a.scale * kLog2e, unit = 1.f / sc;
+
   // tile n of the walk: head kvh * group + n / nt, rows (n % nt) * 64..
   auto stage = [&](int n) {
     const int head = kvh * a.group + n / nt;
@@ -418,68 +443,69 @@ __global__ __launch_bounds__(NW * 64) void doc_attn_dkv_kernel(AttnArgs a) {
                       a.dout.p + tl.start * a.dout.token + head * a.dout.head,
                       a.dout.token, row0, tl.len, a.dim);
     if (threadIdx.x < kKeys) {
-      // a query behind the document's end: exp2(x - inf) is 0
+      // what S and dP begin at; behind the document's end exp2(-inf) is 0
       const int r = row0 + threadIdx.x;
       const long i = (long)head * a.tokens + tl.start + r;
-      stat[n & 1][0][threadIdx.x] = r < tl.len ? a.lse[i] : INFINITY;
-      stat[n & 1][1][threadIdx.x] = r < tl.len ? a.delta[i] : 0.f;
+      stat[n & 1][0][threadIdx.x] = r < tl.len ? a.lse[i] * -unit : -INFINITY;
+      stat[n & 1][1][threadIdx.x] = r < tl.len ? -a.delta[i] : 0.f;
     }
   };
   stage(0);
   s16x8 kf[DP / 16], vf[DP / 16];
   load_rows<DP>(kf, a.k.p + token * a.k.token + kvh * a.k.head, a.dim, lane);
   load_rows<DP>(vf, a.v.p + token * a.v.token + kvh * a.v.head, a.dim, lane);
-  const float sc = a.scale * kLog2e;
+  const Frags<DP> fr(lane);
   f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
 
-  for (int n = 0; n < all; ++n) {
+  auto body = [&](int n, const uint16_t* lq, const float (*st_)[kKeys]) {
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
     if (n + 1 < all) stage(n + 1);
-    const uint16_t* lq = lds + (n & 1) * 2 * TS;
     const uint16_t* lg = lq + TS;
-    const float sl =
-        BIAS ? a.slopes[kvh * a.group + n / nt] * kLog2e : 0.f;
+    const float sl = BIAS ? a.slopes[kvh * a.group + n / nt] / a.scale : 0.f;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      f32x16 s = {}, dp = {};
-#pragma unroll
-      for (int st = 0; st < DP / 16; ++st)
-        s = mfma32<T>(row_frag<DP>(lq, b * 32, st, lane), kf[st], s);
-#pragma unroll
-      for (int st = 0; st < DP / 16; ++st)
-        dp = mfma32<T>(row_frag<DP>(lg, b * 32, st, lane), vf[st], dp);
       const int q0 = b * 32 + half * 4;
       const float d0 = (float)((n % nt) * kKeys + q0 - kpos);
-      float p[16], ds[16];
+      f32x16 s, dp;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const F32x4 ls =
-            *reinterpret_cast<const F32x4*>(&stat[n & 1][0][q0 + g * 8]);
-        const F32x4 de =
-            *reinterpret_cast<const F32x4*>(&stat[n & 1][1][q0 + g * 8]);
+        const F32x4 ls = *reinterpret_cast<const F32x4*>(&st_[0][q0 + g * 8]);
+        const F32x4 de = *reinterpret_cast<const F32x4*>(&st_[1][q0 + g * 8]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int i = g * 4 + e;
-          float x = s[i] * sc - ls.v[e];
-          if (BIAS) x -= sl * fabsf(d0 + (float)reg_row(i));
-          p[i] = __builtin_amdgcn_exp2f(x);
-          ds[i] = p[i] * (dp[i] - de.v[e]);
+          s[g * 4 + e] = ls.v[e];
+          if (BIAS) s[g * 4 + e] -= sl * fabsf(d0 + (float)(g * 8 + e));
+          dp[g * 4 + e] = de.v[e];
         }
       }
 #pragma unroll
+      for (int st = 0; st < DP / 16; ++st)
+        s = mfma32<T>(fr.row(lq, b * 32, st), kf[st], s);
+#pragma unroll
+      for (int st = 0; st < DP / 16; ++st)
+        dp = mfma32<T>(fr.row(lg, b * 32, st), vf[st], dp);
+#pragma unroll
       for (int st = 0; st < 2; ++st) {
-        const s16x8 pf = pack_step<T>(&p[st * 8]);
-        const s16x8 df = pack_step<T>(&ds[st * 8]);
+        float p[8], ds[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          p[e] = __builtin_amdgcn_exp2f(s[st * 8 + e] * sc);
+          ds[e] = p[e] * dp[st * 8 + e];
+        }
+        const s16x8 pf = pack_step<T>(p);
+        const s16x8 df = pack_step<T>(ds);
 #pragma unroll
         for (int db = 0; db < DP / 32; ++db) {
-          dv[db] = mfma32<T>(
-              tr_frag<DP>(lg, b * 32 + st * 16, db * 32, lane), pf, dv[db]);
-          dk[db] = mfma32<T>(
-              tr_frag<DP>(lq, b * 32 + st * 16, db * 32, lane), df, dk[db]);
+          dv[db] = mfma32<T>(fr.tr(lg, b * 32 + st * 16, db), pf, dv[db]);
+          dk[db] = mfma32<T>(fr.tr(lq, b * 32 + st * 16, db), df, dk[db]);
         }
       }
     }
+  };
+  for (int n = 0; n < all; n += 2) {
+    body(n, lds, stat[0]);
+    if (n + 1 < all) body(n + 1, lds + 2 * TS, stat[1]);
   }
   if (!real) return;
   store_rows<T, DP>(a.dk.p + token * a.dk.token + kvh * a.dk.head, dk, a.scale,

@@ -10,11 +10,12 @@
 // makes registers 8a..8a+7 of a result C the operand B of step a of a next
 // product whose k is C's m: a product's result feeds the next one without
 // leaving its lane.  The next product's A, read across its rows, is then two
-// transposing reads of four rows each (tr_frag).
+// transposing reads of four rows each (Frags::tr).
 //
-// LDS tiles are rows of DP elements in chunks of 8, chunk c of row r stored
-// at place c ^ (r & 7): reads of 32 rows at one chunk (row_frag) and of 8
-// rows at 4 chunks (tr_frag) both touch every bank evenly.
+// LDS tiles are rows of DP elements in chunks of 8 (16 bytes), chunk c of row
+// r stored at place c ^ swizzle(r).  The swizzle is linear in the row's bits
+// and chosen so that 8 rows at one chunk fill 128 bytes of banks and 16 rows
+// 256 (Frags::row), and 4 rows at four neighbouring chunks fill 256 (Frags::tr).
 #pragma once
 
 #include "seq_common.h"
@@ -66,31 +67,57 @@ template <typename T> DLX_DEV s16x8 pack_step(const float* p) {
                    pack2<T>(p[4], p[5]), pack2<T>(p[6], p[7])});
 }
 
+template <int DP> DLX_DEV constexpr int swizzle(int r) {
+  if (DP == 32) return ((r >> 2) & 1) | (((r >> 3) ^ (r >> 1)) & 1) << 1;
+  if (DP == 64)
+    return ((r >> 2) & 1) | ((r ^ (r >> 3)) & 1) << 1 | ((r >> 1) & 1) << 2;
+  return ((r >> 2) & 1) | (((r >> 1) ^ (r >> 3)) & 1) << 1 | (r & 1) << 2 |
+         ((r >> 1) & 1) << 3;
+}
+
 template <int DP> DLX_DEV int tile_at(int row, int chunk) {
-  return row * DP + ((chunk ^ (row & 7)) << 3);
+  return row * DP + ((chunk ^ swizzle<DP>(row)) << 3);
 }
 
-// operand A or B of step `step`: rows row0.. along m or n, k along the row
-template <int DP>
-DLX_DEV s16x8 row_frag(const uint16_t* tile, int row0, int step, int lane) {
-  return *reinterpret_cast<const s16x8*>(
-      tile + tile_at<DP>(row0 + (lane & 31), step * 2 + (lane >> 5)));
-}
+// Where a lane's fragments lie in a tile of DP columns, in elements.  The
+// swizzle leaves a place for each chunk a lane reads; rows are offsets that
+// fit the read instruction.
+template <int DP> struct Frags {
+  int row_[DP / 16], tr_[2][DP / 32];
 
-// operand A (or B) whose m (n) runs along the tile's rows, columns col0..31,
-// and whose k runs over its rows row0..row0+15 in the order of pack_step
-template <int DP>
-DLX_DEV s16x8 tr_frag(const uint16_t* tile, int row0, int col0, int lane) {
-  const int col = col0 + (lane & 16) + ((lane & 3) << 2);
-  const int row = row0 + ((lane >> 5) << 2) + ((lane & 15) >> 2);
-  auto* lo = (lds_tr_t*)(tile + tile_at<DP>(row, col >> 3) + (col & 7));
-  auto* hi = (lds_tr_t*)(tile + tile_at<DP>(row + 8, col >> 3) + (col & 7));
-  const s16x4 a = __builtin_bit_cast(
-      s16x4, __builtin_amdgcn_ds_read_tr16_b64_v4bf16(lo));
-  const s16x4 b = __builtin_bit_cast(
-      s16x4, __builtin_amdgcn_ds_read_tr16_b64_v4bf16(hi));
-  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-}
+  // col0: where column block 0 begins, a multiple of 32
+  DLX_DEV explicit Frags(int lane, int col0 = 0) {
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s)
+      row_[s] = tile_at<DP>(lane & 31, s * 2 + (lane >> 5));
+    const int row = ((lane >> 5) << 2) + ((lane & 15) >> 2);
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b) {
+      const int col = col0 + b * 32 + (lane & 16) + ((lane & 3) << 2);
+      tr_[0][b] = tile_at<DP>(row, col >> 3) + (col & 7);
+      tr_[1][b] = tile_at<DP>(row + 8, col >> 3) + (col & 7);
+    }
+  }
+
+  // operand A or B of step `step`: rows row0.. (a multiple of 16) along m or
+  // n, k along the row
+  DLX_DEV s16x8 row(const uint16_t* tile, int row0, int step) const {
+    return *reinterpret_cast<const s16x8*>(tile + row_[step] + row0 * DP);
+  }
+
+  // operand A (or B) whose m (n) runs along the tile's rows, columns
+  // col0 + 32 * block.., and whose k runs over its rows row0..row0+15 (row0 a
+  // multiple of 16) in the order of pack_step
+  DLX_DEV s16x8 tr(const uint16_t* tile, int row0, int block) const {
+    auto* lo = (lds_tr_t*)(tile + tr_[0][block] + row0 * DP);
+    auto* hi = (lds_tr_t*)(tile + tr_[1][block] + row0 * DP);
+    const s16x4 a = __builtin_bit_cast(
+        s16x4, __builtin_amdgcn_ds_read_tr16_b64_v4bf16(lo));
+    const s16x4 b = __builtin_bit_cast(
+        s16x4, __builtin_amdgcn_ds_read_tr16_b64_v4bf16(hi));
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+};
 
 // 16 bytes a lane from memory to LDS, lanes one behind the other there
 DLX_DEV void copy16_to_lds(const void* src, uint16_t* dst) {

@@ -21,9 +21,18 @@ CSRC = ROOT / "deeplearning_cfn_amd" / "ops" / "csrc"
 
 sources = sorted(str(p) for p in CSRC.glob("*.hip"))
 
+# The generated build rules do not follow the kernels' includes: an object
+# older than a header is built again.
+headers = sorted(CSRC.glob("*.h"))
+newest = max(p.stat().st_mtime for p in headers)
+for obj in (ROOT / "build").glob("temp.*/**/*.o"):
+    if obj.stat().st_mtime < newest:
+        obj.unlink()
+
 ext = cpp_extension.CUDAExtension(
     name="deeplearning_cfn_amd.ops._hip_ops",
     sources=sources,
+    depends=[str(p) for p in headers],
     extra_compile_args={
         "cxx": ["-O3", "-std=c++17"],
         # no packed-fp32 instructions: some of their forms have given wrong
