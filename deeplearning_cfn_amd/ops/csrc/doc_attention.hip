@@ -51,7 +51,9 @@ struct AttnArgs {
   float* delta;                       // [heads, tokens]
   const int* cu;
   const float* slopes;                // [heads] or none
-  int docs, tokens, heads, group, dim;
+  float* part;                        // dk, dv: [2, splits, tokens, kv_heads,
+                                      // dim] where the walk is split
+  int docs, tokens, heads, group, dim, splits;
   float scale;
 };
 
@@ -179,7 +181,7 @@ DLX_DEV f32x16 bias(float sl, int k0, int wave_row, int shift) {
 // ---------------------------------------------------------------------------
 
 template <typename T, int DP, int NW, bool BIAS>
-__global__ __launch_bounds__(NW * 64, 2) void doc_attn_fwd_kernel(AttnArgs a) {
+__global__ __launch_bounds__(NW * 64, DP == 64 ? 4 : 2) void doc_attn_fwd_kernel(AttnArgs a) {
   constexpr int NT = NW * 64, ROWS = NW * 32, TS = kKeys * DP;
   __shared__ __attribute__((aligned(16))) uint16_t lds[4 * TS];
 
@@ -209,7 +211,7 @@ __global__ __launch_bounds__(NW * 64, 2) void doc_attn_fwd_kernel(AttnArgs a) {
   s16x8 qf[DP / 16];
   load_rows<DP>(qf, a.q.p + token * a.q.token + head * a.q.head, a.dim, lane);
 
-  const Frags<DP> fr(lane);
+  const Frags<DP> fr(lds, lane);
   const float sc = a.scale * kLog2e;
   const float sl = BIAS ? a.slopes[head] / a.scale : 0.f;
   // m: what the row's exponents are taken next to; it follows the row's
@@ -218,10 +220,11 @@ __global__ __launch_bounds__(NW * 64, 2) void doc_attn_fwd_kernel(AttnArgs a) {
   float m = -INFINITY, ms = 0.f, l = 0.f;
   f32x16 acc[DP / 32] = {};
 
-  auto body = [&](int t, const uint16_t* lk, uint16_t* nx) {
+  auto body = [&](int t, auto half_) {
+    constexpr int LK = decltype(half_)::value * 2 * TS, LV = LK + TS;
+    uint16_t* nx = lds + (2 * TS - LK);
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    const uint16_t* lv = lk + TS;
     if (t + 1 < nt) {
       load_tile<DP, NT>(nx, kb, a.k.token, (t + 1) * kKeys, tl.len, a.dim);
       load_tile<DP, NT>(nx + TS, vb, a.v.token, (t + 1) * kKeys, tl.len, a.dim);
@@ -231,10 +234,13 @@ __global__ __launch_bounds__(NW * 64, 2) void doc_attn_fwd_kernel(AttnArgs a) {
     for (int b = 0; b < 2; ++b) {
       s[b] = BIAS ? bias(sl, t * kKeys + b * 32, wave_row, half * 4 - qpos)
                   : f32x16{};
-#pragma unroll
-      for (int st = 0; st < DP / 16; ++st)
-        s[b] = mfma32<T>(fr.row(lk, b * 32, st), qf[st], s[b]);
     }
+    // two sums in turn: a product does not wait for the one before it
+#pragma unroll
+    for (int st = 0; st < DP / 16; ++st)
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+        s[b] = mfma32<T>(fr.row(LK + b * 32 * DP, st), qf[st], s[b]);
     if ((t + 1) * kKeys > tl.len) {
       const int k0 = t * kKeys + half * 4;
 #pragma unroll
@@ -262,26 +268,26 @@ __global__ __launch_bounds__(NW * 64, 2) void doc_attn_fwd_kernel(AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[b][i] *= by;
     }
+    unroll<4>([&](auto n) {                     // 16 keys at a time
+      constexpr int b = n / 2, st = n % 2;
+      float p[8];
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        float p[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          p[e] = __builtin_amdgcn_exp2f(s[b][st * 8 + e] * sc - ms);
-          l += p[e];
-        }
-        const s16x8 pf = pack_step<T>(p);
-#pragma unroll
-        for (int db = 0; db < DP / 32; ++db)
-          acc[db] = mfma32<T>(fr.tr(lv, b * 32 + st * 16, db), pf, acc[db]);
+      for (int e = 0; e < 8; ++e) {
+        p[e] = __builtin_amdgcn_exp2f(s[b][st * 8 + e] * sc - ms);
+        l += p[e];
       }
+      const s16x8 pf = pack_step<T>(p);
+      s16x8 vf[DP / 32];
+      fr.template tr<DP / 32, LV + n * 16 * DP>(vf);
+#pragma unroll
+      for (int db = 0; db < DP / 32; ++db)
+        acc[db] = mfma32<T>(vf[db], pf, acc[db]);
+    });
   };
   // two tiles a turn, so that each half of LDS has its own addresses
   for (int t = 0; t < nt; t += 2) {
-    body(t, lds, lds + 2 * TS);
-    if (t + 1 < nt) body(t + 1, lds + 2 * TS, lds);
+    body(t, std::integral_constant<int, 0>{});
+    if (t + 1 < nt) body(t + 1, std::integral_constant<int, 1>{});
   }
   l += __shfl_xor(l, 32, kWave);
   if (!real) return;
@@ -297,7 +303,7 @@ __global__ __launch_bounds__(NW * 64, 2) void doc_attn_fwd_kernel(AttnArgs a) {
 // ---------------------------------------------------------------------------
 
 template <typename T, int DP, int NW, bool BIAS>
-__global__ __launch_bounds__(NW * 64, 2) void doc_attn_dq_kernel(AttnArgs a) {
+__global__ __launch_bounds__(NW * 64, DP == 64 ? 3 : 2) void doc_attn_dq_kernel(AttnArgs a) {
   constexpr int NT = NW * 64, ROWS = NW * 32, TS = kKeys * DP;
   __shared__ __attribute__((aligned(16))) uint16_t lds[4 * TS];
 
@@ -342,7 +348,7 @@ __global__ __launch_bounds__(NW * 64, 2) void doc_attn_dq_kernel(AttnArgs a) {
   }
   if (real && half == 0) a.delta[(long)head * a.tokens + token] = delta;
   const float lse = a.lse[(long)head * a.tokens + token];
-  const Frags<DP> fr(lane);
+  const Frags<DP> fr(lds, lane);
   const float sc = a.scale * kLog2e;
   const float sl = BIAS ? a.slopes[head] / a.scale : 0.f;
   f32x16 acc[DP / 32] = {};
@@ -350,25 +356,24 @@ __global__ __launch_bounds__(NW * 64, 2) void doc_attn_dq_kernel(AttnArgs a) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) less[i] = -delta;
 
-  auto body = [&](int t, const uint16_t* lk, uint16_t* nx) {
+  auto body = [&](int t, auto half_) {
+    constexpr int LK = decltype(half_)::value * 2 * TS, LV = LK + TS;
+    uint16_t* nx = lds + (2 * TS - LK);
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    const uint16_t* lv = lk + TS;
     if (t + 1 < nt) {
       load_tile<DP, NT>(nx, kb, a.k.token, (t + 1) * kKeys, tl.len, a.dim);
       load_tile<DP, NT>(nx + TS, vb, a.v.token, (t + 1) * kKeys, tl.len, a.dim);
     }
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    unroll<2>([&](auto b) {
       f32x16 s = BIAS ? bias(sl, t * kKeys + b * 32, wave_row, half * 4 - qpos)
                       : f32x16{};
       f32x16 dp = less;
 #pragma unroll
-      for (int st = 0; st < DP / 16; ++st)
-        s = mfma32<T>(fr.row(lk, b * 32, st), qf[st], s);
-#pragma unroll
-      for (int st = 0; st < DP / 16; ++st)
-        dp = mfma32<T>(fr.row(lv, b * 32, st), gf[st], dp);
+      for (int st = 0; st < DP / 16; ++st) {
+        s = mfma32<T>(fr.row(LK + b * 32 * DP, st), qf[st], s);
+        dp = mfma32<T>(fr.row(LV + b * 32 * DP, st), gf[st], dp);
+      }
       float ds[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i)
@@ -379,18 +384,19 @@ __global__ __launch_bounds__(NW * 64, 2) void doc_attn_dq_kernel(AttnArgs a) {
         for (int i = 0; i < 16; ++i)
           if (k0 + reg_row(i) >= tl.len) ds[i] = 0.f;
       }
-#pragma unroll
-      for (int st = 0; st < 2; ++st) {
+      unroll<2>([&](auto st) {
         const s16x8 df = pack_step<T>(&ds[st * 8]);
+        s16x8 kf[DP / 32];
+        fr.template tr<DP / 32, LK + (b * 2 + st) * 16 * DP>(kf);
 #pragma unroll
         for (int db = 0; db < DP / 32; ++db)
-          acc[db] = mfma32<T>(fr.tr(lk, b * 32 + st * 16, db), df, acc[db]);
-      }
-    }
+          acc[db] = mfma32<T>(kf[db], df, acc[db]);
+      });
+    });
   };
   for (int t = 0; t < nt; t += 2) {
-    body(t, lds, lds + 2 * TS);
-    if (t + 1 < nt) body(t + 1, lds + 2 * TS, lds);
+    body(t, std::integral_constant<int, 0>{});
+    if (t + 1 < nt) body(t + 1, std::integral_constant<int, 1>{});
   }
   if (real)
     store_rows<T, DP>(a.dq.p + token * a.dq.token + head * a.dq.head, acc,
@@ -399,7 +405,9 @@ __global__ __launch_bounds__(NW * 64, 2) void doc_attn_dq_kernel(AttnArgs a) {
 
 // ---------------------------------------------------------------------------
 // gradients of keys and values: a wave owns 32 keys of one key head; the
-// queries of every head that shares it pass in tiles of 64.
+// queries of every head that shares it pass in tiles of 64.  Shared heads
+// leave few such waves and give each a long walk: then the walk is split, its
+// parts' sums stay in fp32 and doc_attn_join_kernel adds them, in their order.
 // ---------------------------------------------------------------------------
 
 template <typename T, int DP, int NW, bool BIAS>
@@ -409,18 +417,26 @@ __global__ __launch_bounds__(NW * 64, 2) void doc_attn_dkv_kernel(AttnArgs a) {
   __shared__ __attribute__((aligned(16))) float stat[2][2][kKeys];
 
   const int kv_heads = a.heads / a.group;
-  const int tiles = gridDim.x / kv_heads;
+  const int tiles = gridDim.x / (kv_heads * a.splits);
   const int bid = xcd_block(blockIdx.x, gridDim.x);
-  const int kvh = bid / tiles;
-  const Tile tl = find_tile<ROWS>(a, bid - kvh * tiles);
+  const int kvh = bid / (tiles * a.splits);
+  const int split = (bid - kvh * tiles * a.splits) / tiles;
+  const Tile tl = find_tile<ROWS>(a, bid % tiles);
   if (tl.row0 >= tl.len) return;
   const int lane = threadIdx.x & (kWave - 1);
   const int wid = threadIdx.x / kWave;
   const int half = lane >> 5;
   const int kpos = tl.row0 + wid * 32 + (lane & 31);
   const bool real = kpos < tl.len;
+  const long half_part = (long)a.splits * a.tokens * kv_heads * a.dim;
+  auto part_row = [&](long t) {
+    return a.part + (((long)split * a.tokens + t) * kv_heads + kvh) * a.dim;
+  };
   if (!tl.doc) {
-    if (real) {
+    if (real && a.splits > 1) {
+      float* row = part_row(tl.start + kpos);
+      for (int c = half; c < a.dim; c += 2) row[c] = row[half_part + c] = 0.f;
+    } else if (real) {
       zero_rows<DP>(a.dk, tl.start + kpos, kvh, a.dim, lane);
       zero_rows<DP>(a.dv, tl.start + kpos, kvh, a.dim, lane);
     }
@@ -428,15 +444,15 @@ __global__ __launch_bounds__(NW * 64, 2) void doc_attn_dkv_kernel(AttnArgs a) {
   }
   const long token = tl.start + (real ? kpos : tl.len - 1);
   const int nt = (tl.len + kKeys - 1) / kKeys;
-  const int all = nt * a.group;
+  const int n0 = (int)((long)nt * a.group * split / a.splits);
+  const int n1 = (int)((long)nt * a.group * (split + 1) / a.splits);
 
   const float sc = a.scale * kLog2e, unit = 1.f / sc;
 
   // tile n of the walk: head kvh * group + n / nt, rows (n % nt) * 64..
-  auto stage = [&](int n) {
+  auto stage = [&](int n, uint16_t* at, float (*st)[kKeys]) {
     const int head = kvh * a.group + n / nt;
     const int row0 = (n % nt) * kKeys;
-    uint16_t* at = lds + (n & 1) * 2 * TS;
     load_tile<DP, NT>(at, a.q.p + tl.start * a.q.token + head * a.q.head,
                       a.q.token, row0, tl.len, a.dim);
     load_tile<DP, NT>(at + TS,
@@ -446,25 +462,26 @@ __global__ __launch_bounds__(NW * 64, 2) void doc_attn_dkv_kernel(AttnArgs a) {
       // what S and dP begin at; behind the document's end exp2(-inf) is 0
       const int r = row0 + threadIdx.x;
       const long i = (long)head * a.tokens + tl.start + r;
-      stat[n & 1][0][threadIdx.x] = r < tl.len ? a.lse[i] * -unit : -INFINITY;
-      stat[n & 1][1][threadIdx.x] = r < tl.len ? -a.delta[i] : 0.f;
+      st[0][threadIdx.x] = r < tl.len ? a.lse[i] * -unit : -INFINITY;
+      st[1][threadIdx.x] = r < tl.len ? -a.delta[i] : 0.f;
     }
   };
-  stage(0);
+  if (n0 < n1) stage(n0, lds, stat[0]);
   s16x8 kf[DP / 16], vf[DP / 16];
   load_rows<DP>(kf, a.k.p + token * a.k.token + kvh * a.k.head, a.dim, lane);
   load_rows<DP>(vf, a.v.p + token * a.v.token + kvh * a.v.head, a.dim, lane);
-  const Frags<DP> fr(lane);
+  const Frags<DP> fr(lds, lane);
   f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
 
-  auto body = [&](int n, const uint16_t* lq, const float (*st_)[kKeys]) {
+  auto body = [&](int n, auto half_) {
+    constexpr int H = decltype(half_)::value;
+    constexpr int LQ = H * 2 * TS, LG = LQ + TS;
+    const float (*st_)[kKeys] = stat[H];
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    if (n + 1 < all) stage(n + 1);
-    const uint16_t* lg = lq + TS;
+    if (n + 1 < n1) stage(n + 1, lds + (2 * TS - LQ), stat[1 - H]);
     const float sl = BIAS ? a.slopes[kvh * a.group + n / nt] / a.scale : 0.f;
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    unroll<2>([&](auto b) {
       const int q0 = b * 32 + half * 4;
       const float d0 = (float)((n % nt) * kKeys + q0 - kpos);
       f32x16 s, dp;
@@ -480,13 +497,11 @@ __global__ __launch_bounds__(NW * 64, 2) void doc_attn_dkv_kernel(AttnArgs a) {
         }
       }
 #pragma unroll
-      for (int st = 0; st < DP / 16; ++st)
-        s = mfma32<T>(fr.row(lq, b * 32, st), kf[st], s);
-#pragma unroll
-      for (int st = 0; st < DP / 16; ++st)
-        dp = mfma32<T>(fr.row(lg, b * 32, st), vf[st], dp);
-#pragma unroll
-      for (int st = 0; st < 2; ++st) {
+      for (int st = 0; st < DP / 16; ++st) {
+        s = mfma32<T>(fr.row(LQ + b * 32 * DP, st), kf[st], s);
+        dp = mfma32<T>(fr.row(LG + b * 32 * DP, st), vf[st], dp);
+      }
+      unroll<2>([&](auto st) {
         float p[8], ds[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -495,23 +510,73 @@ __global__ __launch_bounds__(NW * 64, 2) void doc_attn_dkv_kernel(AttnArgs a) {
         }
         const s16x8 pf = pack_step<T>(p);
         const s16x8 df = pack_step<T>(ds);
-#pragma unroll
-        for (int db = 0; db < DP / 32; ++db) {
-          dv[db] = mfma32<T>(fr.tr(lg, b * 32 + st * 16, db), pf, dv[db]);
-          dk[db] = mfma32<T>(fr.tr(lq, b * 32 + st * 16, db), df, dk[db]);
-        }
-      }
-    }
+        constexpr int at = (b * 2 + st) * 16 * DP;
+        unroll<DP / 64>([&](auto h) {           // two operands at a time
+          s16x8 f[2];
+          fr.template tr<2, LG + at, h * 2>(f);
+          dv[h * 2] = mfma32<T>(f[0], pf, dv[h * 2]);
+          dv[h * 2 + 1] = mfma32<T>(f[1], pf, dv[h * 2 + 1]);
+          fr.template tr<2, LQ + at, h * 2>(f);
+          dk[h * 2] = mfma32<T>(f[0], df, dk[h * 2]);
+          dk[h * 2 + 1] = mfma32<T>(f[1], df, dk[h * 2 + 1]);
+        });
+      });
+    });
   };
-  for (int n = 0; n < all; n += 2) {
-    body(n, lds, stat[0]);
-    if (n + 1 < all) body(n + 1, lds + 2 * TS, stat[1]);
+  for (int n = n0; n < n1; n += 2) {
+    body(n, std::integral_constant<int, 0>{});
+    if (n + 1 < n1) body(n + 1, std::integral_constant<int, 1>{});
   }
   if (!real) return;
+  if (a.splits > 1) {
+    float* row = part_row(token);
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = b * 32 + g * 8 + half * 4;
+        if (d >= a.dim) continue;
+        *reinterpret_cast<F32x4*>(row + d) =
+            F32x4{{dk[b][g * 4], dk[b][g * 4 + 1], dk[b][g * 4 + 2],
+                   dk[b][g * 4 + 3]}};
+        *reinterpret_cast<F32x4*>(row + half_part + d) =
+            F32x4{{dv[b][g * 4], dv[b][g * 4 + 1], dv[b][g * 4 + 2],
+                   dv[b][g * 4 + 3]}};
+      }
+    return;
+  }
   store_rows<T, DP>(a.dk.p + token * a.dk.token + kvh * a.dk.head, dk, a.scale,
                     a.dim, lane);
   store_rows<T, DP>(a.dv.p + token * a.dv.token + kvh * a.dv.head, dv, 1.f,
                     a.dim, lane);
+}
+
+// The sums of a split walk: eight columns of dk or dv a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void doc_attn_join_kernel(AttnArgs a) {
+  const int kv_heads = a.heads / a.group, chunks = a.dim / 8;
+  const long rows = (long)a.tokens * kv_heads, half = rows * chunks;
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= 2 * half) return;
+  const bool is_v = i >= half;
+  const long at = is_v ? i - half : i;
+  const long row = at / chunks, token = row / kv_heads;
+  const int c = (int)(at - row * chunks) * 8;
+  const int head = (int)(row - token * kv_heads);
+  const long stride = rows * a.dim;
+  const float* p =
+      a.part + (is_v ? a.splits * stride : 0) + row * a.dim + c;
+  float x[8] = {};
+  for (int s = 0; s < a.splits; ++s, p += stride)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] += p[e];
+  const float by = is_v ? 1.f : a.scale;
+  const View& v = is_v ? a.dv : a.dk;
+  Pack<uint32_t, 4> y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y.v[e] = pack2<T>(x[2 * e] * by, x[2 * e + 1] * by);
+  *reinterpret_cast<Pack<uint32_t, 4>*>(v.p + token * v.token + head * v.head +
+                                        c) = y;
 }
 
 // ---------------------------------------------------------------------------
@@ -596,8 +661,8 @@ enum { kFwd, kDq, kDkv };
 
 template <typename T, int DP, int NW, bool BIAS>
 void launch_one(int which, const AttnArgs& a, hipStream_t s) {
-  const unsigned b =
-      blocks_of(a, NW * 32, which == kDkv ? a.heads / a.group : a.heads);
+  const unsigned b = blocks_of(
+      a, NW * 32, which == kDkv ? a.heads / a.group * a.splits : a.heads);
   if (which == kFwd)
     doc_attn_fwd_kernel<T, DP, NW, BIAS><<<b, NW * 64, 0, s>>>(a);
   else if (which == kDq)
@@ -687,7 +752,24 @@ void doc_attn_bwd_impl(const at::Tensor& dout_in, const at::Tensor& q_in,
   a.delta = delta.data_ptr<float>();
   const auto s = at::cuda::getCurrentCUDAStream();
   launch(kDq, a, q.scalar_type(), s);
+  // a wave owns 32 keys of a key head: the walk over a group's queries is
+  // split until there are about four waves to each of the 1024 SIMDs
+  const long waves = ((long)a.tokens / 32 + 1) * k.size(1);
+  a.splits = 1;
+  while (a.splits < a.group && waves * a.splits < 4096) ++a.splits;
+  at::Tensor part;
+  if (a.splits > 1) {
+    part = at::empty({2l * a.splits * k.numel()}, lse.options());
+    a.part = part.data_ptr<float>();
+  }
   launch(kDkv, a, q.scalar_type(), s);
+  if (a.splits > 1) {
+    const long n = (k.numel() / 4 + 255) / 256;   // two tensors, 8 a thread
+    if (q.scalar_type() == at::kBFloat16)
+      doc_attn_join_kernel<BF16><<<(unsigned)n, 256, 0, s>>>(a);
+    else
+      doc_attn_join_kernel<FP16><<<(unsigned)n, 256, 0, s>>>(a);
+  }
 }
 
 }  // namespace dlx

@@ -18,6 +18,9 @@
 // 256 (Frags::row), and 4 rows at four neighbouring chunks fill 256 (Frags::tr).
 #pragma once
 
+#include <type_traits>
+#include <utility>
+
 #include "seq_common.h"
 
 namespace dlx {
@@ -25,7 +28,6 @@ namespace dlx {
 using f32x16 = __attribute__((ext_vector_type(16))) float;
 using s16x8 = __attribute__((ext_vector_type(8))) short;
 using s16x4 = __attribute__((ext_vector_type(4))) short;
-using bf16v4_t = __attribute__((ext_vector_type(4))) __bf16;
 using bf16v8_t = __attribute__((ext_vector_type(8))) __bf16;
 using f16v8_t = __attribute__((ext_vector_type(8))) _Float16;
 using bf16v2_t = __attribute__((ext_vector_type(2))) __bf16;
@@ -35,7 +37,6 @@ using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
 
 typedef __attribute__((address_space(3))) uint32_t lds_word_t;
 typedef const __attribute__((address_space(1))) uint32_t glb_word_t;
-typedef __attribute__((address_space(3))) bf16v4_t lds_tr_t;
 
 template <typename T> DLX_DEV f32x16 mfma32(s16x8 a, s16x8 b, f32x16 c);
 template <> DLX_DEV f32x16 mfma32<BF16>(s16x8 a, s16x8 b, f32x16 c) {
@@ -79,14 +80,75 @@ template <int DP> DLX_DEV int tile_at(int row, int chunk) {
   return row * DP + ((chunk ^ swizzle<DP>(row)) << 3);
 }
 
-// Where a lane's fragments lie in a tile of DP columns, in elements.  The
-// swizzle leaves a place for each chunk a lane reads; rows are offsets that
-// fit the read instruction.
-template <int DP> struct Frags {
-  int row_[DP / 16], tr_[2][DP / 32];
+// f(0), f(1), .. with numbers that are known when it is compiled
+template <class F, int... I>
+DLX_DEV void unroll_(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F> DLX_DEV void unroll(F&& f) {
+  unroll_(f, std::make_integer_sequence<int, N>{});
+}
 
-  // col0: where column block 0 begins, a multiple of 32
-  DLX_DEV explicit Frags(int lane, int col0 = 0) {
+// Transposing reads, 2 N of them, at byte OFF from each lane's places.  The
+// builtin would do, but the compiler cannot tell its reads from the tile that
+// copy16_to_lds is filling and waits for that first, at every tile.  The wait
+// for the reads themselves is part of the block.
+template <int OFF>
+DLX_DEV void read_tr2(uint32_t p0, uint32_t p1, s16x4& a, s16x4& b) {
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %2 offset:%4\n\t"
+      "ds_read_b64_tr_b16 %1, %3 offset:%4\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(a), "=&v"(b)
+      : "v"(p0), "v"(p1), "i"(OFF)
+      : "memory");
+}
+
+template <int OFF>
+DLX_DEV void read_tr4(const uint32_t* p, const uint32_t* q, s16x4* a,
+                      s16x4* b) {
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %4 offset:%8\n\t"
+      "ds_read_b64_tr_b16 %1, %5 offset:%8\n\t"
+      "ds_read_b64_tr_b16 %2, %6 offset:%8\n\t"
+      "ds_read_b64_tr_b16 %3, %7 offset:%8\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(a[0]), "=&v"(b[0]), "=&v"(a[1]), "=&v"(b[1])
+      : "v"(p[0]), "v"(q[0]), "v"(p[1]), "v"(q[1]), "i"(OFF)
+      : "memory");
+}
+
+template <int OFF>
+DLX_DEV void read_tr8(const uint32_t* p, const uint32_t* q, s16x4* a,
+                      s16x4* b) {
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8 offset:%16\n\t"
+      "ds_read_b64_tr_b16 %1, %9 offset:%16\n\t"
+      "ds_read_b64_tr_b16 %2, %10 offset:%16\n\t"
+      "ds_read_b64_tr_b16 %3, %11 offset:%16\n\t"
+      "ds_read_b64_tr_b16 %4, %12 offset:%16\n\t"
+      "ds_read_b64_tr_b16 %5, %13 offset:%16\n\t"
+      "ds_read_b64_tr_b16 %6, %14 offset:%16\n\t"
+      "ds_read_b64_tr_b16 %7, %15 offset:%16\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(a[0]), "=&v"(b[0]), "=&v"(a[1]), "=&v"(b[1]), "=&v"(a[2]),
+        "=&v"(b[2]), "=&v"(a[3]), "=&v"(b[3])
+      : "v"(p[0]), "v"(q[0]), "v"(p[1]), "v"(q[1]), "v"(p[2]), "v"(q[2]),
+        "v"(p[3]), "v"(q[3]), "i"(OFF)
+      : "memory");
+}
+
+// Where a lane's fragments lie in a tile of DP columns.  The swizzle leaves a
+// place for each chunk a lane reads; rows are offsets that fit the read
+// instruction.
+template <int DP> struct Frags {
+  const uint16_t* lds;
+  int row_[DP / 16];                  // elements from `lds`
+  uint32_t lo_[DP / 32], hi_[DP / 32];  // LDS addresses
+
+  // base: what the offsets of row() and tr() are taken from; col0: where
+  // tr's block 0 begins, a multiple of 32
+  DLX_DEV Frags(const uint16_t* base, int lane, int col0 = 0) : lds(base) {
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s)
       row_[s] = tile_at<DP>(lane & 31, s * 2 + (lane >> 5));
@@ -94,28 +156,42 @@ template <int DP> struct Frags {
 #pragma unroll
     for (int b = 0; b < DP / 32; ++b) {
       const int col = col0 + b * 32 + (lane & 16) + ((lane & 3) << 2);
-      tr_[0][b] = tile_at<DP>(row, col >> 3) + (col & 7);
-      tr_[1][b] = tile_at<DP>(row + 8, col >> 3) + (col & 7);
+      lo_[b] = address(base + tile_at<DP>(row, col >> 3) + (col & 7));
+      hi_[b] = address(base + tile_at<DP>(row + 8, col >> 3) + (col & 7));
     }
   }
 
-  // operand A or B of step `step`: rows row0.. (a multiple of 16) along m or
-  // n, k along the row
-  DLX_DEV s16x8 row(const uint16_t* tile, int row0, int step) const {
-    return *reinterpret_cast<const s16x8*>(tile + row_[step] + row0 * DP);
+  static DLX_DEV uint32_t address(const uint16_t* p) {
+    return (uint32_t)(uintptr_t)(
+        const __attribute__((address_space(3))) uint16_t*)p;
   }
 
-  // operand A (or B) whose m (n) runs along the tile's rows, columns
-  // col0 + 32 * block.., and whose k runs over its rows row0..row0+15 (row0 a
+  // operand A or B of step `step`, k along the rows: rows off / DP ..+31, the
+  // first a multiple of 16
+  DLX_DEV s16x8 row(int off, int step) const {
+    return *reinterpret_cast<const s16x8*>(lds + row_[step] + off);
+  }
+
+  // N operands A (or B) whose m (n) runs along the rows, columns col0 + 32
+  // (FIRST + n) .., and whose k runs over rows OFF / DP ..+15 (the first a
   // multiple of 16) in the order of pack_step
-  DLX_DEV s16x8 tr(const uint16_t* tile, int row0, int block) const {
-    auto* lo = (lds_tr_t*)(tile + tr_[0][block] + row0 * DP);
-    auto* hi = (lds_tr_t*)(tile + tr_[1][block] + row0 * DP);
-    const s16x4 a = __builtin_bit_cast(
-        s16x4, __builtin_amdgcn_ds_read_tr16_b64_v4bf16(lo));
-    const s16x4 b = __builtin_bit_cast(
-        s16x4, __builtin_amdgcn_ds_read_tr16_b64_v4bf16(hi));
-    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  // `more`: bytes further on, where an offset would not fit
+  template <int N, int OFF, int FIRST = 0>
+  DLX_DEV void tr(s16x8* f, uint32_t more = 0) const {
+    s16x4 a[N], b[N];
+    static_assert(OFF * 2 < 65536 && (N == 1 || N == 2 || N == 4), "");
+    uint32_t lo[N], hi[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      lo[i] = lo_[FIRST + i] + more;
+      hi[i] = hi_[FIRST + i] + more;
+    }
+    if constexpr (N == 1) read_tr2<OFF * 2>(lo[0], hi[0], a[0], b[0]);
+    if constexpr (N == 2) read_tr4<OFF * 2>(lo, hi, a, b);
+    if constexpr (N == 4) read_tr8<OFF * 2>(lo, hi, a, b);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      f[i] = __builtin_shufflevector(a[i], b[i], 0, 1, 2, 3, 4, 5, 6, 7);
   }
 };
 

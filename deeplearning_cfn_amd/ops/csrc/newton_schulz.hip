@@ -28,7 +28,7 @@ namespace dlx {
 
 namespace {
 
-constexpr int kTile = 128;            // output tile, and what sizes pad to
+constexpr int kTile = 128;            // the smaller output tile
 constexpr int kDepth = 64;            // of a stage along k
 constexpr float kXScale = 4096.f;
 constexpr float kNsA = 3.4445f, kNsB = -4.7750f, kNsC = 2.0315f;
@@ -42,13 +42,13 @@ DLX_DEV constexpr int quad_swap(int k) {
 DLX_DEV float h2f(uint16_t h) { return to_f32<FP16>(FP16{h}); }
 
 // Rows row0.. of [., ld] into an LDS tile of DP columns from col0 on.
-template <int ROWS, int DP>
+template <int ROWS, int DP, int NT>
 DLX_DEV void stage_tile(uint16_t* lds, const uint16_t* src, long ld, int row0,
                         int col0) {
   constexpr int CH = DP / 8;
 #pragma unroll
-  for (int u = 0; u < ROWS * CH / 256; ++u) {
-    const int f = u * 256 + threadIdx.x;
+  for (int u = 0; u < ROWS * CH / NT; ++u) {
+    const int f = u * NT + threadIdx.x;
     const int row = f / CH;
     const int chunk = (f % CH) ^ swizzle<DP>(row);
     copy16_to_lds(src + (row0 + row) * ld + col0 + chunk * 8, lds + f * 8);
@@ -131,65 +131,76 @@ __global__ __launch_bounds__(256) void ns_split_kernel(
   }
 }
 
+// Output tiles are TILE x TILE, by WM x WN waves.  A tile reads 2 TILE / 64
+// bytes for every thousand operations, which 128 leaves to the L2s' rate and
+// 256 does not; but 256 leaves few tiles.
+template <int TILE> struct Shape;
+template <> struct Shape<128> { static constexpr int WM = 2, WN = 2; };
+template <> struct Shape<256> { static constexpr int WM = 2, WN = 4; };
+
 // out = by (in in^T)              POLY false: A from X
 // out = b in + c (in in^T)        POLY true: B from A, columns quad-swapped
-template <bool POLY>
-__global__ __launch_bounds__(256) void ns_square_kernel(
-    const uint16_t* __restrict__ in, uint16_t* __restrict__ out, int np, int kp,
-    int pairs) {
-  constexpr int TS = kTile * kDepth;
+template <int TILE, bool POLY>
+__global__ __launch_bounds__(Shape<TILE>::WM* Shape<TILE>::WN* kWave) void
+ns_square_kernel(const uint16_t* __restrict__ in, uint16_t* __restrict__ out,
+                 int np, int kp, int pairs) {
+  constexpr int WM = Shape<TILE>::WM, WN = Shape<TILE>::WN;
+  constexpr int NT = WM * WN * kWave, TS = TILE * kDepth;
+  constexpr int FM = TILE / WM / 32, FN = TILE / WN / 32;
   __shared__ __attribute__((aligned(16))) uint16_t lds[4 * TS];
   const int blk = xcd_block(blockIdx.x, gridDim.x);
   const int batch = blk / pairs;
   int rest = blk - batch * pairs, bi = 0;
-  const int nb = np / kTile;
+  const int nb = np / TILE;
   while (rest >= nb - bi) rest -= nb - bi++;
   const int bj = bi + rest;                   // bj >= bi
   const uint16_t* src = in + (long)batch * np * kp;
   uint16_t* dst = out + (long)batch * np * np;
-  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-  const int wr = wid >> 1, wc = wid & 1;
+  const int lane = threadIdx.x & 63;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int wr = wid / WN, wc = wid % WN;
 
-  const Frags<kDepth> fr(lane);
-  f32x16 acc[2][2] = {};
+  const Frags<kDepth> fr(lds, lane);
+  f32x16 acc[FM][FN] = {};
   const int nt = kp / kDepth;
-  stage_tile<kTile, kDepth>(lds, src, kp, bj * kTile, 0);
-  stage_tile<kTile, kDepth>(lds + TS, src, kp, bi * kTile, 0);
+  stage_tile<TILE, kDepth, NT>(lds, src, kp, bj * TILE, 0);
+  stage_tile<TILE, kDepth, NT>(lds + TS, src, kp, bi * TILE, 0);
   for (int t = 0; t < nt; ++t) {
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    const uint16_t* la = lds + (t & 1) * 2 * TS;
-    const uint16_t* lb = la + TS;
+    const int la = (t & 1) * 2 * TS, lb = la + TS;
     if (t + 1 < nt) {
       uint16_t* nx = lds + ((t + 1) & 1) * 2 * TS;
-      stage_tile<kTile, kDepth>(nx, src, kp, bj * kTile, (t + 1) * kDepth);
-      stage_tile<kTile, kDepth>(nx + TS, src, kp, bi * kTile, (t + 1) * kDepth);
+      stage_tile<TILE, kDepth, NT>(nx, src, kp, bj * TILE, (t + 1) * kDepth);
+      stage_tile<TILE, kDepth, NT>(nx + TS, src, kp, bi * TILE,
+                                   (t + 1) * kDepth);
     }
 #pragma unroll
     for (int st = 0; st < kDepth / 16; ++st) {
-      s16x8 fa[2], fb[2];
+      s16x8 fa[FM], fb[FN];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        fa[u] = fr.row(la, wr * 64 + u * 32, st);
-        fb[u] = fr.row(lb, wc * 64 + u * 32, st);
-      }
+      for (int u = 0; u < FM; ++u)
+        fa[u] = fr.row(la + (wr * FM + u) * 32 * kDepth, st);
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < FN; ++u)
+        fb[u] = fr.row(lb + (wc * FN + u) * 32 * kDepth, st);
 #pragma unroll
-        for (int v = 0; v < 2; ++v)
+      for (int u = 0; u < FM; ++u)
+#pragma unroll
+        for (int v = 0; v < FN; ++v)
           acc[u][v] = mfma32<FP16>(fa[u], fb[v], acc[u][v]);
     }
   }
   constexpr float by = POLY ? kNsC : 1.f / (kXScale * kXScale);
 #pragma unroll
-  for (int u = 0; u < 2; ++u)
+  for (int u = 0; u < FM; ++u)
 #pragma unroll
-    for (int v = 0; v < 2; ++v) {
-      const int i = bi * kTile + wc * 64 + v * 32 + (lane & 31);
+    for (int v = 0; v < FN; ++v) {
+      const int i = bi * TILE + (wc * FN + v) * 32 + (lane & 31);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int j =
-            bj * kTile + wr * 64 + u * 32 + q * 8 + (lane >> 5) * 4;
+            bj * TILE + (wr * FM + u) * 32 + q * 8 + (lane >> 5) * 4;
         float x[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] = acc[u][v][q * 4 + e] * by;
@@ -223,112 +234,119 @@ struct NsUpdate {
 };
 
 // a X + B X
-template <bool LAST>
-__global__ __launch_bounds__(256) void ns_update_kernel(NsUpdate a) {
-  constexpr int TB = kTile * kDepth, TX = kDepth * kTile;
-  __shared__ __attribute__((aligned(16))) uint16_t lds[2 * (TB + TX)];
-  const int nbi = a.np / kTile, nbj = a.mp / kTile;
+template <int TILE, bool LAST>
+__global__ __launch_bounds__(Shape<TILE>::WM* Shape<TILE>::WN* kWave) void
+ns_update_kernel(NsUpdate a) {
+  constexpr int WM = Shape<TILE>::WM, WN = Shape<TILE>::WN;
+  constexpr int NT = WM * WN * kWave, TS = TILE * kDepth;
+  constexpr int FM = TILE / WM / 32, FN = TILE / WN / 32;
+  __shared__ __attribute__((aligned(16))) uint16_t lds[4 * TS];
+  const int nbi = a.np / TILE, nbj = a.mp / TILE;
   int blk = xcd_block(blockIdx.x, gridDim.x);
   const int batch = blk / (nbi * nbj);
   blk -= batch * nbi * nbj;
   const int bj = blk / nbi, bi = blk - bj * nbi;
   const uint16_t* bm = a.b + (long)batch * a.np * a.np;
   const long xo = (long)batch * a.np * a.mp;
-  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-  const int wr = wid >> 1, wc = wid & 1;
+  const int lane = threadIdx.x & 63;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int wr = wid / WN, wc = wid % WN;
 
-  const Frags<kDepth> fr(lane);
-  const Frags<kTile> fx(lane, wr * 64);
-  f32x16 acc[2][2] = {};
+  const Frags<kDepth> fr(lds, lane);
+  const Frags<TILE> fx(lds, lane, wr * FM * 32);
+  f32x16 acc[FM][FN] = {};
   const int nt = a.np / kDepth;
-  stage_tile<kDepth, kTile>(lds, a.xh + xo, a.mp, 0, bj * kTile);
-  stage_tile<kTile, kDepth>(lds + TX, bm, a.np, bi * kTile, 0);
-  for (int t = 0; t < nt; ++t) {
+  stage_tile<kDepth, TILE, NT>(lds, a.xh + xo, a.mp, 0, bj * TILE);
+  stage_tile<TILE, kDepth, NT>(lds + TS, bm, a.np, bi * TILE, 0);
+  auto step = [&](int t, auto half) {
+    // the X tile of a turn at half * TS, so that its offsets stay short
+    constexpr int LX = decltype(half)::value * 2 * TS, LB = LX + TS;
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    const uint16_t* lx = lds + (t & 1) * (TB + TX);
-    const uint16_t* lb = lx + TX;
     if (t + 1 < nt) {
-      uint16_t* nx = lds + ((t + 1) & 1) * (TB + TX);
-      stage_tile<kDepth, kTile>(nx, a.xh + xo, a.mp, (t + 1) * kDepth,
-                                bj * kTile);
-      stage_tile<kTile, kDepth>(nx + TX, bm, a.np, bi * kTile,
-                                (t + 1) * kDepth);
+      uint16_t* nx = lds + (2 * TS - LX);
+      stage_tile<kDepth, TILE, NT>(nx, a.xh + xo, a.mp, (t + 1) * kDepth,
+                                   bj * TILE);
+      stage_tile<TILE, kDepth, NT>(nx + TS, bm, a.np, bi * TILE,
+                                   (t + 1) * kDepth);
     }
+    unroll<kDepth / 16>([&](auto st) {
+      s16x8 fa[FM], fb[FN];
 #pragma unroll
-    for (int st = 0; st < kDepth / 16; ++st) {
-      s16x8 fa[2], fb[2];
+      for (int u = 0; u < FN; ++u)
+        fb[u] = fr.row(LB + (wc * FN + u) * 32 * kDepth, st);
+      fx.template tr<FM, st * 16 * TILE>(fa, LX * 2);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        fa[u] = fx.tr(lx, st * 16, u);
-        fb[u] = fr.row(lb, wc * 64 + u * 32, st);
-      }
+      for (int u = 0; u < FM; ++u)
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int v = 0; v < 2; ++v)
+        for (int v = 0; v < FN; ++v)
           acc[u][v] = mfma32<FP16>(fa[u], fb[v], acc[u][v]);
-    }
+    });
+  };
+  for (int t = 0; t < nt; t += 2) {
+    step(t, std::integral_constant<int, 0>{});
+    if (t + 1 < nt) step(t + 1, std::integral_constant<int, 1>{});
   }
-  // Through LDS as fp32 rows of X, so that memory sees whole lines.  Chunk c
-  // of 4 in row i lies at c ^ (i & 31).
-  __syncthreads();
+
+  // Through LDS as fp32 rows of X, 32 of each column of waves a turn, so that
+  // memory sees whole lines.  Chunk c of 4 in a row lies at c ^ (row & 31).
   float* img = reinterpret_cast<float*>(lds);
+  uint16_t* out = LAST ? a.out + (long)batch * a.rows * a.cols : nullptr;
+  constexpr int PR = TILE / 8;                 // threads to a row
+  using P8 = Pack<uint16_t, 8>;
+  const int cj = threadIdx.x % PR * 8;
+  const int j = bj * TILE + cj;
+  auto place = [&](int row, int chunk) {
+    return img + row * TILE + ((chunk ^ (row & 31)) << 2);
+  };
 #pragma unroll
-  for (int u = 0; u < 2; ++u)
+  for (int v = 0; v < FN; ++v) {
+    __syncthreads();
 #pragma unroll
-    for (int v = 0; v < 2; ++v) {
-      const int i = wc * 64 + v * 32 + (lane & 31);
+    for (int u = 0; u < FM; ++u)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int c = (wr * 64 + u * 32 + q * 8 + (lane >> 5) * 4) >> 2;
-        *reinterpret_cast<F32x4*>(img + i * kTile + ((c ^ (i & 31)) << 2)) =
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<F32x4*>(
+            place(wc * 32 + (lane & 31),
+                  ((wr * FM + u) * 32 + q * 8 + (lane >> 5) * 4) >> 2)) =
             F32x4{{acc[u][v][q * 4], acc[u][v][q * 4 + 1],
                    acc[u][v][q * 4 + 2], acc[u][v][q * 4 + 3]}};
-      }
-    }
-  __syncthreads();
-  const int cj = (threadIdx.x & 15) * 8;
-  const int j = bj * kTile + cj;
+    __syncthreads();
 #pragma unroll 2
-  for (int p = 0; p < kTile / 16; ++p) {
-    const int il = p * 16 + (threadIdx.x >> 4);
-    const int i = bi * kTile + il;
-    const long o = xo + (long)i * a.mp + j;
-    using P8 = Pack<uint16_t, 8>;
-    const P8 h = *reinterpret_cast<const P8*>(a.xh + o);
-    P8 l = {};
-    if (a.xl) l = *reinterpret_cast<const P8*>(a.xl + o);
-    float x[8];
+    for (int row = threadIdx.x / PR; row < WN * 32; row += NT / PR) {
+      const int i = bi * TILE + (row / 32 * FN + v) * 32 + row % 32;
+      const long o = xo + (long)i * a.mp + j;
+      const P8 h = *reinterpret_cast<const P8*>(a.xh + o);
+      P8 l = {};
+      if (a.xl) l = *reinterpret_cast<const P8*>(a.xl + o);
+      float x[8];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const F32x4 y = *reinterpret_cast<const F32x4*>(
-          img + il * kTile + ((((cj >> 2) + e) ^ (il & 31)) << 2));
+      for (int e = 0; e < 2; ++e) {
+        const F32x4 y =
+            *reinterpret_cast<const F32x4*>(place(row, (cj >> 2) + e));
 #pragma unroll
-      for (int k = 0; k < 4; ++k) x[e * 4 + k] = y.v[k];
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float w = h2f(h.v[e]);
-      if (a.xl) w += h2f(l.v[e]);
-      x[e] += kNsA * w;
-    }
-    if (!LAST) {
-      P8 yh, yl;
+        for (int k = 0; k < 4; ++k) x[e * 4 + k] = y.v[k];
+      }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        yh.v[e] = from_f32<FP16>(x[e]).v;
-        yl.v[e] = from_f32<FP16>(x[e] - h2f(yh.v[e])).v;
+        float w = h2f(h.v[e]);
+        if (a.xl) w += h2f(l.v[e]);
+        x[e] += kNsA * w;
       }
-      *reinterpret_cast<P8*>(a.yh + o) = yh;
-      if (a.yl) *reinterpret_cast<P8*>(a.yl + o) = yl;
-    } else {
-      P8 y;
+      if (!LAST) {
+        P8 yh, yl;
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        y.v[e] = from_f32<BF16>(x[e] * (1.f / kXScale)).v;
-      uint16_t* out = a.out + (long)batch * a.rows * a.cols;
-      if (!a.tall) {
+        for (int e = 0; e < 8; ++e) {
+          yh.v[e] = from_f32<FP16>(x[e]).v;
+          yl.v[e] = from_f32<FP16>(x[e] - h2f(yh.v[e])).v;
+        }
+        *reinterpret_cast<P8*>(a.yh + o) = yh;
+        if (a.yl) *reinterpret_cast<P8*>(a.yl + o) = yl;
+      } else if (!a.tall) {
+        P8 y;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          y.v[e] = from_f32<BF16>(x[e] * (1.f / kXScale)).v;
         uint16_t* at = out + (long)i * a.cols + j;
         if (i < a.rows) {
           if (a.cols % 8 == 0 && j < a.cols) {
@@ -343,30 +361,191 @@ __global__ __launch_bounds__(256) void ns_update_kernel(NsUpdate a) {
         // back into the image: its columns are the result's rows
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          *reinterpret_cast<F32x4*>(
-              img + il * kTile + ((((cj >> 2) + e) ^ (il & 31)) << 2)) =
-              F32x4{{x[e * 4], x[e * 4 + 1], x[e * 4 + 2], x[e * 4 + 3]}};
+          *reinterpret_cast<F32x4*>(place(row, (cj >> 2) + e)) = F32x4{
+              {x[e * 4], x[e * 4 + 1], x[e * 4 + 2], x[e * 4 + 3]}};
+      }
+    }
+    if (LAST && a.tall) {
+      __syncthreads();
+      const int row = threadIdx.x % (WN * 32);
+      const int c = bi * TILE + (row / 32 * FN + v) * 32 + row % 32;
+      for (int jl = threadIdx.x / (WN * 32); jl < TILE; jl += NT / (WN * 32)) {
+        const int r = bj * TILE + jl;
+        if (r < a.rows && c < a.cols)
+          out[(long)r * a.cols + c] =
+              from_f32<BF16>(place(row, jl >> 2)[jl & 3] * (1.f / kXScale)).v;
       }
     }
   }
-  if (LAST && a.tall) {
-    __syncthreads();
-    uint16_t* out = a.out + (long)batch * a.rows * a.cols;
-    const int il = (threadIdx.x & 63) * 2;
-    for (int jl = threadIdx.x >> 6; jl < kTile; jl += 4) {
-      const int r = bj * kTile + jl, c = bi * kTile + il;
-      if (r >= a.rows) break;
+}
+
+// ---------------------------------------------------------------------------
+// Small matrices (up to 128 x 256): a block holds one and does every step.
+// X stays in fp32 in the registers, in the layout of the update's result;
+// its fp16 copy, A and B lie in LDS.  Bound by the waits between the three
+// products of a step.  One of 64 x 128: 15 us (in seventeen launches 127),
+// 512 of 128 x 256: 240 us (406 for 128 x 264, which takes the launches).
+// ---------------------------------------------------------------------------
+
+template <typename T, int NP, int MP, int WAVES>
+__global__ __launch_bounds__(WAVES* kWave) void ns_small_kernel(
+    const T* __restrict__ g, uint16_t* __restrict__ out, int rows, int cols,
+    int steps, float eps) {
+  constexpr int TI = NP / 32, TJ = MP / 32;
+  constexpr int MINE = (TI * TJ + WAVES - 1) / WAVES;
+  constexpr int SQ = (TI * TI + WAVES - 1) / WAVES;
+  __shared__ __attribute__((aligned(16))) uint16_t lx[NP * MP], la[NP * NP],
+      lb[NP * NP];
+  __shared__ double red[WAVES];
+  const int lane = threadIdx.x & 63;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int half = lane >> 5;
+  const bool tall = rows > cols;
+  const int size = rows * cols;
+  const T* gb = g + (long)blockIdx.x * size;
+  uint16_t* ob = out + (long)blockIdx.x * size;
+
+  // tile u of this wave: rows ti * 32.., columns tj * 32.. of X; register r
+  // of a lane: row lane & 31, column 8 (r >> 2) + 4 half + (r & 3)
+  f32x16 x[MINE];
+  double sum = 0;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int i = il + e;
-        const float x =
-            img[i * kTile + (((jl >> 2) ^ (i & 31)) << 2) + (jl & 3)];
-        if (c + e < a.cols)
-          out[(long)r * a.cols + c + e] =
-              from_f32<BF16>(x * (1.f / kXScale)).v;
-      }
+  for (int u = 0; u < MINE; ++u) {
+    const int q = wid + u * WAVES;
+    const int i = q % TI * 32 + (lane & 31), j0 = q / TI * 32 + half * 4;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int j = j0 + 8 * (r >> 2) + (r & 3);
+      const int gr = tall ? j : i, gc = tall ? i : j;
+      const bool in = q < TI * TJ && gr < rows && gc < cols;
+      x[u][r] = in ? to_f32<T>(gb[gr * cols + gc]) : 0.f;
+      sum += (double)x[u][r] * (double)x[u][r];
     }
   }
+  for (int off = kWave / 2; off; off >>= 1) sum += __shfl_xor(sum, off, kWave);
+  if (lane == 0) red[wid] = sum;
+  __syncthreads();
+  sum = 0;
+  for (int i = 0; i < WAVES; ++i) sum += red[i];
+  const float by = (float)(kXScale / (sqrt(sum) + (double)eps));
+#pragma unroll
+  for (int u = 0; u < MINE; ++u)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[u][r] *= by;
+
+  auto put = [&](uint16_t* tile, auto dp, int row, int col, const float* v) {
+    constexpr int DP = decltype(dp)::value;
+    Pack<uint16_t, 4> y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y.v[e] = from_f32<FP16>(v[e]).v;
+    *reinterpret_cast<Pack<uint16_t, 4>*>(tile + tile_at<DP>(row, col >> 3) +
+                                          (col & 7)) = y;
+  };
+  using XW = std::integral_constant<int, MP>;
+  using AW = std::integral_constant<int, NP>;
+  const Frags<MP> fx(lx, lane);
+  const Frags<NP> fa(la, lane), fb(lb, lane);
+
+  for (int k = 0; k < steps; ++k) {
+#pragma unroll
+    for (int u = 0; u < MINE; ++u) {
+      const int q = wid + u * WAVES;
+      if (q >= TI * TJ) break;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float v[4] = {x[u][c * 4], x[u][c * 4 + 1], x[u][c * 4 + 2],
+                            x[u][c * 4 + 3]};
+        put(lx, XW{}, q % TI * 32 + (lane & 31), q / TI * 32 + c * 8 + half * 4,
+            v);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < SQ; ++u) {              // A = X X^T
+      const int q = wid + u * WAVES;
+      if (q >= TI * TI) break;
+      const int ti = q % TI * 32, tj = q / TI * 32;
+      f32x16 acc = {};
+#pragma unroll
+      for (int st = 0; st < MP / 16; ++st)
+        acc = mfma32<FP16>(fx.row(tj * MP, st), fx.row(ti * MP, st), acc);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v[e] = acc[c * 4 + e] * (1.f / (kXScale * kXScale));
+        put(la, AW{}, ti + (lane & 31), tj + c * 8 + half * 4, v);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < SQ; ++u) {              // B = b A + c A A
+      const int q = wid + u * WAVES;
+      if (q >= TI * TI) break;
+      const int ti = q % TI * 32, tj = q / TI * 32;
+      f32x16 acc = {};
+#pragma unroll
+      for (int st = 0; st < NP / 16; ++st)
+        acc = mfma32<FP16>(fa.row(tj * NP, st), fa.row(ti * NP, st), acc);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int i = ti + (lane & 31), j = tj + c * 8 + half * 4;
+        const Pack<uint16_t, 4> o = *reinterpret_cast<const Pack<uint16_t, 4>*>(
+            la + tile_at<NP>(i, j >> 3) + (j & 7));
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v[e] = kNsC * acc[c * 4 + e] + kNsB * h2f(o.v[e]);
+        put(lb, AW{}, i, quad_swap(j), v);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < MINE; ++u) {            // X = a X + B X
+      const int q = wid + u * WAVES;
+      if (q >= TI * TJ) break;
+      const Frags<MP> ft(lx, lane, q / TI * 32);
+      f32x16 acc = {};
+      unroll<NP / 16>([&](auto st) {
+        s16x8 f;
+        ft.template tr<1, st * 16 * MP>(&f);
+        acc = mfma32<FP16>(f, fb.row(q % TI * 32 * NP, st), acc);
+      });
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[u][r] = kNsA * x[u][r] + acc[r];
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int u = 0; u < MINE; ++u) {
+    const int q = wid + u * WAVES;
+    const int i = q % TI * 32 + (lane & 31), j0 = q / TI * 32 + half * 4;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int j = j0 + 8 * (r >> 2) + (r & 3);
+      const int gr = tall ? j : i, gc = tall ? i : j;
+      if (q < TI * TJ && gr < rows && gc < cols)
+        ob[gr * cols + gc] = from_f32<BF16>(x[u][r] * (1.f / kXScale)).v;
+    }
+  }
+}
+
+template <typename T>
+void launch_small(const at::Tensor& g, at::Tensor& out, int batch, int rows,
+                  int cols, int steps, float eps, hipStream_t s) {
+  const int n = std::min(rows, cols), m = std::max(rows, cols);
+  auto go = [&](auto kernel, int waves) {
+    kernel<<<batch, waves * kWave, 0, s>>>(
+        static_cast<const T*>(g.data_ptr()),
+        static_cast<uint16_t*>(out.data_ptr()), rows, cols, steps, eps);
+  };
+  // waves: so that a lane's share of X is at most 32 registers
+  if (n <= 64 && m <= 64) go(ns_small_kernel<T, 64, 64, 4>, 4);
+  else if (n <= 64 && m <= 128) go(ns_small_kernel<T, 64, 128, 8>, 8);
+  else if (n <= 64) go(ns_small_kernel<T, 64, 256, 8>, 8);
+  else if (m <= 128) go(ns_small_kernel<T, 128, 128, 16>, 16);
+  else go(ns_small_kernel<T, 128, 256, 16>, 16);
 }
 
 template <typename T, int V>
@@ -397,13 +576,40 @@ at::Tensor newton_schulz_impl(const at::Tensor& g_in, int64_t steps,
   if (g.numel() == 0) return out;
   TORCH_CHECK(rows <= (1 << 20) && cols <= (1 << 20) && batch <= 65535,
               "newton_schulz: the matrices are too large or too many");
-  auto pad = [](long x) { return (x + kTile - 1) / kTile * kTile; };
-  const long np = pad(std::min(rows, cols)), mp = pad(std::max(rows, cols));
-  const long nb = np / kTile, pairs = nb * (nb + 1) / 2;
-  TORCH_CHECK(batch * nb * (mp / kTile) <= std::numeric_limits<int>::max() &&
+  // The larger tile where it pads little and leaves about a tile a CU.  us, of
+  // 128 / 256: update of 24 1024x4096 in one part 305 / 246, of 12 768x2304
+  // 60 / 62; X X^T of the first 150 / 128, of the second, 72 tiles, 31 / 64.
+  const long lo = std::min(rows, cols), hi = std::max(rows, cols);
+  auto pad = [](long x, long t) { return (x + t - 1) / t * t; };
+  const long n256 = pad(lo, 256) / 256, m256 = pad(hi, 256) / 256;
+  const bool large = pad(lo, 256) * pad(hi, 256) * 8 <=
+                         pad(lo, kTile) * pad(hi, kTile) * 9 &&
+                     batch * n256 * m256 >= 200;
+  const bool large_square = large && batch * n256 * (n256 + 1) / 2 >= 200;
+  const long unit = large ? 256 : kTile;
+  const long np = pad(lo, unit), mp = pad(hi, unit);
+  TORCH_CHECK(batch * (np / kTile) * (mp / kTile) <=
+                      std::numeric_limits<int>::max() &&
                   mp / 64 <= 65535,
               "newton_schulz: the matrices are too large or too many");
   const long parts = (rows * cols + kNormChunk - 1) / kNormChunk;
+
+  const auto s = at::cuda::getCurrentCUDAStream();
+  if (std::min(rows, cols) <= 128 && std::max(rows, cols) <= 256) {
+    auto small = [&](auto tag) {
+      launch_small<decltype(tag)>(g, out, (int)batch, (int)rows, (int)cols,
+                                  (int)steps, (float)eps, s);
+    };
+    switch (g.scalar_type()) {
+      case at::kFloat: small(float{}); break;
+      case at::kBFloat16: small(BF16{}); break;
+      case at::kHalf: small(FP16{}); break;
+      default:
+        TORCH_CHECK(false, "newton_schulz: unsupported dtype ",
+                    g.scalar_type());
+    }
+    return out;
+  }
 
   const auto half = g.options().dtype(at::kHalf);
   auto x = at::empty({4, batch, np, mp}, half);       // X twice, in two parts
@@ -413,7 +619,6 @@ at::Tensor newton_schulz_impl(const at::Tensor& g_in, int64_t steps,
   auto* pa = static_cast<uint16_t*>(sq.data_ptr());
   const long xs = batch * np * mp;
   uint16_t* pb = pa + batch * np * np;
-  const auto s = at::cuda::getCurrentCUDAStream();
 
   auto start = [&](auto tag) {
     using T = decltype(tag);
@@ -431,23 +636,45 @@ at::Tensor newton_schulz_impl(const at::Tensor& g_in, int64_t steps,
     default:
       TORCH_CHECK(false, "newton_schulz: unsupported dtype ", g.scalar_type());
   }
+  using Small = std::integral_constant<int, 128>;
+  using Large = std::integral_constant<int, 256>;
+  auto square = [&](auto tile, auto poly, const uint16_t* in, uint16_t* to,
+                    long depth) {
+    constexpr int TILE = decltype(tile)::value;
+    constexpr int NT = Shape<TILE>::WM * Shape<TILE>::WN * kWave;
+    const long nb = np / TILE, pairs = nb * (nb + 1) / 2;
+    ns_square_kernel<TILE, decltype(poly)::value>
+        <<<(unsigned)(batch * pairs), NT, 0, s>>>(in, to, (int)np, (int)depth,
+                                                  (int)pairs);
+  };
+  auto update = [&](auto tile, auto last, const NsUpdate& u) {
+    constexpr int TILE = decltype(tile)::value;
+    constexpr int NT = Shape<TILE>::WM * Shape<TILE>::WN * kWave;
+    ns_update_kernel<TILE, decltype(last)::value>
+        <<<(unsigned)(batch * (np / TILE) * (mp / TILE)), NT, 0, s>>>(u);
+  };
   for (int64_t k = 0; k < steps; ++k) {
     uint16_t* cur = px + (k & 1) * 2 * xs;
     uint16_t* nxt = px + ((k + 1) & 1) * 2 * xs;
-    ns_square_kernel<false><<<(unsigned)(batch * pairs), 256, 0, s>>>(
-        cur, pa, (int)np, (int)mp, (int)pairs);
-    ns_square_kernel<true><<<(unsigned)(batch * pairs), 256, 0, s>>>(
-        pa, pb, (int)np, (int)np, (int)pairs);
+    if (large_square) {
+      square(Large{}, std::false_type{}, cur, pa, mp);
+      square(Large{}, std::true_type{}, pa, pb, np);
+    } else {
+      square(Small{}, std::false_type{}, cur, pa, mp);
+      square(Small{}, std::true_type{}, pa, pb, np);
+    }
     // the last two X that are multiplied have one part
-    NsUpdate u{pb, cur, k + 2 < steps ? cur + xs : nullptr, nxt,
-               k + 3 < steps ? nxt + xs : nullptr,
-               static_cast<uint16_t*>(out.data_ptr()), (int)np, (int)mp,
-               (int)rows, (int)cols, rows > cols};
-    const unsigned blocks = (unsigned)(batch * nb * (mp / kTile));
-    if (k + 1 < steps)
-      ns_update_kernel<false><<<blocks, 256, 0, s>>>(u);
+    const NsUpdate u{pb, cur, k + 2 < steps ? cur + xs : nullptr, nxt,
+                     k + 3 < steps ? nxt + xs : nullptr,
+                     static_cast<uint16_t*>(out.data_ptr()), (int)np, (int)mp,
+                     (int)rows, (int)cols, rows > cols};
+    const bool last = k + 1 == steps;
+    if (large)
+      last ? update(Large{}, std::true_type{}, u)
+           : update(Large{}, std::false_type{}, u);
     else
-      ns_update_kernel<true><<<blocks, 256, 0, s>>>(u);
+      last ? update(Small{}, std::true_type{}, u)
+           : update(Small{}, std::false_type{}, u);
   }
   return out;
 }

@@ -61,6 +61,14 @@ def test_sizes(n, m):
     _check(_matrix(3, n, m, "flat"))
 
 
+@pytest.mark.parametrize("b,n,m", [
+    (24, 512, 1100), (24, 1100, 512), (60, 500, 500), (23, 700, 768),
+    (200, 130, 250)])
+def test_many_matrices(b, n, m):
+    """Enough of them for the larger tile, and next to that border."""
+    _check(_matrix(b, n, m, "flat"))
+
+
 @pytest.mark.parametrize("kind", ["flat", "power", "steep", "low"])
 @pytest.mark.parametrize("n,m", [(64, 64), (256, 1024), (768, 512)])
 def test_spectra(kind, n, m):
