@@ -70,12 +70,20 @@ class SyntheticImages:
 
 
 class SyntheticBertBatches:
-    """Yields (input_ids, mlm_labels, nsp_labels) for BERT pretraining."""
+    """Yields (input_ids, mlm_labels, nsp_labels) for BERT pretraining.
+
+    ``doc_len`` > 0 packs documents of about that length into the rows and
+    yields (input_ids, mlm_labels, nsp_labels, cu_seqlens): the documents'
+    borders in the tokens of all rows, and a label for each.  Their number is
+    fixed (a graph can be captured): unused ones are empty, at the end, with
+    the label -100.
+    """
 
     def __init__(self, batch_size: int, seq_len: int = 128,
                  vocab_size: int = 30522, mask_frac: float = 0.15,
                  seed: int = 0, rank: int = 0, device: str = "cpu",
-                 pinned: bool = False, pool: int = 0):
+                 pinned: bool = False, pool: int = 0, doc_len: int = 0):
+        self.doc_len = doc_len
         self.batch_size, self.seq_len = batch_size, seq_len
         self.vocab_size, self.mask_frac = vocab_size, mask_frac
         self.device, self.pinned = device, pinned
@@ -89,14 +97,35 @@ class SyntheticBertBatches:
         labels = ids.clone()
         mask = torch.rand(ids.shape, generator=self.gen) < self.mask_frac
         labels[~mask] = -100
-        nsp = torch.randint(0, 2, (self.batch_size,), generator=self.gen)
+        if self.doc_len > 0:
+            cu = self._pack()
+            nsp = torch.randint(0, 2, (cu.numel() - 1,), generator=self.gen)
+            nsp[cu[1:] == cu[:-1]] = -100
+            batch = (ids, labels, nsp, cu)
+        else:
+            nsp = torch.randint(0, 2, (self.batch_size,), generator=self.gen)
+            batch = (ids, labels, nsp)
         if self.pinned:
-            ids, labels, nsp = ids.pin_memory(), labels.pin_memory(), nsp.pin_memory()
+            batch = tuple(t.pin_memory() for t in batch)
         if self.device != "cpu":
-            ids = ids.to(self.device, non_blocking=True)
-            labels = labels.to(self.device, non_blocking=True)
-            nsp = nsp.to(self.device, non_blocking=True)
-        return ids, labels, nsp
+            batch = tuple(t.to(self.device, non_blocking=True) for t in batch)
+        return batch
+
+    def _pack(self) -> torch.Tensor:
+        """Borders of documents of half to one and a half of doc_len, none
+        across two rows: int32, of a fixed number."""
+        low = max(1, self.doc_len // 2)
+        slots = self.batch_size * (-(-self.seq_len // low))
+        ends = []
+        for row in range(self.batch_size):
+            at, end = row * self.seq_len, (row + 1) * self.seq_len
+            while at < end:
+                n = int(torch.randint(low, self.doc_len + low + 1, (1,),
+                                      generator=self.gen))
+                at = min(at + n, end)
+                ends.append(at)
+        ends += [self.batch_size * self.seq_len] * (slots - len(ends))
+        return torch.tensor([0, *ends], dtype=torch.int32)
 
     def __iter__(self):
         if self.pool > 0:

@@ -9,14 +9,17 @@ param/grad pair with ONE fused HIP kernel launch per bucket
 (sgd_momentum_flat: wd + momentum + nesterov + lr in a single pass,
 fp32 momentum for bf16 params).  Torch fallback keeps CPU tests running.
 ``FlatAdam`` is the BERT-path equivalent (fused adamw_flat kernel).
+``FlatMuon`` orthogonalises the momentum of hidden matrices (all of a shape
+in one batch of Newton-Schulz products) and runs AdamW on everything else.
 """
 
 from __future__ import annotations
 
-from typing import List, Optional
+from typing import Dict, List, Optional, Tuple
 
 import torch
 
+from ..ops import functional as F_amd
 from ..ops import native, native_available
 from .ddp import DataParallel
 
@@ -183,3 +186,152 @@ class FlatAdam(_FlatOptimBase):
         self.betas = tuple(sd.get("betas", self.betas))
         self.eps = sd.get("eps", self.eps)
         self.weight_decay = sd.get("weight_decay", self.weight_decay)
+
+
+class FlatMuon(_FlatOptimBase):
+    """Muon for hidden matrices, AdamW for the other parameters.
+
+    A hidden matrix is the weight of an ``nn.Linear`` with at least 16 rows
+    and columns.  Its step is ``lr * max(1, rows / cols) ** 0.5`` times the
+    orthogonalised momentum (``F_amd.newton_schulz``); matrices of one shape
+    go through it together.  Embeddings, norms, biases and small heads take
+    an AdamW step of ``adam_lr``.  Weight decay is decoupled in both.
+
+    Every rank orthogonalises every matrix from the same averaged gradients,
+    bit for bit, so ranks stay in step without an exchange.
+    """
+
+    MIN_SIDE = 16
+
+    def __init__(self, engine: DataParallel, lr: float = 0.02,
+                 momentum: float = 0.95, nesterov: bool = True,
+                 ns_steps: int = 5, ns_eps: float = 1e-7,
+                 weight_decay: float = 0.01, adam_lr: float = 3e-4,
+                 betas=(0.9, 0.999), eps: float = 1e-8):
+        super().__init__(engine)
+        self.lr, self.momentum, self.nesterov = lr, momentum, nesterov
+        self.ns_steps, self.ns_eps = ns_steps, ns_eps
+        self.weight_decay = weight_decay
+        self.adam_lr, self.betas, self.eps = adam_lr, betas, eps
+        self.t = 0
+        hidden = {id(m.weight) for m in engine.module.modules()
+                  if isinstance(m, torch.nn.Linear)
+                  and min(m.weight.shape) >= self.MIN_SIDE}
+        # a weight that an embedding shares (a tied head) is not hidden
+        hidden -= {id(m.weight) for m in engine.module.modules()
+                   if isinstance(m, torch.nn.Embedding)}
+        # momentum of a matrix, or first moment of anything else
+        self.m = [torch.zeros(fp.numel(), dtype=torch.float32,
+                              device=fp.device) for fp in self.flat_params]
+        # (bucket, start, end) of each matrix, by shape and type ..
+        self.groups: Dict[tuple, List[Tuple[int, int, int]]] = {}
+        # .. and of each stretch of the rest, with its second moments
+        self.rest: List[Tuple[int, int, int]] = []
+        for bi, b in enumerate(self.buckets):
+            off = 0
+            for p in b.params:
+                end = off + p.numel()
+                if id(p) in hidden:
+                    self.groups.setdefault(
+                        (*p.shape, p.dtype, p.device), []).append(
+                            (bi, off, end))
+                elif self.rest and self.rest[-1][0] == bi \
+                        and self.rest[-1][2] == off:
+                    self.rest[-1] = (bi, self.rest[-1][1], end)
+                else:
+                    self.rest.append((bi, off, end))
+                off = end
+        # the fused AdamW takes four elements at a time from where a stretch
+        # begins: up to three in front of such a border are one of their own
+        self.rest = [span for bi, a, e in self.rest
+                     for span in ((bi, a, min(e, -(-a // 4) * 4)),
+                                  (bi, min(e, -(-a // 4) * 4), e))
+                     if span[1] < span[2]]
+        self.v = [torch.zeros(e - a, dtype=torch.float32,
+                              device=self.flat_params[bi].device)
+                  for bi, a, e in self.rest]
+
+    def _matrices(self, spans):
+        cut = lambda flats: [flats[bi][a:e] for bi, a, e in spans]  # noqa: E731
+        masters = [] if self.masters[spans[0][0]] is None \
+            else cut(self.masters)
+        return (cut(self.flat_params), cut([b.flat for b in self.buckets]),
+                cut(self.m), masters)
+
+    def _step_matrices(self, rows: int, cols: int, spans) -> None:
+        params, grads, moms, masters = self._matrices(spans)
+        step = self.lr * max(1.0, rows / cols) ** 0.5
+        keep = 1.0 - self.lr * self.weight_decay
+        u = torch.empty(len(spans), rows, cols, dtype=torch.float32,
+                        device=params[0].device)
+        if u.is_cuda and native_available():
+            native().muon_momentum(grads, moms, u, self.momentum,
+                                   self.nesterov)
+            o = F_amd.newton_schulz(u, self.ns_steps, self.ns_eps)
+            native().muon_apply(params, masters, o, step, keep)
+            return
+        for i, (g, m) in enumerate(zip(grads, moms)):
+            m.mul_(self.momentum).add_(g.float())
+            u[i] = (g.float().add(m, alpha=self.momentum) if self.nesterov
+                    else m).view(rows, cols)
+        o = F_amd.newton_schulz(u, self.ns_steps, self.ns_eps).float()
+        for i, p in enumerate(params):
+            w = masters[i] if masters else p
+            w.copy_(keep * w.float() - step * o[i].reshape(-1))
+            if masters:
+                p.copy_(w.to(p.dtype))
+
+    def _step_rest(self, span, v: torch.Tensor, bc1: float,
+                   bc2: float) -> None:
+        bi, a, e = span
+        b1, b2 = self.betas
+        fp, g = self.flat_params[bi][a:e], self.buckets[bi].flat[a:e]
+        m = self.m[bi][a:e]
+        master = self.masters[bi]
+        master = None if master is None else master[a:e]
+        if fp.is_cuda and native_available():
+            args = (self.adam_lr, b1, b2, self.eps, self.weight_decay, bc1,
+                    bc2)
+            if master is not None:
+                native().adamw_flat_master(fp, g, m, v, master, *args)
+            else:
+                native().adamw_flat(fp, g, m, v, *args)
+            return
+        g32 = g.float()
+        m.mul_(b1).add_(g32, alpha=1 - b1)
+        v.mul_(b2).addcmul_(g32, g32, value=1 - b2)
+        p32 = master if master is not None else fp.float()
+        p32 = p32 - self.adam_lr * self.weight_decay * p32
+        p32 = p32 - self.adam_lr * (m / bc1) / ((v / bc2).sqrt() + self.eps)
+        if master is not None:
+            master.copy_(p32)
+        fp.copy_(p32.to(fp.dtype))
+
+    @torch.no_grad()
+    def step(self) -> None:
+        self.t += 1
+        bc1 = 1 - self.betas[0] ** self.t
+        bc2 = 1 - self.betas[1] ** self.t
+        for (rows, cols, _, _), spans in self.groups.items():
+            self._step_matrices(rows, cols, spans)
+        for span, v in zip(self.rest, self.v):
+            self._step_rest(span, v, bc1, bc2)
+
+    def state_dict(self) -> dict:
+        return {"m": self.m, "v": self.v, "masters": self.masters,
+                "t": self.t, "lr": self.lr, "momentum": self.momentum,
+                "nesterov": self.nesterov, "ns_steps": self.ns_steps,
+                "ns_eps": self.ns_eps, "adam_lr": self.adam_lr,
+                "betas": self.betas, "eps": self.eps,
+                "weight_decay": self.weight_decay}
+
+    def load_state_dict(self, sd: dict) -> None:
+        for mine, theirs in ((self.m, sd["m"]), (self.v, sd["v"]),
+                             (self.masters, sd.get("masters", []))):
+            for dst, src in zip(mine, theirs):
+                if dst is not None and src is not None:
+                    dst.copy_(src.to(dst.device))
+        for k in ("t", "lr", "momentum", "nesterov", "ns_steps", "ns_eps",
+                  "adam_lr", "eps", "weight_decay"):
+            setattr(self, k, sd[k])
+        self.betas = tuple(sd["betas"])

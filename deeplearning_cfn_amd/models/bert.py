@@ -6,6 +6,11 @@ scratch on the same ops seam: Linear routes through the MFMA GEMM kernel,
 LayerNorm/GELU through their HIP kernels when native is selected,
 attention through torch SDPA (flash-style, memory-bound-safe in 288 GB).
 Data-parallel only, per SURVEY.md §3.3 scope ruling.
+
+Documents of a batch may be packed: with ``cu_seqlens`` the tokens are read
+one row behind the other, document i being the tokens from cu_seqlens[i] to
+cu_seqlens[i + 1].  A document sees only itself, its positions begin at 0,
+and its first token is what the NSP head reads.
 """
 
 from __future__ import annotations
@@ -29,6 +34,9 @@ class BertConfig:
     type_vocab: int = 2
     dropout: float = 0.0          # pretraining-benchmark default: off
     layer_norm_eps: float = 1e-12
+    # scores fall off with distance (slope 2 ** (-8 (h + 1) / heads) of head
+    # h, both ways) instead of a table of positions
+    alibi: bool = False
 
 
 class MFMALinear(nn.Linear):
@@ -58,7 +66,15 @@ class SelfAttention(nn.Module):
         self.qkv = MFMALinear(cfg.hidden, 3 * cfg.hidden)
         self.proj = MFMALinear(cfg.hidden, cfg.hidden)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, cu_seqlens: torch.Tensor | None = None,
+                slopes: torch.Tensor | None = None) -> torch.Tensor:
+        if cu_seqlens is not None:              # x: [tokens, hidden]
+            from ..ops import functional as F_amd
+            qkv = self.qkv(x).view(-1, 3, self.heads, self.dh)
+            o = F_amd.document_attention_qkv(
+                qkv, cu_seqlens, scale=1.0 / math.sqrt(self.dh),
+                slopes=slopes)
+            return self.proj(o.reshape(x.shape))
         B, S, H = x.shape
         qkv = self.qkv(x).view(B, S, 3, self.heads, self.dh)
         q, k, v = (qkv[:, :, i].transpose(1, 2) for i in range(3))
@@ -84,9 +100,10 @@ class Block(nn.Module):
         self.fc2 = MFMALinear(cfg.intermediate, cfg.hidden)
         self.ln2 = FusedLayerNorm(cfg.hidden, eps=cfg.layer_norm_eps)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, cu_seqlens: torch.Tensor | None = None,
+                slopes: torch.Tensor | None = None) -> torch.Tensor:
         from ..ops import functional as F_amd
-        x = self.ln1(x + self.attn(x))
+        x = self.ln1(x + self.attn(x, cu_seqlens, slopes))
         h = self.fc1(x)
         h = F_amd.gelu(h) if hasattr(F_amd, "gelu") else F.gelu(h)
         return self.ln2(x + self.fc2(h))
@@ -103,7 +120,14 @@ class BertForPretraining(nn.Module):
         # pad rows are never labeled, CE simply learns them away
         self.vocab_padded = (cfg.vocab_size + 63) // 64 * 64
         self.tok = nn.Embedding(self.vocab_padded, cfg.hidden)
-        self.pos = nn.Embedding(cfg.max_seq, cfg.hidden)
+        if cfg.alibi:
+            slopes = torch.tensor([2.0 ** (-8.0 * (h + 1) / cfg.heads)
+                                   for h in range(cfg.heads)])
+            # as integers: a change of the model's type leaves them alone
+            self.register_buffer("slope_bits", slopes.view(torch.int32),
+                                 persistent=False)
+        else:
+            self.pos = nn.Embedding(cfg.max_seq, cfg.hidden)
         self.typ = nn.Embedding(cfg.type_vocab, cfg.hidden)
         self.ln = FusedLayerNorm(cfg.hidden, eps=cfg.layer_norm_eps)
         self.blocks = nn.ModuleList(Block(cfg) for _ in range(cfg.layers))
@@ -119,8 +143,38 @@ class BertForPretraining(nn.Module):
             if isinstance(m, nn.Linear) and m.bias is not None:
                 nn.init.zeros_(m.bias)
 
+    def encode_documents(self, input_ids: torch.Tensor,
+                         cu_seqlens: torch.Tensor,
+                         token_type: torch.Tensor | None = None
+                         ) -> torch.Tensor:
+        """Packed documents: [*input_ids.shape, hidden]."""
+        from ..ops import functional as F_amd
+        ids = input_ids.reshape(-1)
+        cu = cu_seqlens.to(torch.int32)
+        typ = (token_type.reshape(-1) if token_type is not None
+               else torch.zeros_like(ids))
+        tables, index = [self.tok.weight, self.typ.weight], [ids, typ]
+        slopes = None
+        if self.cfg.alibi:
+            slopes = self.slope_bits.view(torch.float32)
+        else:
+            tables.append(self.pos.weight)
+            index.append(F_amd.document_positions(cu, ids.numel())
+                         .clamp_(max=self.cfg.max_seq - 1))
+        x = self.ln(F_amd.embedding_sum(index, tables))
+        for blk in self.blocks:
+            x = blk(x, cu, slopes)
+        return x.view(*input_ids.shape, -1)
+
     def encode(self, input_ids: torch.Tensor,
-               token_type: torch.Tensor | None = None) -> torch.Tensor:
+               token_type: torch.Tensor | None = None,
+               cu_seqlens: torch.Tensor | None = None) -> torch.Tensor:
+        if self.cfg.alibi and cu_seqlens is None:
+            n, S = input_ids.numel(), input_ids.shape[-1]
+            cu_seqlens = torch.arange(0, n + 1, S, dtype=torch.int32,
+                                      device=input_ids.device)
+        if cu_seqlens is not None:
+            return self.encode_documents(input_ids, cu_seqlens, token_type)
         B, S = input_ids.shape
         pos = torch.arange(S, device=input_ids.device).unsqueeze(0)
         typ = token_type if token_type is not None else torch.zeros_like(input_ids)
@@ -131,27 +185,36 @@ class BertForPretraining(nn.Module):
 
     def forward(self, input_ids: torch.Tensor,
                 mlm_labels: torch.Tensor | None = None,
-                nsp_labels: torch.Tensor | None = None):
-        x = self.encode(input_ids)
+                nsp_labels: torch.Tensor | None = None,
+                cu_seqlens: torch.Tensor | None = None):
+        """``nsp_labels``: one a sequence, or one a document with
+        ``cu_seqlens`` (-100 for an unused, empty one)."""
+        x = self.encode(input_ids, cu_seqlens=cu_seqlens)
         h = self.mlm_ln(F.gelu(self.mlm_dense(x)))
         # MLM logits via weight tying with the token embedding; routed
         # through the MFMA GEMM (padded vocab keeps N % 16 == 0)
         from ..ops import functional as F_amd
-        B, S, H = h.shape
-        logits = F_amd.linear(h.reshape(-1, H), self.tok.weight)
-        logits = logits.reshape(B, S, self.vocab_padded)
+        logits = F_amd.linear(h.reshape(-1, h.shape[-1]), self.tok.weight)
+        logits = logits.reshape(*h.shape[:-1], self.vocab_padded)
         if mlm_labels is None:
             return logits
         loss = F.cross_entropy(
             logits.float().view(-1, self.vocab_padded),
             mlm_labels.view(-1), ignore_index=-100)
         if nsp_labels is not None:
-            cls = self.nsp(x[:, 0])
+            if cu_seqlens is None:
+                first = x[:, 0]
+            else:
+                flat = x.reshape(-1, x.shape[-1])
+                first = flat[cu_seqlens[:-1].long()
+                             .clamp(0, flat.shape[0] - 1)]
+            cls = self.nsp(first)
             loss = loss + F.cross_entropy(cls.float(), nsp_labels)
         return loss
 
 
-def build_bert(size: str = "base", seq_len: int = 128) -> BertForPretraining:
+def build_bert(size: str = "base", seq_len: int = 128,
+               alibi: bool = False) -> BertForPretraining:
     if size == "base":
         cfg = BertConfig()
     elif size == "large":
@@ -159,4 +222,5 @@ def build_bert(size: str = "base", seq_len: int = 128) -> BertForPretraining:
     else:
         raise ValueError(f"unknown bert size {size!r}")
     cfg.max_seq = max(cfg.max_seq, seq_len)
+    cfg.alibi = alibi
     return BertForPretraining(cfg)

@@ -25,7 +25,8 @@ def build_model(network: str, **kw: Any) -> torch.nn.Module:
         )
     if network == "bert":
         return build_bert(size=kw.get("size", "base"),
-                          seq_len=int(kw.get("seq_len", 128)))
+                          seq_len=int(kw.get("seq_len", 128)),
+                          alibi=bool(kw.get("alibi", False)))
     raise ValueError(f"unknown --network {network!r}; families: {MODEL_FAMILIES}")
 
 

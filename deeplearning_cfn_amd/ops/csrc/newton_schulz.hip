@@ -559,7 +559,157 @@ void launch_start(const at::Tensor& g, double* part, int parts, uint16_t* xh,
       p, part, parts, xh, xl, rows, cols, rows > cols, np, mp, eps);
 }
 
+// ---------------------------------------------------------------------------
+// What Muon does around it, for matrices of one shape that lie anywhere:
+//   v <- mu v + g,  u = g + mu v (nesterov) or v         before
+//   p <- (1 - decay) p - step o                          after
+// Both stream each array once.
+// ---------------------------------------------------------------------------
+
+constexpr int kMuonList = 48;         // matrices a launch
+
+template <typename T> struct MuonList {
+  T* p[kMuonList];                    // gradients, or weights
+  float* f[kMuonList];                // momenta, or fp32 masters (or none)
+};
+
+template <typename T, int V>
+__global__ __launch_bounds__(256) void muon_momentum_kernel(
+    MuonList<T> a, float* __restrict__ u, long size, float mu, bool nesterov) {
+  const T* g = a.p[blockIdx.y];
+  float* v = a.f[blockIdx.y];
+  u += (long)blockIdx.y * size;
+  for (long i = ((long)blockIdx.x * 256 + threadIdx.x) * V; i < size;
+       i += (long)gridDim.x * 256 * V) {
+    float x[V], m[V], y[V];
+    load_vec<T, V>(g + i, x);
+    load_vec<float, V>(v + i, m);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      m[e] = mu * m[e] + x[e];
+      y[e] = nesterov ? x[e] + mu * m[e] : m[e];
+    }
+    store_vec<float, V>(v + i, m);
+    store_vec<float, V>(u + i, y);
+  }
+}
+
+template <typename T, int V>
+__global__ __launch_bounds__(256) void muon_apply_kernel(
+    MuonList<T> a, const BF16* __restrict__ o, long size, float step,
+    float keep) {
+  T* p = a.p[blockIdx.y];
+  float* master = a.f[blockIdx.y];
+  o += (long)blockIdx.y * size;
+  for (long i = ((long)blockIdx.x * 256 + threadIdx.x) * V; i < size;
+       i += (long)gridDim.x * 256 * V) {
+    float w[V], x[V];
+    if (master) load_vec<float, V>(master + i, w);
+    else load_vec<T, V>(p + i, w);
+    load_vec<BF16, V>(o + i, x);
+#pragma unroll
+    for (int e = 0; e < V; ++e) w[e] = keep * w[e] - step * x[e];
+    if (master) store_vec<float, V>(master + i, w);
+    store_vec<T, V>(p + i, w);
+  }
+}
+
+// One launch for each 48 of the matrices; f: as many as p, or none.
+template <typename T, typename Launch>
+void muon_lists(at::TensorList p, at::TensorList f, long size, Launch launch) {
+  for (size_t i0 = 0; i0 < p.size(); i0 += kMuonList) {
+    MuonList<T> a{};
+    const size_t k = std::min<size_t>(p.size() - i0, kMuonList);
+    // elements at a time: what every matrix's place in its bucket allows
+    int vec = size % 4 == 0 ? 4 : size % 2 == 0 ? 2 : 1;
+    for (size_t i = 0; i < k; ++i) {
+      a.p[i] = static_cast<T*>(p[i0 + i].data_ptr());
+      a.f[i] = f.empty() ? nullptr : f[i0 + i].data_ptr<float>();
+      while (reinterpret_cast<uintptr_t>(a.p[i]) % (vec * sizeof(T)) ||
+             reinterpret_cast<uintptr_t>(a.f[i]) % (vec * sizeof(float)))
+        vec /= 2;
+    }
+    const long per = 256 * vec;
+    const dim3 grid((unsigned)std::min<long>((size + per - 1) / per, 512),
+                    (unsigned)k);
+    if (vec == 4) launch(a, grid, std::integral_constant<int, 4>{}, (long)i0);
+    else if (vec == 2)
+      launch(a, grid, std::integral_constant<int, 2>{}, (long)i0);
+    else launch(a, grid, std::integral_constant<int, 1>{}, (long)i0);
+  }
+}
+
+void muon_check(at::TensorList p, at::TensorList f, const at::Tensor& batch) {
+  TORCH_CHECK(batch.dim() == 3 && batch.is_contiguous() &&
+                  (size_t)batch.size(0) == p.size() &&
+                  (f.empty() || f.size() == p.size()),
+              "muon: as many matrices as [batch, rows, cols] holds");
+  const long size = batch.size(1) * batch.size(2);
+  for (const auto& t : p)
+    TORCH_CHECK(t.numel() == size && t.is_contiguous() &&
+                    t.scalar_type() == p[0].scalar_type() &&
+                    t.device() == batch.device(),
+                "muon: the matrices differ in size, type or device");
+  for (const auto& t : f)
+    TORCH_CHECK(t.numel() == size && t.is_contiguous() &&
+                    t.scalar_type() == at::kFloat &&
+                    t.device() == batch.device(),
+                "muon: momenta and masters are float32, of the matrices' size");
+}
+
 }  // namespace
+
+// v <- mu v + g; u [n, rows, cols] fp32: what is orthogonalised
+void muon_momentum_impl(at::TensorList g, at::TensorList v, at::Tensor u,
+                        double mu, bool nesterov) {
+  if (g.empty()) return;
+  TORCH_CHECK(u.scalar_type() == at::kFloat && !v.empty(),
+              "muon: u is float32, and each matrix has a momentum");
+  muon_check(g, v, u);
+  const c10::DeviceGuard guard(u.device());
+  const long size = u.size(1) * u.size(2);
+  if (size == 0) return;
+  const auto s = at::cuda::getCurrentCUDAStream();
+  auto go = [&](auto tag) {
+    using T = decltype(tag);
+    muon_lists<T>(g, v, size, [&](auto& a, dim3 grid, auto vec, long i0) {
+      muon_momentum_kernel<T, decltype(vec)::value><<<grid, 256, 0, s>>>(
+          a, u.data_ptr<float>() + i0 * size, size, (float)mu, nesterov);
+    });
+  };
+  switch (g[0].scalar_type()) {
+    case at::kFloat: go(float{}); break;
+    case at::kBFloat16: go(BF16{}); break;
+    default:
+      TORCH_CHECK(false, "muon: unsupported dtype ", g[0].scalar_type());
+  }
+}
+
+// p (and its fp32 master, where there is one) <- keep p - step o
+void muon_apply_impl(at::TensorList p, at::TensorList master,
+                     const at::Tensor& o, double step, double keep) {
+  if (p.empty()) return;
+  TORCH_CHECK(o.scalar_type() == at::kBFloat16, "muon: o is bfloat16");
+  muon_check(p, master, o);
+  const c10::DeviceGuard guard(o.device());
+  const long size = o.size(1) * o.size(2);
+  if (size == 0) return;
+  const auto s = at::cuda::getCurrentCUDAStream();
+  auto go = [&](auto tag) {
+    using T = decltype(tag);
+    muon_lists<T>(p, master, size, [&](auto& a, dim3 grid, auto vec, long i0) {
+      muon_apply_kernel<T, decltype(vec)::value><<<grid, 256, 0, s>>>(
+          a, static_cast<const BF16*>(o.data_ptr()) + i0 * size, size,
+          (float)step, (float)keep);
+    });
+  };
+  switch (p[0].scalar_type()) {
+    case at::kFloat: go(float{}); break;
+    case at::kBFloat16: go(BF16{}); break;
+    default:
+      TORCH_CHECK(false, "muon: unsupported dtype ", p[0].scalar_type());
+  }
+}
 
 // g: [batch, rows, cols] -> bf16 of the same shape
 at::Tensor newton_schulz_impl(const at::Tensor& g_in, int64_t steps,

@@ -168,6 +168,10 @@ at::Tensor doc_attention_qkv(const at::Tensor& qkv, const at::Tensor& cu,
 
 // newton_schulz.hip
 at::Tensor newton_schulz_impl(const at::Tensor& g, int64_t steps, double eps);
+void muon_momentum_impl(at::TensorList g, at::TensorList v, at::Tensor u,
+                        double mu, bool nesterov);
+void muon_apply_impl(at::TensorList p, at::TensorList master,
+                     const at::Tensor& o, double step, double keep);
 
 namespace {
 
@@ -348,6 +352,8 @@ TORCH_LIBRARY(dlx_hip, m) {
   m.def("doc_attention(Tensor q, Tensor k, Tensor v, Tensor cu, Tensor? slopes, float scale) -> Tensor");
   m.def("doc_attention_qkv(Tensor qkv, Tensor cu, Tensor? slopes, float scale) -> Tensor");
   m.def("newton_schulz(Tensor g, int steps, float eps) -> Tensor");
+  m.def("muon_momentum(Tensor[] g, Tensor(a!)[] v, Tensor(b!) u, float mu, bool nesterov) -> ()");
+  m.def("muon_apply(Tensor(a!)[] p, Tensor(b!)[] master, Tensor o, float step, float keep) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(dlx_hip, CUDA, m) {
@@ -396,6 +402,8 @@ TORCH_LIBRARY_IMPL(dlx_hip, CUDA, m) {
   m.impl("doc_attn_fwd", dlx::doc_attn_fwd_impl);
   m.impl("doc_attn_bwd", dlx::doc_attn_bwd_impl);
   m.impl("newton_schulz", dlx::newton_schulz_impl);
+  m.impl("muon_momentum", dlx::muon_momentum_impl);
+  m.impl("muon_apply", dlx::muon_apply_impl);
 }
 
 TORCH_LIBRARY_IMPL(dlx_hip, AutogradCUDA, m) {

@@ -763,6 +763,17 @@ def document_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     return _doc_attention_composed(q, k, v, cu, scale, slopes)
 
 
+def document_positions(cu_seqlens: torch.Tensor, tokens: int) -> torch.Tensor:
+    """Each token's place in its document (0 for tokens in none): int64."""
+    at = torch.arange(tokens, device=cu_seqlens.device)
+    cu = cu_seqlens.long()
+    # the last border that is not behind the token
+    doc = torch.searchsorted(cu, at, right=True) - 1
+    start = cu[doc.clamp(0, cu.numel() - 1)]
+    inside = (doc >= 0) & (doc < cu.numel() - 1)
+    return torch.where(inside, at - start, 0)
+
+
 def document_attention_qkv(qkv: torch.Tensor, cu_seqlens: torch.Tensor,
                            scale: Optional[float] = None,
                            slopes: Optional[torch.Tensor] = None

@@ -27,7 +27,7 @@ from .data import HostPinnedPrefetcher, SyntheticBertBatches, SyntheticImages
 from .engine import DataParallel, init_from_env
 from .engine.dist import shutdown
 from .engine.kvstore import resolve as resolve_kvstore
-from .engine.optim import FlatAdam, FlatSGD
+from .engine.optim import FlatAdam, FlatMuon, FlatSGD
 from .metrics import MetricsLogger, StepTimer
 from .models import build_model
 from .models.registry import model_manifest
@@ -63,6 +63,18 @@ def build_argparser() -> argparse.ArgumentParser:
                    help="gradient bucket size; default auto (xGMI-sized)")
     p.add_argument("--steps-per-epoch", type=int, default=100)
     p.add_argument("--seq-len", type=int, default=128, help="bert only")
+    p.add_argument("--optimizer", default="auto",
+                   help="auto (adam for bert, sgd otherwise) | sgd | adam | "
+                        "muon (hidden matrices by Muon at --lr, the rest by "
+                        "AdamW at --adam-lr)")
+    p.add_argument("--adam-lr", type=float, default=3e-4,
+                   help="muon only: step of what is no hidden matrix")
+    p.add_argument("--doc-len", type=int, default=0,
+                   help="bert only: pack documents of about this length into "
+                        "the rows, each seeing only itself (0 = one a row)")
+    p.add_argument("--alibi", action="store_true",
+                   help="bert only: scores that fall off with distance "
+                        "instead of a table of positions")
     p.add_argument("--seed", type=int, default=42)
     p.add_argument("--no-prefetch", action="store_true")
     p.add_argument("--data-pool", type=int, default=0,
@@ -112,8 +124,8 @@ def _evaluate(engine, eval_batches, args, ctx) -> float:
     for _ in range(args.eval_steps):
         batch = next(eval_batches)
         if args.network == "bert":
-            ids, mlm, _ = (t.to(ctx.device) for t in batch)
-            logits = model(ids)                     # [B,S,V], no labels
+            ids, mlm, _, *cu = (t.to(ctx.device) for t in batch)
+            logits = model(ids, cu_seqlens=cu[0] if cu else None)  # [B,S,V]
             mask = mlm != -100
             pred = logits.argmax(dim=-1)
             correct += (pred[mask] == mlm[mask]).sum().item()
@@ -152,6 +164,8 @@ def train(args: argparse.Namespace) -> dict:
     is_bert = args.network == "bert"
     model_kw = (dict(size="base", seq_len=args.seq_len) if is_bert else
                 dict(num_layers=args.num_layers, dataset=args.dataset))
+    if is_bert and args.alibi:
+        model_kw["alibi"] = True
     model = build_model(args.network, **model_kw)
     model = model.to(ctx.device)
     if not is_bert:
@@ -161,11 +175,19 @@ def train(args: argparse.Namespace) -> dict:
 
     bucket_bytes = int(args.bucket_mb * (1 << 20)) if args.bucket_mb else None
     engine = DataParallel(model, bucket_bytes=bucket_bytes, mode=mode)
-    if is_bert:
+    kind = args.optimizer
+    if kind == "auto":
+        kind = "adam" if is_bert else "sgd"
+    if kind == "adam":
         opt = FlatAdam(engine, lr=args.lr, weight_decay=args.wd)
-    else:
+    elif kind == "sgd":
         opt = FlatSGD(engine, lr=args.lr, momentum=args.mom,
                       weight_decay=args.wd)
+    elif kind == "muon":
+        opt = FlatMuon(engine, lr=args.lr, momentum=args.mom,
+                       weight_decay=args.wd, adam_lr=args.adam_lr)
+    else:
+        raise ValueError(f"unknown --optimizer {kind!r}")
 
     efs = os.environ.get(EFS_MOUNT, "/tmp/dlx_efs")
     prefix = args.model_prefix or str(
@@ -194,7 +216,8 @@ def train(args: argparse.Namespace) -> dict:
         source = SyntheticBertBatches(args.batch_size, seq_len=args.seq_len,
                                       seed=args.seed, rank=ctx.rank,
                                       pinned=ctx.device.type == "cuda",
-                                      pool=args.data_pool)
+                                      pool=args.data_pool,
+                                      doc_len=args.doc_len)
     else:
         image_size = 32 if args.dataset.startswith("cifar") else 224
         ncls = 10 if args.dataset.startswith("cifar") else 1000
@@ -222,7 +245,8 @@ def train(args: argparse.Namespace) -> dict:
         elif is_bert:
             eval_batches = iter(SyntheticBertBatches(
                 args.batch_size, seq_len=args.seq_len,
-                seed=args.seed + 7919, rank=ctx.rank))
+                seed=args.seed + 7919, rank=ctx.rank,
+                doc_len=args.doc_len))
         else:
             eval_batches = iter(SyntheticImages(
                 args.batch_size, image_size=image_size, num_classes=ncls,
@@ -269,8 +293,7 @@ def train(args: argparse.Namespace) -> dict:
             batch = next(batches)
             engine.zero_grad()
             if is_bert:
-                ids, mlm, nsp = (t.to(ctx.device) for t in batch)
-                loss = engine(ids, mlm, nsp)
+                loss = engine(*(t.to(ctx.device) for t in batch))
             else:
                 x, y = batch
                 x, y = x.to(ctx.device), y.to(ctx.device)
