@@ -69,7 +69,13 @@ class HostPinnedPrefetcher:
             cur, ev = next_batch
             staged = self._q.get()
             next_batch = self._stage(staged) if staged is not None else None
-            torch.cuda.current_stream().wait_event(ev)
+            stream = torch.cuda.current_stream()
+            stream.wait_event(ev)
+            for t in cur:
+                # the memory belongs to the copy stream: without this it may
+                # take the next batch while this one's step still reads it
+                if isinstance(t, torch.Tensor):
+                    t.record_stream(stream)
             yield cur
 
     def _stage(self, host_batch):
