@@ -1,7 +1,7 @@
 // Orthogonalisation of matrices by Newton-Schulz products (the Muon update).
 //
 //   X_0 = G / (|G|_F + eps)             G wide: n <= m (a tall one transposed)
-//   A = X X^T,  B = b A + c A A,  X <- a X + B X         `steps` times
+//   A = X X^T,  B = a I + b A + c A A,  X <- B X         `steps` times
 //
 // Every matrix of a batch runs in the same launches, three a step.  X X^T and
 // A A are symmetric: tiles on and above the diagonal are computed and stored
@@ -10,12 +10,15 @@
 // Precision.  The products take fp16 operands (11 bits; bf16's 8 would leave
 // an error of 1e-2) and add in fp32.  Small singular values grow about 3.4
 // times a step, and what X loses to rounding grows with them, so X is kept as
-// a sum of two fp16 numbers (22 bits): the term a X takes both, the products
-// the first alone.  B X's rounding lies in the directions where B is large,
-// which are those that no longer grow.  Against 64 bits that leaves 4e-4 to
-// 2.2e-3 relative (CPU model of these roundings, five spectra, sizes 64 to
-// 768), next to bf16's own 1.7e-3 in the result.  X is stored times 2^12:
-// its entries stay under 2 and its small ones clear of fp16's subnormals.
+// an fp16 number and an fp8 one (e4m3) for what that leaves, 15 bits: the
+// products take the first, the term a X both, the first by way of a's place
+// on B's diagonal.  The last two X that are multiplied are fp16 alone,
+// for what they lose has no time to grow.  B X's rounding lies in the
+// directions where B is large, which are those that no longer grow.  Against
+// 64 bits that leaves 7e-4 to 2.9e-3 relative (CPU model of these roundings,
+// four spectra, sizes 64 to 1024), next to bf16's own 1.7e-3 in the result.
+// X is stored times 2^12: its entries stay under 2 and its small ones clear
+// of fp16's subnormals.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 
@@ -40,6 +43,27 @@ DLX_DEV constexpr int quad_swap(int k) {
 }
 
 DLX_DEV float h2f(uint16_t h) { return to_f32<FP16>(FP16{h}); }
+
+// What fp16 leaves of four numbers, as fp8 times 2^6, and back.  X times 2^12
+// is under 2^13, so that a low part is at most 2^2 and stays inside e4m3.
+constexpr float kLowScale = 64.f;
+
+DLX_DEV uint32_t low_parts(const float* x, const uint16_t* h) {
+  float d[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) d[e] = (x[e] - h2f(h[e])) * kLowScale;
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(d[0], d[1], 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(d[2], d[3], w, true);
+}
+
+DLX_DEV void add_low(float* x, uint32_t low, float by) {
+  const f32v2_t a = __builtin_amdgcn_cvt_pk_f32_fp8((int)low, false);
+  const f32v2_t b = __builtin_amdgcn_cvt_pk_f32_fp8((int)low, true);
+  x[0] += by * a[0];
+  x[1] += by * a[1];
+  x[2] += by * b[0];
+  x[3] += by * b[1];
+}
 
 // Rows row0.. of [., ld] into an LDS tile of DP columns from col0 on.
 template <int ROWS, int DP, int NT>
@@ -94,7 +118,7 @@ DLX_DEV double ns_sum(const double* part, int parts, double* red) {
 template <typename T, int V>
 __global__ __launch_bounds__(256) void ns_split_kernel(
     const T* __restrict__ g, const double* __restrict__ part, int parts,
-    uint16_t* __restrict__ xh, uint16_t* __restrict__ xl, int rows, int cols,
+    uint16_t* __restrict__ xh, uint8_t* __restrict__ xl, int rows, int cols,
     bool tall, int np, int mp, float eps) {
   __shared__ float t[64][65];
   __shared__ double red[4];
@@ -119,15 +143,15 @@ __global__ __launch_bounds__(256) void ns_split_kernel(
 #pragma unroll
   for (int r = threadIdx.x >> 4; r < 64; r += 16) {
     const long o = ((long)b * np + i0 + r) * mp + j0 + xj;
-    Pack<uint16_t, 4> h, l;
+    Pack<uint16_t, 4> h;
+    float v[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float v = tall ? t[xj + e][r] : t[r][xj + e];
-      h.v[e] = from_f32<FP16>(v).v;
-      l.v[e] = from_f32<FP16>(v - h2f(h.v[e])).v;
+      v[e] = tall ? t[xj + e][r] : t[r][xj + e];
+      h.v[e] = from_f32<FP16>(v[e]).v;
     }
     *reinterpret_cast<Pack<uint16_t, 4>*>(xh + o) = h;
-    *reinterpret_cast<Pack<uint16_t, 4>*>(xl + o) = l;
+    if (xl) *reinterpret_cast<uint32_t*>(xl + o) = low_parts(v, h.v);
   }
 }
 
@@ -139,7 +163,7 @@ template <> struct Shape<128> { static constexpr int WM = 2, WN = 2; };
 template <> struct Shape<256> { static constexpr int WM = 2, WN = 4; };
 
 // out = by (in in^T)              POLY false: A from X
-// out = b in + c (in in^T)        POLY true: B from A, columns quad-swapped
+// out = a I + b in + c (in in^T)  POLY true: B from A, columns quad-swapped
 template <int TILE, bool POLY>
 __global__ __launch_bounds__(Shape<TILE>::WM* Shape<TILE>::WN* kWave) void
 ns_square_kernel(const uint16_t* __restrict__ in, uint16_t* __restrict__ out,
@@ -209,7 +233,8 @@ ns_square_kernel(const uint16_t* __restrict__ in, uint16_t* __restrict__ out,
               *reinterpret_cast<const Pack<uint16_t, 4>*>(src + (long)i * np +
                                                           j);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] += kNsB * h2f(o.v[e]);
+          for (int e = 0; e < 4; ++e)
+            x[e] += kNsB * h2f(o.v[e]) + (i == j + e ? kNsA : 0.f);
         }
         Pack<uint16_t, 4> y;
 #pragma unroll
@@ -226,14 +251,16 @@ ns_square_kernel(const uint16_t* __restrict__ in, uint16_t* __restrict__ out,
 }
 
 struct NsUpdate {
-  const uint16_t *b, *xh, *xl;        // b: columns quad-swapped; xl or none
-  uint16_t *yh, *yl;                  // the next X (yl or none), or
+  const uint16_t *b, *xh;             // b: columns quad-swapped
+  const uint8_t* xl;                  // or none
+  uint16_t* yh;                       // the next X, or
+  uint8_t* yl;                        // (or none)
   uint16_t* out;                      // the result, bf16
   int np, mp, rows, cols;
   bool tall;
 };
 
-// a X + B X
+// B X, and a times the low part of X
 template <int TILE, bool LAST>
 __global__ __launch_bounds__(Shape<TILE>::WM* Shape<TILE>::WN* kWave) void
 ns_update_kernel(NsUpdate a) {
@@ -299,8 +326,20 @@ ns_update_kernel(NsUpdate a) {
   auto place = [&](int row, int chunk) {
     return img + row * TILE + ((chunk ^ (row & 31)) << 2);
   };
+  constexpr int ROWS = NT / PR, TURNS = WN * 32 / ROWS;
+  auto row_of = [&](int n) { return threadIdx.x / PR + n * ROWS; };
+  auto place_of = [&](int v, int row) {
+    return xo + (long)(bi * TILE + (row / 32 * FN + v) * 32 + row % 32) * a.mp +
+           j;
+  };
 #pragma unroll
   for (int v = 0; v < FN; ++v) {
+    uint2 low[TURNS] = {};                     // on their way meanwhile
+    if (a.xl) {
+#pragma unroll
+      for (int n = 0; n < TURNS; ++n)
+        low[n] = *reinterpret_cast<const uint2*>(a.xl + place_of(v, row_of(n)));
+    }
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < FM; ++u)
@@ -312,13 +351,11 @@ ns_update_kernel(NsUpdate a) {
             F32x4{{acc[u][v][q * 4], acc[u][v][q * 4 + 1],
                    acc[u][v][q * 4 + 2], acc[u][v][q * 4 + 3]}};
     __syncthreads();
-#pragma unroll 2
-    for (int row = threadIdx.x / PR; row < WN * 32; row += NT / PR) {
+#pragma unroll
+    for (int n = 0; n < TURNS; ++n) {
+      const int row = row_of(n);
       const int i = bi * TILE + (row / 32 * FN + v) * 32 + row % 32;
-      const long o = xo + (long)i * a.mp + j;
-      const P8 h = *reinterpret_cast<const P8*>(a.xh + o);
-      P8 l = {};
-      if (a.xl) l = *reinterpret_cast<const P8*>(a.xl + o);
+      const long o = place_of(v, row);
       float x[8];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -327,21 +364,19 @@ ns_update_kernel(NsUpdate a) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) x[e * 4 + k] = y.v[k];
       }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float w = h2f(h.v[e]);
-        if (a.xl) w += h2f(l.v[e]);
-        x[e] += kNsA * w;
+      if (a.xl) {
+        add_low(x, low[n].x, kNsA / kLowScale);
+        add_low(x + 4, low[n].y, kNsA / kLowScale);
       }
       if (!LAST) {
-        P8 yh, yl;
+        P8 yh;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          yh.v[e] = from_f32<FP16>(x[e]).v;
-          yl.v[e] = from_f32<FP16>(x[e] - h2f(yh.v[e])).v;
-        }
+        for (int e = 0; e < 8; ++e) yh.v[e] = from_f32<FP16>(x[e]).v;
         *reinterpret_cast<P8*>(a.yh + o) = yh;
-        if (a.yl) *reinterpret_cast<P8*>(a.yl + o) = yl;
+        if (a.yl) {
+          *reinterpret_cast<uint2*>(a.yl + o) =
+              make_uint2(low_parts(x, yh.v), low_parts(x + 4, yh.v + 4));
+        }
       } else if (!a.tall) {
         P8 y;
 #pragma unroll
@@ -550,7 +585,7 @@ void launch_small(const at::Tensor& g, at::Tensor& out, int batch, int rows,
 
 template <typename T, int V>
 void launch_start(const at::Tensor& g, double* part, int parts, uint16_t* xh,
-                  uint16_t* xl, int batch, int rows, int cols, int np, int mp,
+                  uint8_t* xl, int batch, int rows, int cols, int np, int mp,
                   float eps, hipStream_t s) {
   const T* p = static_cast<const T*>(g.data_ptr());
   ns_norm_kernel<T, V><<<dim3(parts, batch), 256, 0, s>>>(p, part,
@@ -762,11 +797,13 @@ at::Tensor newton_schulz_impl(const at::Tensor& g_in, int64_t steps,
   }
 
   const auto half = g.options().dtype(at::kHalf);
-  auto x = at::empty({4, batch, np, mp}, half);       // X twice, in two parts
+  auto x = at::empty({2, batch, np, mp}, half);       // X twice
+  auto low = at::empty({2, batch, np, mp}, g.options().dtype(at::kByte));
   auto sq = at::empty({2, batch, np, np}, half);      // A, B
   auto part = at::empty({batch, parts}, g.options().dtype(at::kDouble));
   auto* px = static_cast<uint16_t*>(x.data_ptr());
   auto* pa = static_cast<uint16_t*>(sq.data_ptr());
+  auto* pl = static_cast<uint8_t*>(low.data_ptr());
   const long xs = batch * np * mp;
   uint16_t* pb = pa + batch * np * np;
 
@@ -776,8 +813,8 @@ at::Tensor newton_schulz_impl(const at::Tensor& g_in, int64_t steps,
     const bool v4 = cols % 4 == 0 &&
                     reinterpret_cast<uintptr_t>(g.data_ptr()) % 16 == 0;
     (v4 ? launch_start<T, 4> : launch_start<T, 1>)(
-        g, part.data_ptr<double>(), (int)parts, px, px + xs, (int)batch,
-        (int)rows, (int)cols, (int)np, (int)mp, (float)eps, s);
+        g, part.data_ptr<double>(), (int)parts, px,
+        steps > 2 ? pl : nullptr, (int)batch, (int)rows, (int)cols, (int)np, (int)mp, (float)eps, s);
   };
   switch (g.scalar_type()) {
     case at::kFloat: start(float{}); break;
@@ -804,8 +841,8 @@ at::Tensor newton_schulz_impl(const at::Tensor& g_in, int64_t steps,
         <<<(unsigned)(batch * (np / TILE) * (mp / TILE)), NT, 0, s>>>(u);
   };
   for (int64_t k = 0; k < steps; ++k) {
-    uint16_t* cur = px + (k & 1) * 2 * xs;
-    uint16_t* nxt = px + ((k + 1) & 1) * 2 * xs;
+    uint16_t* cur = px + (k & 1) * xs;
+    uint16_t* nxt = px + ((k + 1) & 1) * xs;
     if (large_square) {
       square(Large{}, std::false_type{}, cur, pa, mp);
       square(Large{}, std::true_type{}, pa, pb, np);
@@ -813,9 +850,9 @@ at::Tensor newton_schulz_impl(const at::Tensor& g_in, int64_t steps,
       square(Small{}, std::false_type{}, cur, pa, mp);
       square(Small{}, std::true_type{}, pa, pb, np);
     }
-    // the last two X that are multiplied have one part
-    const NsUpdate u{pb, cur, k + 2 < steps ? cur + xs : nullptr, nxt,
-                     k + 3 < steps ? nxt + xs : nullptr,
+    // the last two X that are multiplied have no low part
+    const NsUpdate u{pb, cur, k + 2 < steps ? pl + (k & 1) * xs : nullptr, nxt,
+                     k + 3 < steps ? pl + ((k + 1) & 1) * xs : nullptr,
                      static_cast<uint16_t*>(out.data_ptr()), (int)np, (int)mp,
                      (int)rows, (int)cols, rows > cols};
     const bool last = k + 1 == steps;

@@ -805,7 +805,7 @@ def newton_schulz(g: torch.Tensor, steps: int = 5,
     ``X = g / (|g| + eps)``; the result, in bf16, has singular values near 1.
 
     ``g`` is fp32, bf16 or fp16.  Matrices of a batch share their launches.
-    The products take fp16 operands with fp32 sums; X itself is carried in 22
+    The products take fp16 operands with fp32 sums; X itself is carried in 15
     bits.  A zero matrix stays zero.  Gives no gradient.
     """
     if g.dim() < 2 or not g.is_floating_point():
