@@ -36,6 +36,14 @@ namespace {
 
 constexpr int kKeys = 64;             // rows of an LDS tile
 constexpr float kLog2e = 1.4426950408889634f;
+// Tokens to a document from which blocks have eight waves instead of four,
+// which halves what each query (or key) reads but leaves short documents
+// waves without rows.  us, four / eight, 16384 tokens in documents of 512,
+// 1024, 4096: forward of 12 heads of 64 52 / 50, 88 / 78, 259 / 240; of 8
+// heads of 128 52 / 70, 85 / 84, 290 / 269; gradients of those 166 / 224,
+// 273 / 269, 919 / 857, of the narrow ones 141 / 176, 231 / 255, 744 / 745,
+// which stay with four.
+constexpr int kWide = 1024;
 constexpr float kLazy = 8.f;          // P stays under 2^8
 
 __device__ const uint4 g_zero16 = {0, 0, 0, 0};
@@ -78,26 +86,29 @@ struct Tile {
 template <int ROWS> DLX_DEV Tile find_tile(const AttnArgs& a, int t) {
   const int lane = threadIdx.x & (kWave - 1);
   int lo = 0, n = a.docs + 2;         // the document is one of lo..lo+n-1
-  while (n > 1) {
+  Tile x;
+  while (true) {
     const int step = (n + kWave - 1) / kWave;
     const int e = lo + lane * step;
-    const bool at = lane * step < n && border(a, e) / ROWS + e <= t;
-    int c = __popcll(__ballot(at));
+    // one border more than there are documents, where a lane is left for it
+    const int at = border(a, e < a.docs + 2 ? e : a.docs + 2);
+    const uint64_t in = __ballot(lane * step < n && at / ROWS + e <= t);
+    int c = __popcll(in);
     c = c < 1 ? 1 : c;
+    lo = __builtin_amdgcn_readfirstlane(lo + (c - 1) * step);
+    if (step == 1) {
+      x.start = __builtin_amdgcn_readlane(at, c - 1);
+      x.len = (c < kWave ? __builtin_amdgcn_readlane(at, c)
+                         : __builtin_amdgcn_readfirstlane(border(a, lo + 1))) -
+              x.start;
+      break;
+    }
     const int left = n - (c - 1) * step;
-    lo += (c - 1) * step;
     n = left < step ? left : step;
   }
-  lo = __builtin_amdgcn_readfirstlane(lo);
-  Tile x;
-  x.start = border(a, lo);
-  x.len = border(a, lo + 1) - x.start;
   x.row0 = (t - (x.start / ROWS + lo)) * ROWS;
   x.doc = lo > 0 && lo <= a.docs;
   if (x.row0 < 0) x.row0 = x.len < 0 ? 0 : x.len;
-  x.start = __builtin_amdgcn_readfirstlane(x.start);
-  x.len = __builtin_amdgcn_readfirstlane(x.len);
-  x.row0 = __builtin_amdgcn_readfirstlane(x.row0);
   return x;
 }
 
@@ -194,6 +205,7 @@ __global__ __launch_bounds__(NW * 64, DP == 64 ? 4 : 2) void doc_attn_fwd_kernel
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int half = lane >> 5;
   const int wave_row = tl.row0 + wid * 32;
+  const bool mine = wave_row < tl.len;   // else this wave only moves tiles
   const int qpos = wave_row + (lane & 31);
   const bool real = qpos < tl.len;
   if (!tl.doc) {
@@ -229,6 +241,7 @@ __global__ __launch_bounds__(NW * 64, DP == 64 ? 4 : 2) void doc_attn_fwd_kernel
       load_tile<DP, NT>(nx, kb, a.k.token, (t + 1) * kKeys, tl.len, a.dim);
       load_tile<DP, NT>(nx + TS, vb, a.v.token, (t + 1) * kKeys, tl.len, a.dim);
     }
+    if (!mine) return;
     f32x16 s[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
@@ -316,6 +329,7 @@ __global__ __launch_bounds__(NW * 64, DP == 64 ? 3 : 2) void doc_attn_dq_kernel(
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int half = lane >> 5;
   const int wave_row = tl.row0 + wid * 32;
+  const bool mine = wave_row < tl.len;   // else this wave only moves tiles
   const int qpos = wave_row + (lane & 31);
   const bool real = qpos < tl.len;
   if (!tl.doc) {
@@ -365,6 +379,7 @@ __global__ __launch_bounds__(NW * 64, DP == 64 ? 3 : 2) void doc_attn_dq_kernel(
       load_tile<DP, NT>(nx, kb, a.k.token, (t + 1) * kKeys, tl.len, a.dim);
       load_tile<DP, NT>(nx + TS, vb, a.v.token, (t + 1) * kKeys, tl.len, a.dim);
     }
+    if (!mine) return;
     unroll<2>([&](auto b) {
       f32x16 s = BIAS ? bias(sl, t * kKeys + b * 32, wave_row, half * 4 - qpos)
                       : f32x16{};
@@ -424,8 +439,9 @@ __global__ __launch_bounds__(NW * 64, 2) void doc_attn_dkv_kernel(AttnArgs a) {
   const Tile tl = find_tile<ROWS>(a, bid % tiles);
   if (tl.row0 >= tl.len) return;
   const int lane = threadIdx.x & (kWave - 1);
-  const int wid = threadIdx.x / kWave;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int half = lane >> 5;
+  const bool mine = tl.row0 + wid * 32 < tl.len;
   const int kpos = tl.row0 + wid * 32 + (lane & 31);
   const bool real = kpos < tl.len;
   const long half_part = (long)a.splits * a.tokens * kv_heads * a.dim;
@@ -480,6 +496,7 @@ __global__ __launch_bounds__(NW * 64, 2) void doc_attn_dkv_kernel(AttnArgs a) {
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
     if (n + 1 < n1) stage(n + 1, lds + (2 * TS - LQ), stat[1 - H]);
+    if (!mine) return;
     const float sl = BIAS ? a.slopes[kvh * a.group + n / nt] / a.scale : 0.f;
     unroll<2>([&](auto b) {
       const int q0 = b * 32 + half * 4;
@@ -660,33 +677,46 @@ unsigned blocks_of(const AttnArgs& a, int rows_, int heads) {
 enum { kFwd, kDq, kDkv };
 
 template <typename T, int DP, int NW, bool BIAS>
-void launch_one(int which, const AttnArgs& a, hipStream_t s) {
+void launch_grad(int which, const AttnArgs& a, hipStream_t s) {
   const unsigned b = blocks_of(
       a, NW * 32, which == kDkv ? a.heads / a.group * a.splits : a.heads);
-  if (which == kFwd)
-    doc_attn_fwd_kernel<T, DP, NW, BIAS><<<b, NW * 64, 0, s>>>(a);
-  else if (which == kDq)
+  if (which == kDq)
     doc_attn_dq_kernel<T, DP, NW, BIAS><<<b, NW * 64, 0, s>>>(a);
   else
     doc_attn_dkv_kernel<T, DP, NW, BIAS><<<b, NW * 64, 0, s>>>(a);
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool BIAS>
 void launch_tile(int which, const AttnArgs& a, hipStream_t s) {
-  if (a.slopes)
-    launch_one<T, DP, 4, true>(which, a, s);
+  const bool wide = a.tokens / (a.docs < 1 ? 1 : a.docs) >= kWide;
+  if (which == kFwd) {
+    if (wide)
+      doc_attn_fwd_kernel<T, DP, 8, BIAS>
+          <<<blocks_of(a, 256, a.heads), 512, 0, s>>>(a);
+    else
+      doc_attn_fwd_kernel<T, DP, 4, BIAS>
+          <<<blocks_of(a, 128, a.heads), 256, 0, s>>>(a);
+    return;
+  }
+  if constexpr (DP == 128) {
+    if (wide) return launch_grad<T, DP, 8, BIAS>(which, a, s);
+  }
+  launch_grad<T, DP, 4, BIAS>(which, a, s);
+}
+
+template <typename T>
+void launch_type(int which, const AttnArgs& a, hipStream_t s) {
+  if (a.dim <= 64)
+    a.slopes ? launch_tile<T, 64, true>(which, a, s)
+             : launch_tile<T, 64, false>(which, a, s);
   else
-    launch_one<T, DP, 4, false>(which, a, s);
+    a.slopes ? launch_tile<T, 128, true>(which, a, s)
+             : launch_tile<T, 128, false>(which, a, s);
 }
 
 void launch(int which, const AttnArgs& a, at::ScalarType t, hipStream_t s) {
-  if (t == at::kBFloat16) {
-    if (a.dim <= 64) launch_tile<BF16, 64>(which, a, s);
-    else launch_tile<BF16, 128>(which, a, s);
-  } else {
-    if (a.dim <= 64) launch_tile<FP16, 64>(which, a, s);
-    else launch_tile<FP16, 128>(which, a, s);
-  }
+  if (t == at::kBFloat16) launch_type<BF16>(which, a, s);
+  else launch_type<FP16>(which, a, s);
 }
 
 }  // namespace
