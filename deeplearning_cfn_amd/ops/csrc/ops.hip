@@ -144,14 +144,14 @@ std::vector<at::Tensor> embed_sum_bwd_impl(const at::Tensor& dy,
                                            at::ArrayRef<double> scales);
 
 // doc_attention.hip
-std::tuple<at::Tensor, at::Tensor> doc_attn_fwd_impl(
+std::tuple<at::Tensor, at::Tensor, at::Tensor> doc_attn_fwd_impl(
     const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
     const at::Tensor& cu, const c10::optional<at::Tensor>& slopes,
-    double scale, bool need_lse);
+    double scale, bool need_grad);
 void doc_attn_bwd_impl(const at::Tensor& dout, const at::Tensor& q,
                        const at::Tensor& k, const at::Tensor& v,
                        const at::Tensor& o, const at::Tensor& lse,
-                       const at::Tensor& cu,
+                       const at::Tensor& low, const at::Tensor& cu,
                        const c10::optional<at::Tensor>& slopes, double scale,
                        at::Tensor dq, at::Tensor dk, at::Tensor dv);
 
@@ -346,8 +346,8 @@ TORCH_LIBRARY(dlx_hip, m) {
   m.def("attn_bwd(Tensor grad, Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, float scale) -> (Tensor, Tensor, Tensor)");
   m.def("embed_sum_fwd(Tensor[] ids, Tensor[] tables, float[] scales) -> Tensor");
   m.def("embed_sum_bwd(Tensor dy, Tensor[] ids, int[] rows, float[] scales) -> Tensor[]");
-  m.def("doc_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor cu, Tensor? slopes, float scale, bool need_lse) -> (Tensor, Tensor)");
-  m.def("doc_attn_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, Tensor cu, Tensor? slopes, float scale, Tensor(a!) dq, Tensor(b!) dk, Tensor(c!) dv) -> ()");
+  m.def("doc_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor cu, Tensor? slopes, float scale, bool need_grad) -> (Tensor, Tensor, Tensor)");
+  m.def("doc_attn_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, Tensor low, Tensor cu, Tensor? slopes, float scale, Tensor(a!) dq, Tensor(b!) dk, Tensor(c!) dv) -> ()");
   m.def("embedding_sum(Tensor[] ids, Tensor[] tables, float[] scales) -> Tensor");
   m.def("doc_attention(Tensor q, Tensor k, Tensor v, Tensor cu, Tensor? slopes, float scale) -> Tensor");
   m.def("doc_attention_qkv(Tensor qkv, Tensor cu, Tensor? slopes, float scale) -> Tensor");

@@ -19,14 +19,14 @@ std::vector<at::Tensor> embed_sum_bwd_impl(const at::Tensor& dy,
                                            at::TensorList ids,
                                            at::IntArrayRef rows,
                                            at::ArrayRef<double> scales);
-std::tuple<at::Tensor, at::Tensor> doc_attn_fwd_impl(
+std::tuple<at::Tensor, at::Tensor, at::Tensor> doc_attn_fwd_impl(
     const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
     const at::Tensor& cu, const c10::optional<at::Tensor>& slopes,
-    double scale, bool need_lse);
+    double scale, bool need_grad);
 void doc_attn_bwd_impl(const at::Tensor& dout, const at::Tensor& q,
                        const at::Tensor& k, const at::Tensor& v,
                        const at::Tensor& o, const at::Tensor& lse,
-                       const at::Tensor& cu,
+                       const at::Tensor& low, const at::Tensor& cu,
                        const c10::optional<at::Tensor>& slopes, double scale,
                        at::Tensor dq, at::Tensor dk, at::Tensor dv);
 
@@ -94,9 +94,9 @@ struct DocAttention : Function<DocAttention> {
                             const c10::optional<at::Tensor>& slopes,
                             double scale) {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [o, lse] = doc_attn_fwd_impl(q, k, v, cu, slopes, scale, true);
+    auto [o, lse, low] = doc_attn_fwd_impl(q, k, v, cu, slopes, scale, true);
     ctx->save_for_backward(
-        {q, k, v, o, lse, cu, slopes ? *slopes : at::Tensor()});
+        {q, k, v, o, lse, low, cu, slopes ? *slopes : at::Tensor()});
     ctx->saved_data["scale"] = scale;
     return o;
   }
@@ -108,10 +108,10 @@ struct DocAttention : Function<DocAttention> {
     const auto s = ctx->get_saved_variables();
     for (int i = 0; i < 3; ++i) out[i] = at::empty(s[i].sizes(), s[i].options());
     c10::optional<at::Tensor> slopes;
-    if (s[6].defined()) slopes = s[6];
-    doc_attn_bwd_impl(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], slopes,
-                      ctx->saved_data["scale"].toDouble(), out[0], out[1],
-                      out[2]);
+    if (s[7].defined()) slopes = s[7];
+    doc_attn_bwd_impl(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], s[6],
+                      slopes, ctx->saved_data["scale"].toDouble(), out[0],
+                      out[1], out[2]);
     return out;
   }
 };
@@ -124,10 +124,11 @@ struct DocAttentionQKV : Function<DocAttentionQKV> {
                             const c10::optional<at::Tensor>& slopes,
                             double scale) {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [o, lse] =
+    auto [o, lse, low] =
         doc_attn_fwd_impl(qkv.select(1, 0), qkv.select(1, 1), qkv.select(1, 2),
                           cu, slopes, scale, true);
-    ctx->save_for_backward({qkv, o, lse, cu, slopes ? *slopes : at::Tensor()});
+    ctx->save_for_backward(
+        {qkv, o, lse, low, cu, slopes ? *slopes : at::Tensor()});
     ctx->saved_data["scale"] = scale;
     return o;
   }
@@ -140,9 +141,9 @@ struct DocAttentionQKV : Function<DocAttentionQKV> {
     const auto& qkv = s[0];
     out[0] = at::empty(qkv.sizes(), qkv.options());
     c10::optional<at::Tensor> slopes;
-    if (s[4].defined()) slopes = s[4];
+    if (s[5].defined()) slopes = s[5];
     doc_attn_bwd_impl(grads[0], qkv.select(1, 0), qkv.select(1, 1),
-                      qkv.select(1, 2), s[1], s[2], s[3], slopes,
+                      qkv.select(1, 2), s[1], s[2], s[3], s[4], slopes,
                       ctx->saved_data["scale"].toDouble(), out[0].select(1, 0),
                       out[0].select(1, 1), out[0].select(1, 2));
     return out;
