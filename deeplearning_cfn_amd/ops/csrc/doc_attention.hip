@@ -29,9 +29,6 @@
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 
-#include <cmath>
-#include <limits>
-
 #include "mfma_tile.h"
 
 namespace dlx {
@@ -679,8 +676,8 @@ void check_inputs(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                     slopes->size(0) == q.size(1) && slopes->is_contiguous() &&
                     slopes->device() == q.device(),
                 "document_attention: slopes is a float32 vector, one a head");
-  TORCH_CHECK(std::isfinite(scale) && scale > 0,
-              "document_attention: scale has to be positive and finite");
+  TORCH_CHECK(scale >= 1e-30 && scale <= 1e30,
+              "document_attention: scale has to lie between 1e-30 and 1e30");
 }
 
 void fill(AttnArgs& a, const at::Tensor& q, const at::Tensor& k,
@@ -701,7 +698,8 @@ void fill(AttnArgs& a, const at::Tensor& q, const at::Tensor& k,
 
 unsigned blocks_of(const AttnArgs& a, int rows_, int heads) {
   const long n = ((long)a.tokens / rows_ + a.docs + 2) * heads;
-  TORCH_CHECK(n <= std::numeric_limits<int>::max(),
+  // a grid has under 2^32 threads, two a row
+  TORCH_CHECK(n * rows_ < (1l << 31),
               "document_attention: too many tokens or documents");
   return (unsigned)n;
 }
@@ -808,7 +806,11 @@ void doc_attn_bwd_impl(const at::Tensor& dout_in, const at::Tensor& q_in,
                   dq.device() == q_in.device() &&
                   dk.device() == q_in.device() && dv.device() == q_in.device(),
               "document_attention: dq, dk, dv do not fit q, k, v");
-  if (q_in.numel() == 0) return;
+  if (q_in.numel() == 0) {
+    dk.zero_();
+    dv.zero_();
+    return;
+  }
   const auto q = rows(q_in), k = rows(k_in), v = rows(v_in);
   const auto dout = rows(dout_in);
   auto delta = at::empty({q.size(1), q.size(0)}, lse.options());

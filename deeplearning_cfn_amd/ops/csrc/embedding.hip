@@ -27,8 +27,6 @@
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 
-#include <limits>
-
 #include "seq_common.h"
 
 namespace dlx {
@@ -78,31 +76,33 @@ template <typename T, int VEC>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(
     LookupArgs a, T* __restrict__ y, long n, int width, int nvec,
     uint32_t div_mul, int div_sh, int tokens) {
-  const long t0 = (long)blockIdx.x * tokens;
-  const int here = (int)(n - t0 < tokens ? n - t0 : tokens);
-  const int items = here * nvec;
+  for (long t0 = (long)blockIdx.x * tokens; t0 < n;
+       t0 += (long)gridDim.x * tokens) {
+    const int here = (int)(n - t0 < tokens ? n - t0 : tokens);
+    const int items = here * nvec;
 #pragma unroll 4
-  for (int it = threadIdx.x; it < items; it += 256) {
-    const int tl = (int)(((uint64_t)it * div_mul) >> div_sh);
-    const int c = (it - tl * nvec) * VEC;
-    float acc[VEC];
+    for (int it = threadIdx.x; it < items; it += 256) {
+      const int tl = (int)(((uint64_t)it * div_mul) >> div_sh);
+      const int c = (it - tl * nvec) * VEC;
+      float acc[VEC];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
-    for (int j = 0; j < a.n; ++j) {
-      const long id = read_id(a.t[j].ids, a.t[j].ids64, t0 + tl);
-      if (id < 0 || id >= a.t[j].rows) {
+      for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
+      for (int j = 0; j < a.n; ++j) {
+        const long id = read_id(a.t[j].ids, a.t[j].ids64, t0 + tl);
+        if (id < 0 || id >= a.t[j].rows) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i)
-          acc[i] = __builtin_nanf("");
-      } else {
-        float w[VEC];
-        load_vec<T, VEC>(static_cast<const T*>(a.t[j].weight) + id * width + c,
-                         w);
+          for (int i = 0; i < VEC; ++i)
+            acc[i] = __builtin_nanf("");
+        } else {
+          float w[VEC];
+          load_vec<T, VEC>(static_cast<const T*>(a.t[j].weight) + id * width + c,
+                           w);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) acc[i] += a.t[j].scale * w[i];
+          for (int i = 0; i < VEC; ++i) acc[i] += a.t[j].scale * w[i];
+        }
       }
+      store_vec<T, VEC>(y + (t0 + tl) * width + c, acc);
     }
-    store_vec<T, VEC>(y + (t0 + tl) * width + c, acc);
   }
 }
 
@@ -627,9 +627,7 @@ void launch_fwd(const LookupArgs& a, at::Tensor& y, long n, int width,
   int sh = 31;
   while ((1ull << (sh - 31)) < (uint64_t)nvec) ++sh;
   const uint64_t mul = ((1ull << sh) + nvec - 1) / nvec;
-  const long blocks = (n + tokens - 1) / tokens;
-  TORCH_CHECK(blocks <= std::numeric_limits<int>::max(),
-              "embedding: too many tokens");
+  const long blocks = std::min<long>((n + tokens - 1) / tokens, 1 << 20);
   embed_fwd_kernel<T, VEC><<<(unsigned)blocks, 256, 0, s>>>(
       a, static_cast<T*>(y.data_ptr()), n, width, nvec, (uint32_t)mul, sh,
       (int)tokens);
@@ -666,7 +664,7 @@ at::Tensor embed_sum_fwd_impl(at::TensorList ids_in, at::TensorList tables_in,
   TORCH_CHECK(w0.dim() == 2, "embedding: a table is [rows, width]");
   const c10::DeviceGuard guard(w0.device());
   const long n = ids_in[0].numel(), width = w0.size(1);
-  TORCH_CHECK(width <= (1 << 22), "embedding: a row is too wide");
+  TORCH_CHECK(width <= (1 << 21), "embedding: a row is too wide");
   std::vector<at::Tensor> hold;
   LookupArgs a{};
   a.n = (int)nt;
@@ -722,7 +720,7 @@ std::vector<at::Tensor> embed_sum_bwd_impl(const at::Tensor& dy_in,
   const c10::DeviceGuard guard(dy_in.device());
   const auto dy = dy_in.contiguous();
   const long n = dy.size(0), width = dy.size(1);
-  TORCH_CHECK(width <= (1 << 22) && n <= (1 << 30),
+  TORCH_CHECK(width <= (1 << 21) && n <= (1 << 30),
               "embedding: the gradient is too large");
   const long slots = n / kSlotUnit + 1;
   const long joins = n / kPiece + 1;
@@ -783,8 +781,9 @@ std::vector<at::Tensor> embed_sum_bwd_impl(const at::Tensor& dy_in,
     t.part = part.data_ptr<float>() + (long)j * slots * width;
   }
   const long blocks = (long)nt * slots + light_blocks;
-  TORCH_CHECK(blocks <= std::numeric_limits<int>::max(),
-              "embedding: the tables are too large");
+  // a grid has under 2^32 threads in x
+  TORCH_CHECK(blocks < (1l << 24),
+              "embedding: too many tokens, or too large tables");
   auto s = at::cuda::getCurrentCUDAStream();
   const size_t lds = ((size_t)kSortWaves * (most + 2)) * sizeof(int);
   if (direct) {

@@ -680,27 +680,30 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor,
 # attention inside packed documents (doc_attention.hip)
 # ---------------------------------------------------------------------------
 
-def _doc_attention_args(name, q, k, cu, scale, slopes):
+def _doc_attention_args(name, q, heads, kv_heads, cu, scale, slopes):
     if cu.dim() != 1 or cu.numel() < 1 or cu.dtype not in (torch.int32,
                                                            torch.int64):
         raise ValueError(f"{name}: cu_seqlens is a vector of int32 or int64")
-    if k.shape[1] < 1 or q.shape[1] % k.shape[1]:
+    if kv_heads < 1 or heads % kv_heads:
         raise ValueError(f"{name}: query heads have to be a multiple of key "
-                         f"heads, got {q.shape[1]} and {k.shape[1]}")
+                         f"heads, got {heads} and {kv_heads}")
     if cu.device != q.device:
         raise ValueError(f"{name}: cu_seqlens is on another device")
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
-    if not (math.isfinite(scale) and scale > 0):
-        raise ValueError(f"{name}: scale has to be positive and finite")
+    if not 1e-30 <= scale <= 1e30:
+        raise ValueError(f"{name}: scale has to lie between 1e-30 and 1e30")
     if slopes is not None:
         if slopes.requires_grad:
             raise ValueError(f"{name}: slopes are constants, they get no "
                              "gradient")
-        if slopes.shape != (q.shape[1],) or slopes.device != q.device:
+        if slopes.shape != (heads,) or slopes.device != q.device:
             raise ValueError(f"{name}: slopes has one number a query head, "
                              "on the same device")
         slopes = slopes.float().contiguous()
-    return cu.to(torch.int32).contiguous(), scale, slopes
+    if cu.dtype != torch.int32 or not cu.is_contiguous():
+        # what lies outside int32 is cut off like what lies outside the tokens
+        cu = cu.clamp(-1, 2 ** 31 - 1).to(torch.int32).contiguous()
+    return cu, scale, slopes
 
 
 def _doc_attention_native(t: torch.Tensor) -> bool:
@@ -742,7 +745,8 @@ def document_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     ``cu_seqlens`` [documents + 1]: document i is the tokens from
     ``cu_seqlens[i]`` to ``cu_seqlens[i + 1]``, in rising order; empty ones
     are allowed.  Tokens in no document get zeros, and zero gradients.
-    ``scale`` (default dim ** -0.5) is positive.  ``slopes`` [heads] takes
+    ``scale`` (default dim ** -0.5) lies between 1e-30 and
+    1e30.  ``slopes`` [heads] takes
     ``slopes[h] * |i - j|`` off the scores; it gets no gradient.
 
     Fused CDNA4 kernels for bf16 and fp16 with dim a multiple of 8 up to 128;
@@ -756,8 +760,9 @@ def document_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
             f"{tuple(k.shape)}, {tuple(v.shape)}")
     if not q.dtype == k.dtype == v.dtype:
         raise ValueError("document_attention: q, k and v differ in type")
-    cu, scale, slopes = _doc_attention_args("document_attention", q, k,
-                                            cu_seqlens, scale, slopes)
+    cu, scale, slopes = _doc_attention_args(
+        "document_attention", q, q.shape[1], k.shape[1], cu_seqlens, scale,
+        slopes)
     if _doc_attention_native(q):
         return native().doc_attention(q, k, v, cu, slopes, scale)
     return _doc_attention_composed(q, k, v, cu, scale, slopes)
@@ -783,12 +788,12 @@ def document_attention_qkv(qkv: torch.Tensor, cu_seqlens: torch.Tensor,
     if qkv.dim() != 4 or qkv.shape[1] != 3:
         raise ValueError("document_attention_qkv: [tokens, 3, heads, dim] "
                          f"expected, got {tuple(qkv.shape)}")
-    q, k, v = qkv.unbind(1)
-    cu, scale, slopes = _doc_attention_args("document_attention_qkv", q, k,
-                                            cu_seqlens, scale, slopes)
+    heads = qkv.shape[2]
+    cu, scale, slopes = _doc_attention_args(
+        "document_attention_qkv", qkv, heads, heads, cu_seqlens, scale, slopes)
     if _doc_attention_native(qkv):
         return native().doc_attention_qkv(qkv, cu, slopes, scale)
-    return _doc_attention_composed(q, k, v, cu, scale, slopes)
+    return _doc_attention_composed(*qkv.unbind(1), cu, scale, slopes)
 
 
 # ---------------------------------------------------------------------------

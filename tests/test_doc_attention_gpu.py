@@ -351,3 +351,119 @@ def test_on_another_stream():
     s.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+def test_extreme_scales():
+    """Close to the borders of what scale may be, all stays finite and right:
+    the mean of the values, and the value of the best key."""
+    F_amd = _f()
+    q, k, v, do = _inputs(60, 1, 1, 64, torch.bfloat16)
+    cu = torch.tensor([0, 60], device="cuda", dtype=torch.int32)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    o = F_amd.document_attention(*leaves, cu, scale=1e-30)
+    mean = v.double().mean(0, keepdim=True)
+    size = v.double().abs().mean(0, keepdim=True)
+    assert ((o.double() - mean).abs() <= 2.0 ** -7 * size).all()
+    for g in torch.autograd.grad(o, leaves, do):
+        assert g.isfinite().all()
+    o = F_amd.document_attention(*leaves, cu, scale=1e5)
+    best = (q[:, 0].double() @ k[:, 0].double().t()).argmax(1)
+    # the best key's exponent is its score less the row's rounded one, up to
+    # 2^22 * 2^-24 apart: its p is near 1, not 1, and is rounded (2^-8) before
+    # it is divided by itself; the result is rounded again (2^-8)
+    assert ((o.double() - v[best].double()).abs()
+            <= 2.0 ** -7 * 1.01 * v[best].double().abs()).all()
+
+
+def test_no_heads_and_no_tokens():
+    F_amd = _f()
+    cu = torch.tensor([0, 0], device="cuda", dtype=torch.int32)
+    q = torch.empty(0, 2, 64, device="cuda", dtype=torch.bfloat16,
+                    requires_grad=True)
+    o = F_amd.document_attention(q, q, q, cu)
+    assert o.shape == (0, 2, 64)
+    d, = torch.autograd.grad(o, [q], torch.empty_like(o))
+    assert d.shape == q.shape
+
+
+def test_large_borders_in_int64():
+    """Borders past 32 bits are cut off at the tokens like any other."""
+    F_amd = _f()
+    q, k, v, _ = _inputs(100, 1, 1, 64, torch.bfloat16)
+    cu = torch.tensor([-2 ** 40, 50, 2 ** 32 + 7], device="cuda")
+    want = torch.tensor([0, 50, 100], device="cuda", dtype=torch.int32)
+    assert torch.equal(F_amd.document_attention(q, k, v, cu),
+                       F_amd.document_attention(q, k, v, want))
+
+
+def test_what_the_graph_refuses():
+    """A graph of the gradients, and inputs changed before their use."""
+    F_amd = _f()
+    q, k, v, do = _inputs(50, 1, 1, 64, torch.bfloat16)
+    cu = torch.tensor([0, 20, 50], device="cuda", dtype=torch.int32)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    o = F_amd.document_attention(*leaves, cu)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        torch.autograd.grad(o, leaves, do, create_graph=True)
+    o = F_amd.document_attention(*leaves, cu)
+    cu[1] = 30
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(o, leaves, do)
+
+
+def test_only_some_gradients():
+    F_amd = _f()
+    q, k, v, do = _inputs(50, 2, 1, 64, torch.bfloat16)
+    cu = torch.tensor([0, 20, 50], device="cuda", dtype=torch.int32)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    want = torch.autograd.grad(F_amd.document_attention(*leaves, cu), leaves,
+                               do)
+    for n in range(3):
+        some = [t.detach().requires_grad_(i == n)
+                for i, t in enumerate(leaves)]
+        got, = torch.autograd.grad(F_amd.document_attention(*some, cu),
+                                   [some[n]], do)
+        assert torch.equal(got, want[n])
+    with torch.no_grad():
+        o = F_amd.document_attention(*leaves, cu)
+    assert not o.requires_grad
+    with torch.inference_mode():
+        assert torch.equal(F_amd.document_attention(*leaves, cu), o)
+
+
+def test_two_calls_at_once():
+    """Two streams, and two captured graphs replayed side by side."""
+    F_amd = _f()
+    sets = []
+    for seed in (1, 2):
+        q, k, v, do = _inputs(1500, 4, 1, 128, torch.bfloat16, seed)
+        sets.append(([t.requires_grad_(True) for t in (q, k, v)], do))
+    cu = torch.tensor([0, 700, 1500], device="cuda", dtype=torch.int32)
+
+    def step(n):
+        leaves, do = sets[n]
+        o = F_amd.document_attention(*leaves, cu)
+        return [o.detach(), *torch.autograd.grad(o, leaves, do)]
+
+    want = [step(0), step(1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for n, s in enumerate(streams):
+        with torch.cuda.stream(s):
+            got.append(step(n))
+    torch.cuda.synchronize()
+    graphs = []
+    for n in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step(n)
+        graphs.append((g, out))
+    for _ in range(3):
+        for (g, _), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for n in range(2):
+        for a, b, c in zip(want[n], got[n], graphs[n][1]):
+            assert torch.equal(a, b) and torch.equal(a, c)

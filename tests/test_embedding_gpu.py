@@ -213,3 +213,38 @@ def test_on_another_stream():
         d, = torch.autograd.grad(y, w, g)
     s.synchronize()
     assert torch.equal(y, want) and torch.equal(d, dwant)
+
+
+def test_one_table_twice_and_expanded_ids():
+    """The same table in two places of a sum; ids that are one row repeated."""
+    F_amd = _f()
+    w = _tables([40], 24, torch.float32)[0]
+    a = torch.randint(0, 40, (1, 50), device="cuda").expand(30, 50)
+    b = torch.randint(0, 40, (30, 50), device="cuda")
+    y = F_amd.embedding_sum([a, b], [w, w], [1.0, -0.5])
+    g = torch.randn_like(y)
+    d, = torch.autograd.grad(y, [w], g)
+    _, _, parts = _reference([a, b], [w, w], [1.0, -0.5], g)
+    _close(d, parts[0][0] + parts[1][0], parts[0][1] + parts[1][1],
+           parts[0][2] + parts[1][2])
+
+
+def test_what_the_graph_refuses():
+    F_amd = _f()
+    w = _tables([10], 8, torch.float32)
+    ids = torch.tensor([1, 2, 3], device="cuda")
+    y = F_amd.embedding(ids, w[0])
+    with pytest.raises(RuntimeError, match="no gradient"):
+        torch.autograd.grad(y, w, torch.ones_like(y), create_graph=True)
+    y = F_amd.embedding(ids, w[0])
+    ids[0] = 5
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(y, w, torch.ones_like(y))
+
+
+def test_many_short_rows():
+    """More tokens than one block each, around the border at which the sort
+    makes buckets first."""
+    for n in (4095, 4096, 4097, 70000):
+        ids = torch.randint(0, 3000, (n,), device="cuda")
+        _check([ids], _tables([3000], 3, torch.float32), [1.0])

@@ -122,6 +122,8 @@ CU = torch.tensor([0, 4])
     ((*_qkv(), CU), {"scale": -1.0}),
     ((*_qkv(), CU), {"scale": float("nan")}),
     ((*_qkv(), CU), {"scale": float("inf")}),
+    ((*_qkv(), CU), {"scale": 1e-40}),
+    ((*_qkv(H=0), CU), {"scale": 1e40}),
     ((*_qkv(), CU), {"slopes": torch.zeros(3)}),
     ((*_qkv(), CU), {"slopes": torch.zeros(2, 1)}),
     ((*_qkv(), CU), {"slopes": torch.zeros(2, requires_grad=True)}),
