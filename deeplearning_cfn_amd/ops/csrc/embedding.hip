@@ -335,7 +335,11 @@ __global__ __launch_bounds__(kSortThreads) void embed_order_kernel(GradArgs a,
   const int s1 = s0 + seg < end ? s0 + seg : end;
   const int bits = own > 1 ? 32 - __clz(own - 1) : 0;
   int less = 0, unused = 0;
-  for (int i = s0; i < s1; i += U * kWave) {
+  // a bucket of one id is in order already: of the three tables of 16384
+  // tokens, the small ones' (16384 tokens: 17.8 -> 13.4 us for this launch)
+  const bool alone = !DIRECT && own == 1;
+  if (alone && threadIdx.x == 0) lds[0] = end - start;
+  for (int i = s0; i < s1 && !alone; i += U * kWave) {
     int2 x[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -405,6 +409,11 @@ __global__ __launch_bounds__(kSortThreads) void embed_order_kernel(GradArgs a,
     }
   }
   if (top && threadIdx.x == 0) tb.first[lo + own] = last;
+  if (alone) {
+    for (int i = start + threadIdx.x; i < end; i += kSortThreads)
+      tb.order[i] = tb.loose[i].x;
+    return;
+  }
   __syncthreads();
 
   for (int i = s0; i < s1; i += U * kWave) {
