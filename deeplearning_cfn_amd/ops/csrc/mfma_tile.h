@@ -193,6 +193,19 @@ template <int DP> struct Frags {
     for (int i = 0; i < N; ++i)
       f[i] = __builtin_shufflevector(a[i], b[i], 0, 1, 2, 3, 4, 5, 6, 7);
   }
+
+  // tr of block 0 in two tiles, `more` bytes apart, for one wait
+  template <int OFF>
+  DLX_DEV void tr_both(s16x8* f, uint32_t more) const {
+    s16x4 a[2], b[2];
+    static_assert(OFF * 2 < 65536, "");
+    const uint32_t lo[2] = {lo_[0], lo_[0] + more};
+    const uint32_t hi[2] = {hi_[0], hi_[0] + more};
+    read_tr4<OFF * 2>(lo, hi, a, b);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      f[i] = __builtin_shufflevector(a[i], b[i], 0, 1, 2, 3, 4, 5, 6, 7);
+  }
 };
 
 // 16 bytes a lane from memory to LDS, lanes one behind the other there

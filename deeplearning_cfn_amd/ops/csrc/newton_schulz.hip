@@ -17,6 +17,8 @@
 // directions where B is large, which are those that no longer grow.  Against
 // 64 bits that leaves 7e-4 to 2.9e-3 relative (CPU model of these roundings,
 // four spectra, sizes 64 to 1024), next to bf16's own 1.7e-3 in the result.
+// With up to 64 rows, where few directions share a step's rounding, X, A and
+// B are two fp16 numbers each: 1.7e-3, the rounding of the result.
 // X is stored times 2^12: its entries stay under 2 and its small ones clear
 // of fp16's subnormals.
 #include <torch/extension.h>
@@ -54,6 +56,16 @@ DLX_DEV uint32_t low_parts(const float* x, const uint16_t* h) {
   for (int e = 0; e < 4; ++e) d[e] = (x[e] - h2f(h[e])) * kLowScale;
   int w = __builtin_amdgcn_cvt_pk_fp8_f32(d[0], d[1], 0, false);
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(d[2], d[3], w, true);
+}
+
+// The same as fp16, unscaled.
+template <int N>
+DLX_DEV Pack<uint16_t, N> low_halves(const float* x,
+                                     const Pack<uint16_t, N>& h) {
+  Pack<uint16_t, N> y;
+#pragma unroll
+  for (int e = 0; e < N; ++e) y.v[e] = from_f32<FP16>(x[e] - h2f(h.v[e])).v;
+  return y;
 }
 
 DLX_DEV void add_low(float* x, uint32_t low, float by) {
@@ -114,11 +126,11 @@ DLX_DEV double ns_sum(const double* part, int parts, double* red) {
 }
 
 // G to X_0: scaled, split in two, padded with zeros, a tall one transposed.
-// A block writes a 64 x 64 tile of X.
-template <typename T, int V>
+// A block writes a 64 x 64 tile of X.  WIDE: low parts of 16 bits.
+template <typename T, int V, bool WIDE>
 __global__ __launch_bounds__(256) void ns_split_kernel(
     const T* __restrict__ g, const double* __restrict__ part, int parts,
-    uint16_t* __restrict__ xh, uint8_t* __restrict__ xl, int rows, int cols,
+    uint16_t* __restrict__ xh, void* __restrict__ xl, int rows, int cols,
     bool tall, int np, int mp, float eps) {
   __shared__ float t[64][65];
   __shared__ double red[4];
@@ -151,7 +163,12 @@ __global__ __launch_bounds__(256) void ns_split_kernel(
       h.v[e] = from_f32<FP16>(v[e]).v;
     }
     *reinterpret_cast<Pack<uint16_t, 4>*>(xh + o) = h;
-    if (xl) *reinterpret_cast<uint32_t*>(xl + o) = low_parts(v, h.v);
+    if (WIDE)
+      *reinterpret_cast<Pack<uint16_t, 4>*>(static_cast<uint16_t*>(xl) + o) =
+          low_halves(v, h);
+    else if (xl)
+      *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(xl) + o) =
+          low_parts(v, h.v);
   }
 }
 
@@ -159,19 +176,24 @@ __global__ __launch_bounds__(256) void ns_split_kernel(
 // bytes for every thousand operations, which 128 leaves to the L2s' rate and
 // 256 does not; but 256 leaves few tiles.
 template <int TILE> struct Shape;
+template <> struct Shape<64> { static constexpr int WM = 2, WN = 2; };
 template <> struct Shape<128> { static constexpr int WM = 2, WN = 2; };
 template <> struct Shape<256> { static constexpr int WM = 2, WN = 4; };
 
 // out = by (in in^T)              POLY false: A from X
 // out = a I + b in + c (in in^T)  POLY true: B from A, columns quad-swapped
-template <int TILE, bool POLY>
+// SPLIT: in and out are two fp16 numbers each (all but the product of the low
+// ones is taken), and a matrix has one tile.
+template <int TILE, bool POLY, bool SPLIT>
 __global__ __launch_bounds__(Shape<TILE>::WM* Shape<TILE>::WN* kWave) void
 ns_square_kernel(const uint16_t* __restrict__ in, uint16_t* __restrict__ out,
-                 int np, int kp, int pairs) {
+                 const uint16_t* __restrict__ in_low,
+                 uint16_t* __restrict__ out_low, int np, int kp, int pairs) {
   constexpr int WM = Shape<TILE>::WM, WN = Shape<TILE>::WN;
   constexpr int NT = WM * WN * kWave, TS = TILE * kDepth;
   constexpr int FM = TILE / WM / 32, FN = TILE / WN / 32;
-  __shared__ __attribute__((aligned(16))) uint16_t lds[4 * TS];
+  constexpr int BUF = 2 * TS;                 // of one turn
+  __shared__ __attribute__((aligned(16))) uint16_t lds[2 * BUF];
   const int blk = xcd_block(blockIdx.x, gridDim.x);
   const int batch = blk / pairs;
   int rest = blk - batch * pairs, bi = 0;
@@ -187,18 +209,22 @@ ns_square_kernel(const uint16_t* __restrict__ in, uint16_t* __restrict__ out,
   const Frags<kDepth> fr(lds, lane);
   f32x16 acc[FM][FN] = {};
   const int nt = kp / kDepth;
-  stage_tile<TILE, kDepth, NT>(lds, src, kp, bj * TILE, 0);
-  stage_tile<TILE, kDepth, NT>(lds + TS, src, kp, bi * TILE, 0);
+  auto stage = [&](int t) {
+    uint16_t* to = lds + (t & 1) * BUF;
+    stage_tile<TILE, kDepth, NT>(to, src, kp, bj * TILE, t * kDepth);
+    // one tile alone is multiplied by itself
+    if (!SPLIT)
+      stage_tile<TILE, kDepth, NT>(to + TS, src, kp, bi * TILE, t * kDepth);
+    else
+      stage_tile<TILE, kDepth, NT>(to + TS, in_low + (long)batch * np * kp, kp,
+                                   0, t * kDepth);
+  };
+  stage(0);
   for (int t = 0; t < nt; ++t) {
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    const int la = (t & 1) * 2 * TS, lb = la + TS;
-    if (t + 1 < nt) {
-      uint16_t* nx = lds + ((t + 1) & 1) * 2 * TS;
-      stage_tile<TILE, kDepth, NT>(nx, src, kp, bj * TILE, (t + 1) * kDepth);
-      stage_tile<TILE, kDepth, NT>(nx + TS, src, kp, bi * TILE,
-                                   (t + 1) * kDepth);
-    }
+    const int la = (t & 1) * BUF, lb = SPLIT ? la : la + TS;
+    if (t + 1 < nt) stage(t + 1);
 #pragma unroll
     for (int st = 0; st < kDepth / 16; ++st) {
       s16x8 fa[FM], fb[FN];
@@ -213,6 +239,22 @@ ns_square_kernel(const uint16_t* __restrict__ in, uint16_t* __restrict__ out,
 #pragma unroll
         for (int v = 0; v < FN; ++v)
           acc[u][v] = mfma32<FP16>(fa[u], fb[v], acc[u][v]);
+      if constexpr (SPLIT) {
+        s16x8 ga[FM], gb[FN];
+#pragma unroll
+        for (int u = 0; u < FM; ++u)
+          ga[u] = fr.row(la + TS + (wr * FM + u) * 32 * kDepth, st);
+#pragma unroll
+        for (int u = 0; u < FN; ++u)
+          gb[u] = fr.row(la + TS + (wc * FN + u) * 32 * kDepth, st);
+#pragma unroll
+        for (int u = 0; u < FM; ++u)
+#pragma unroll
+          for (int v = 0; v < FN; ++v) {
+            acc[u][v] = mfma32<FP16>(ga[u], fb[v], acc[u][v]);
+            acc[u][v] = mfma32<FP16>(fa[u], gb[v], acc[u][v]);
+          }
+      }
     }
   }
   constexpr float by = POLY ? kNsC : 1.f / (kXScale * kXScale);
@@ -232,16 +274,24 @@ ns_square_kernel(const uint16_t* __restrict__ in, uint16_t* __restrict__ out,
           const Pack<uint16_t, 4> o =
               *reinterpret_cast<const Pack<uint16_t, 4>*>(src + (long)i * np +
                                                           j);
+          Pack<uint16_t, 4> l = {};
+          if (SPLIT)
+            l = *reinterpret_cast<const Pack<uint16_t, 4>*>(
+                in_low + ((long)batch * np + i) * np + j);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            x[e] += kNsB * h2f(o.v[e]) + (i == j + e ? kNsA : 0.f);
+            x[e] += kNsB * (SPLIT ? h2f(o.v[e]) + h2f(l.v[e]) : h2f(o.v[e])) +
+                    (i == j + e ? kNsA : 0.f);
         }
         Pack<uint16_t, 4> y;
 #pragma unroll
         for (int e = 0; e < 4; ++e) y.v[e] = from_f32<FP16>(x[e]).v;
         const int js = POLY ? quad_swap(j) : j;
         *reinterpret_cast<Pack<uint16_t, 4>*>(dst + (long)i * np + js) = y;
-        if (bi != bj) {
+        if (SPLIT)
+          *reinterpret_cast<Pack<uint16_t, 4>*>(
+              out_low + ((long)batch * np + i) * np + js) = low_halves(x, y);
+        if (!SPLIT && bi != bj) {
           const int is = POLY ? quad_swap(i) : i;
 #pragma unroll
           for (int e = 0; e < 4; ++e) dst[(long)(j + e) * np + is] = y.v[e];
@@ -255,19 +305,23 @@ struct NsUpdate {
   const uint8_t* xl;                  // or none
   uint16_t* yh;                       // the next X, or
   uint8_t* yl;                        // (or none)
+  const uint16_t *bw, *xw;            // SPLIT: the low halves
+  uint16_t* yw;
   uint16_t* out;                      // the result, bf16
   int np, mp, rows, cols;
   bool tall;
 };
 
 // B X, and a times the low part of X
-template <int TILE, bool LAST>
+// SPLIT: all but the product of the low halves (a lies on B's diagonal)
+template <int TILE, bool LAST, bool SPLIT>
 __global__ __launch_bounds__(Shape<TILE>::WM* Shape<TILE>::WN* kWave) void
 ns_update_kernel(NsUpdate a) {
   constexpr int WM = Shape<TILE>::WM, WN = Shape<TILE>::WN;
   constexpr int NT = WM * WN * kWave, TS = TILE * kDepth;
   constexpr int FM = TILE / WM / 32, FN = TILE / WN / 32;
-  __shared__ __attribute__((aligned(16))) uint16_t lds[4 * TS];
+  constexpr int BUF = (SPLIT ? 4 : 2) * TS;   // of one turn
+  __shared__ __attribute__((aligned(16))) uint16_t lds[2 * BUF];
   const int nbi = a.np / TILE, nbj = a.mp / TILE;
   int blk = xcd_block(blockIdx.x, gridDim.x);
   const int batch = blk / (nbi * nbj);
@@ -283,20 +337,23 @@ ns_update_kernel(NsUpdate a) {
   const Frags<TILE> fx(lds, lane, wr * FM * 32);
   f32x16 acc[FM][FN] = {};
   const int nt = a.np / kDepth;
-  stage_tile<kDepth, TILE, NT>(lds, a.xh + xo, a.mp, 0, bj * TILE);
-  stage_tile<TILE, kDepth, NT>(lds + TS, bm, a.np, bi * TILE, 0);
+  auto stage = [&](uint16_t* to, int t) {
+    stage_tile<kDepth, TILE, NT>(to, a.xh + xo, a.mp, t * kDepth, bj * TILE);
+    stage_tile<TILE, kDepth, NT>(to + TS, bm, a.np, bi * TILE, t * kDepth);
+    if (SPLIT) {
+      stage_tile<kDepth, TILE, NT>(to + 2 * TS, a.xw + xo, a.mp, t * kDepth,
+                                   bj * TILE);
+      stage_tile<TILE, kDepth, NT>(to + 3 * TS,
+                                   a.bw + (long)batch * a.np * a.np, a.np,
+                                   bi * TILE, t * kDepth);
+    }
+  };
+  stage(lds, 0);
   auto step = [&](int t, auto half) {
-    // the X tile of a turn at half * TS, so that its offsets stay short
-    constexpr int LX = decltype(half)::value * 2 * TS, LB = LX + TS;
+    constexpr int LX = decltype(half)::value * BUF, LB = LX + TS;
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    if (t + 1 < nt) {
-      uint16_t* nx = lds + (2 * TS - LX);
-      stage_tile<kDepth, TILE, NT>(nx, a.xh + xo, a.mp, (t + 1) * kDepth,
-                                   bj * TILE);
-      stage_tile<TILE, kDepth, NT>(nx + TS, bm, a.np, bi * TILE,
-                                   (t + 1) * kDepth);
-    }
+    if (t + 1 < nt) stage(lds + (BUF - LX), t + 1);
     unroll<kDepth / 16>([&](auto st) {
       s16x8 fa[FM], fb[FN];
 #pragma unroll
@@ -308,6 +365,22 @@ ns_update_kernel(NsUpdate a) {
 #pragma unroll
         for (int v = 0; v < FN; ++v)
           acc[u][v] = mfma32<FP16>(fa[u], fb[v], acc[u][v]);
+      if constexpr (SPLIT) {
+        s16x8 g[FM];
+        fx.template tr<FM, st * 16 * TILE>(g, (LX + 2 * TS) * 2);
+#pragma unroll
+        for (int u = 0; u < FM; ++u)
+#pragma unroll
+          for (int v = 0; v < FN; ++v)
+            acc[u][v] = mfma32<FP16>(g[u], fb[v], acc[u][v]);
+#pragma unroll
+        for (int v = 0; v < FN; ++v) {
+          const s16x8 low = fr.row(LX + 3 * TS + (wc * FN + v) * 32 * kDepth, st);
+#pragma unroll
+          for (int u = 0; u < FM; ++u)
+            acc[u][v] = mfma32<FP16>(fa[u], low, acc[u][v]);
+        }
+      }
     });
   };
   for (int t = 0; t < nt; t += 2) {
@@ -324,7 +397,7 @@ ns_update_kernel(NsUpdate a) {
   const int cj = threadIdx.x % PR * 8;
   const int j = bj * TILE + cj;
   auto place = [&](int row, int chunk) {
-    return img + row * TILE + ((chunk ^ (row & 31)) << 2);
+    return img + row * TILE + ((chunk ^ (row & 31 & (TILE / 4 - 1))) << 2);
   };
   constexpr int ROWS = NT / PR, TURNS = WN * 32 / ROWS;
   auto row_of = [&](int n) { return threadIdx.x / PR + n * ROWS; };
@@ -335,7 +408,7 @@ ns_update_kernel(NsUpdate a) {
 #pragma unroll
   for (int v = 0; v < FN; ++v) {
     uint2 low[TURNS] = {};                     // on their way meanwhile
-    if (a.xl) {
+    if (!SPLIT && a.xl) {
 #pragma unroll
       for (int n = 0; n < TURNS; ++n)
         low[n] = *reinterpret_cast<const uint2*>(a.xl + place_of(v, row_of(n)));
@@ -364,7 +437,7 @@ ns_update_kernel(NsUpdate a) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) x[e * 4 + k] = y.v[k];
       }
-      if (a.xl) {
+      if (!SPLIT && a.xl) {
         add_low(x, low[n].x, kNsA / kLowScale);
         add_low(x + 4, low[n].y, kNsA / kLowScale);
       }
@@ -373,7 +446,9 @@ ns_update_kernel(NsUpdate a) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) yh.v[e] = from_f32<FP16>(x[e]).v;
         *reinterpret_cast<P8*>(a.yh + o) = yh;
-        if (a.yl) {
+        if (SPLIT) {
+          *reinterpret_cast<P8*>(a.yw + o) = low_halves(x, yh);
+        } else if (a.yl) {
           *reinterpret_cast<uint2*>(a.yl + o) =
               make_uint2(low_parts(x, yh.v), low_parts(x + 4, yh.v + 4));
         }
@@ -416,10 +491,16 @@ ns_update_kernel(NsUpdate a) {
 
 // ---------------------------------------------------------------------------
 // Small matrices (up to 128 x 256): a block holds one and does every step.
-// X stays in fp32 in the registers, in the layout of the update's result;
-// its fp16 copy, A and B lie in LDS.  Bound by the waits between the three
-// products of a step.  One of 64 x 128: 15 us (in seventeen launches 127),
-// 512 of 128 x 256: 240 us (406 for 128 x 264, which takes the launches).
+// X stays in fp32 in the registers, in the layout of the update's result; its
+// fp16 copy, A and B lie in LDS.  With few singular values nothing evens out
+// what roundings to fp16 do to them in a step: up to 64 rows X, A and B are
+// two fp16 numbers each, and all products but those of two low ones are taken
+// (fp16 alone: 64 x 128 off by 1.6 times what rounding the result costs,
+// 1 x 5 by up to 14; so by 1.0); up to 128 rows B alone is (1.5; 1.3).
+// Bound by the waits between the three products of a step, and in the first
+// two by four waves' matrix instructions.  One of 64 x 128: 22 us (fp16 alone
+// 15; in seventeen launches 127), 512 of 128 x 256: 245 us (350 for
+// 128 x 264, which takes the launches).
 // ---------------------------------------------------------------------------
 
 template <typename T, int NP, int MP, int WAVES>
@@ -429,8 +510,13 @@ __global__ __launch_bounds__(WAVES* kWave) void ns_small_kernel(
   constexpr int TI = NP / 32, TJ = MP / 32;
   constexpr int MINE = (TI * TJ + WAVES - 1) / WAVES;
   constexpr int SQ = (TI * TI + WAVES - 1) / WAVES;
-  __shared__ __attribute__((aligned(16))) uint16_t lx[NP * MP], la[NP * NP],
-      lb[NP * NP];
+  // the second NP * MP of X and the second NP * NP of A and B: their low
+  // parts; B lies in A's place where LDS is short
+  constexpr bool ALL = NP == 64, SHARE = NP * MP > 1 << 14;
+  constexpr int XS = NP * MP, AS = NP * NP;
+  __shared__ __attribute__((aligned(16))) uint16_t lx[ALL ? 2 * XS : XS],
+      lb[2 * AS], la_own[SHARE ? 8 : ALL ? 2 * AS : AS];
+  uint16_t* la = SHARE ? lb : la_own;
   __shared__ double red[WAVES];
   const int lane = threadIdx.x & 63;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -468,16 +554,22 @@ __global__ __launch_bounds__(WAVES* kWave) void ns_small_kernel(
 #pragma unroll
     for (int r = 0; r < 16; ++r) x[u][r] *= by;
 
-  auto put = [&](uint16_t* tile, auto dp, int row, int col, const float* v) {
-    constexpr int DP = decltype(dp)::value;
-    Pack<uint16_t, 4> y;
+  auto put = [&](uint16_t* tile, auto dp, auto low, int row, int col,
+                 const float* v) {
+    constexpr int DP = decltype(dp)::value, LOW = decltype(low)::value;
+    using P4 = Pack<uint16_t, 4>;
+    P4 y;
 #pragma unroll
     for (int e = 0; e < 4; ++e) y.v[e] = from_f32<FP16>(v[e]).v;
-    *reinterpret_cast<Pack<uint16_t, 4>*>(tile + tile_at<DP>(row, col >> 3) +
-                                          (col & 7)) = y;
+    uint16_t* at = tile + tile_at<DP>(row, col >> 3) + (col & 7);
+    *reinterpret_cast<P4*>(at) = y;
+    if (LOW) *reinterpret_cast<P4*>(at + LOW) = low_halves(v, y);
   };
   using XW = std::integral_constant<int, MP>;
   using AW = std::integral_constant<int, NP>;
+  using XL = std::integral_constant<int, ALL ? XS : 0>;
+  using AL = std::integral_constant<int, ALL ? AS : 0>;
+  using BL = std::integral_constant<int, AS>;
   const Frags<MP> fx(lx, lane);
   const Frags<NP> fa(la, lane), fb(lb, lane);
 
@@ -490,7 +582,7 @@ __global__ __launch_bounds__(WAVES* kWave) void ns_small_kernel(
       for (int c = 0; c < 4; ++c) {
         const float v[4] = {x[u][c * 4], x[u][c * 4 + 1], x[u][c * 4 + 2],
                             x[u][c * 4 + 3]};
-        put(lx, XW{}, q % TI * 32 + (lane & 31), q / TI * 32 + c * 8 + half * 4,
+        put(lx, XW{}, XL{}, q % TI * 32 + (lane & 31), q / TI * 32 + c * 8 + half * 4,
             v);
       }
     }
@@ -500,39 +592,69 @@ __global__ __launch_bounds__(WAVES* kWave) void ns_small_kernel(
       const int q = wid + u * WAVES;
       if (q >= TI * TI) break;
       const int ti = q % TI * 32, tj = q / TI * 32;
-      f32x16 acc = {};
+      f32x16 acc = {}, low = {};                // two chains of products
 #pragma unroll
-      for (int st = 0; st < MP / 16; ++st)
-        acc = mfma32<FP16>(fx.row(tj * MP, st), fx.row(ti * MP, st), acc);
+      for (int st = 0; st < MP / 16; ++st) {
+        const s16x8 f = fx.row(tj * MP, st), h = fx.row(ti * MP, st);
+        acc = mfma32<FP16>(f, h, acc);
+        if (ALL) {
+          low = mfma32<FP16>(fx.row(XS + tj * MP, st), h, low);
+          low = mfma32<FP16>(f, fx.row(XS + ti * MP, st), low);
+        }
+      }
+      if (ALL) acc += low;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         float v[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           v[e] = acc[c * 4 + e] * (1.f / (kXScale * kXScale));
-        put(la, AW{}, ti + (lane & 31), tj + c * 8 + half * 4, v);
+        put(la, AW{}, AL{}, ti + (lane & 31), tj + c * 8 + half * 4, v);
       }
     }
     __syncthreads();
+    f32x16 bt[SQ] = {};
 #pragma unroll
     for (int u = 0; u < SQ; ++u) {              // B = b A + c A A
       const int q = wid + u * WAVES;
       if (q >= TI * TI) break;
       const int ti = q % TI * 32, tj = q / TI * 32;
-      f32x16 acc = {};
+      f32x16 low = {};
 #pragma unroll
-      for (int st = 0; st < NP / 16; ++st)
-        acc = mfma32<FP16>(fa.row(tj * NP, st), fa.row(ti * NP, st), acc);
+      for (int st = 0; st < NP / 16; ++st) {
+        const s16x8 f = fa.row(tj * NP, st), h = fa.row(ti * NP, st);
+        bt[u] = mfma32<FP16>(f, h, bt[u]);
+        if (ALL) {
+          low = mfma32<FP16>(fa.row(AS + tj * NP, st), h, low);
+          low = mfma32<FP16>(f, fa.row(AS + ti * NP, st), low);
+        }
+      }
+      if (ALL) bt[u] += low;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const int i = ti + (lane & 31), j = tj + c * 8 + half * 4;
-        const Pack<uint16_t, 4> o = *reinterpret_cast<const Pack<uint16_t, 4>*>(
-            la + tile_at<NP>(i, j >> 3) + (j & 7));
-        float v[4];
+        const uint16_t* at = la + tile_at<NP>(i, j >> 3) + (j & 7);
+        const auto o = *reinterpret_cast<const Pack<uint16_t, 4>*>(at);
+        Pack<uint16_t, 4> l = {};
+        if (ALL) l = *reinterpret_cast<const Pack<uint16_t, 4>*>(at + AS);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          v[e] = kNsC * acc[c * 4 + e] + kNsB * h2f(o.v[e]);
-        put(lb, AW{}, i, quad_swap(j), v);
+          bt[u][c * 4 + e] =
+              kNsC * bt[u][c * 4 + e] +
+              kNsB * (ALL ? h2f(o.v[e]) + h2f(l.v[e]) : h2f(o.v[e]));
+      }
+    }
+    if (SHARE) __syncthreads();
+#pragma unroll
+    for (int u = 0; u < SQ; ++u) {
+      const int q = wid + u * WAVES;
+      if (q >= TI * TI) break;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float v[4] = {bt[u][c * 4], bt[u][c * 4 + 1], bt[u][c * 4 + 2],
+                            bt[u][c * 4 + 3]};
+        put(lb, AW{}, BL{}, q % TI * 32 + (lane & 31),
+            quad_swap(q / TI * 32 + c * 8 + half * 4), v);
       }
     }
     __syncthreads();
@@ -541,14 +663,20 @@ __global__ __launch_bounds__(WAVES* kWave) void ns_small_kernel(
       const int q = wid + u * WAVES;
       if (q >= TI * TJ) break;
       const Frags<MP> ft(lx, lane, q / TI * 32);
-      f32x16 acc = {};
+      f32x16 acc = {}, low = {};
       unroll<NP / 16>([&](auto st) {
-        s16x8 f;
-        ft.template tr<1, st * 16 * MP>(&f);
-        acc = mfma32<FP16>(f, fb.row(q % TI * 32 * NP, st), acc);
+        s16x8 f[2];
+        if constexpr (ALL) ft.template tr_both<st * 16 * MP>(f, XS * 2);
+        else ft.template tr<1, st * 16 * MP>(f);
+        const s16x8 h = fb.row(q % TI * 32 * NP, st);
+        acc = mfma32<FP16>(f[0], h, acc);
+        if (ALL) low = mfma32<FP16>(f[1], h, low);
+        auto& to = ALL ? low : acc;
+        to = mfma32<FP16>(f[0], fb.row(AS + q % TI * 32 * NP, st), to);
       });
 #pragma unroll
-      for (int r = 0; r < 16; ++r) x[u][r] = kNsA * x[u][r] + acc[r];
+      for (int r = 0; r < 16; ++r)
+        x[u][r] = kNsA * x[u][r] + (ALL ? acc[r] + low[r] : acc[r]);
     }
     __syncthreads();
   }
@@ -585,13 +713,18 @@ void launch_small(const at::Tensor& g, at::Tensor& out, int batch, int rows,
 
 template <typename T, int V>
 void launch_start(const at::Tensor& g, double* part, int parts, uint16_t* xh,
-                  uint8_t* xl, int batch, int rows, int cols, int np, int mp,
+                  void* xl, bool wide, int batch, int rows, int cols, int np, int mp,
                   float eps, hipStream_t s) {
   const T* p = static_cast<const T*>(g.data_ptr());
   ns_norm_kernel<T, V><<<dim3(parts, batch), 256, 0, s>>>(p, part,
                                                           (long)rows * cols);
-  ns_split_kernel<T, V><<<dim3(mp / 64, np / 64, batch), 256, 0, s>>>(
-      p, part, parts, xh, xl, rows, cols, rows > cols, np, mp, eps);
+  const dim3 grid(mp / 64, np / 64, batch);
+  if (wide)
+    ns_split_kernel<T, V, true><<<grid, 256, 0, s>>>(
+        p, part, parts, xh, xl, rows, cols, rows > cols, np, mp, eps);
+  else
+    ns_split_kernel<T, V, false><<<grid, 256, 0, s>>>(
+        p, part, parts, xh, xl, rows, cols, rows > cols, np, mp, eps);
 }
 
 // ---------------------------------------------------------------------------
@@ -771,9 +904,15 @@ at::Tensor newton_schulz_impl(const at::Tensor& g_in, int64_t steps,
                          pad(lo, kTile) * pad(hi, kTile) * 9 &&
                      batch * n256 * m256 >= 200;
   const bool large_square = large && batch * n256 * (n256 + 1) / 2 >= 200;
-  const long unit = large ? 256 : kTile;
+  // Few singular values: nothing evens out what they lose to a step, so X, A
+  // and B are two fp16 numbers each, in tiles of 64 (with the parts that more
+  // rows get, 40 x 1000 is off by 2.0 times what rounding the result costs,
+  // 4 x 400 by up to 2.75, 64 x 512 by 1.4, 128 x 264 by 1.25; so by 1.0; one of
+  // 40 x 1000 takes 92 us, in tiles of 128 without it 132).
+  const bool wide = lo <= 64;
+  const long unit = large ? 256 : wide ? 64 : kTile;
   const long np = pad(lo, unit), mp = pad(hi, unit);
-  TORCH_CHECK(batch * (np / kTile) * (mp / kTile) <=
+  TORCH_CHECK(batch * (np / 64) * (mp / 64) <=
                       std::numeric_limits<int>::max() &&
                   mp / 64 <= 65535,
               "newton_schulz: the matrices are too large or too many");
@@ -798,14 +937,17 @@ at::Tensor newton_schulz_impl(const at::Tensor& g_in, int64_t steps,
 
   const auto half = g.options().dtype(at::kHalf);
   auto x = at::empty({2, batch, np, mp}, half);       // X twice
-  auto low = at::empty({2, batch, np, mp}, g.options().dtype(at::kByte));
-  auto sq = at::empty({2, batch, np, np}, half);      // A, B
+  auto low = at::empty({2, batch, np, mp},
+                       wide ? half : g.options().dtype(at::kByte));
+  auto sq = at::empty({wide ? 4 : 2, batch, np, np}, half);   // A, B
   auto part = at::empty({batch, parts}, g.options().dtype(at::kDouble));
   auto* px = static_cast<uint16_t*>(x.data_ptr());
   auto* pa = static_cast<uint16_t*>(sq.data_ptr());
   auto* pl = static_cast<uint8_t*>(low.data_ptr());
+  auto* pw = static_cast<uint16_t*>(low.data_ptr());
   const long xs = batch * np * mp;
-  uint16_t* pb = pa + batch * np * np;
+  const long as = batch * np * np;
+  uint16_t* pb = pa + as;
 
   auto start = [&](auto tag) {
     using T = decltype(tag);
@@ -814,7 +956,8 @@ at::Tensor newton_schulz_impl(const at::Tensor& g_in, int64_t steps,
                     reinterpret_cast<uintptr_t>(g.data_ptr()) % 16 == 0;
     (v4 ? launch_start<T, 4> : launch_start<T, 1>)(
         g, part.data_ptr<double>(), (int)parts, px,
-        steps > 2 ? pl : nullptr, (int)batch, (int)rows, (int)cols, (int)np, (int)mp, (float)eps, s);
+        wide || steps > 2 ? low.data_ptr() : nullptr, wide, (int)batch,
+        (int)rows, (int)cols, (int)np, (int)mp, (float)eps, s);
   };
   switch (g.scalar_type()) {
     case at::kFloat: start(float{}); break;
@@ -823,45 +966,59 @@ at::Tensor newton_schulz_impl(const at::Tensor& g_in, int64_t steps,
     default:
       TORCH_CHECK(false, "newton_schulz: unsupported dtype ", g.scalar_type());
   }
+  using Thin = std::integral_constant<int, 64>;
   using Small = std::integral_constant<int, 128>;
   using Large = std::integral_constant<int, 256>;
-  auto square = [&](auto tile, auto poly, const uint16_t* in, uint16_t* to,
+  using Yes = std::true_type;
+  using No = std::false_type;
+  auto square = [&](auto tile, auto poly, auto split, const uint16_t* in,
+                    uint16_t* to, const uint16_t* in_low, uint16_t* to_low,
                     long depth) {
     constexpr int TILE = decltype(tile)::value;
     constexpr int NT = Shape<TILE>::WM * Shape<TILE>::WN * kWave;
     const long nb = np / TILE, pairs = nb * (nb + 1) / 2;
-    ns_square_kernel<TILE, decltype(poly)::value>
-        <<<(unsigned)(batch * pairs), NT, 0, s>>>(in, to, (int)np, (int)depth,
-                                                  (int)pairs);
+    ns_square_kernel<TILE, decltype(poly)::value, decltype(split)::value>
+        <<<(unsigned)(batch * pairs), NT, 0, s>>>(
+            in, to, in_low, to_low, (int)np, (int)depth, (int)pairs);
   };
-  auto update = [&](auto tile, auto last, const NsUpdate& u) {
+  auto update = [&](auto tile, auto split, bool last, const NsUpdate& u) {
     constexpr int TILE = decltype(tile)::value;
     constexpr int NT = Shape<TILE>::WM * Shape<TILE>::WN * kWave;
-    ns_update_kernel<TILE, decltype(last)::value>
-        <<<(unsigned)(batch * (np / TILE) * (mp / TILE)), NT, 0, s>>>(u);
+    const unsigned blocks = (unsigned)(batch * (np / TILE) * (mp / TILE));
+    if (last)
+      ns_update_kernel<TILE, true, decltype(split)::value>
+          <<<blocks, NT, 0, s>>>(u);
+    else
+      ns_update_kernel<TILE, false, decltype(split)::value>
+          <<<blocks, NT, 0, s>>>(u);
   };
   for (int64_t k = 0; k < steps; ++k) {
     uint16_t* cur = px + (k & 1) * xs;
     uint16_t* nxt = px + ((k + 1) & 1) * xs;
-    if (large_square) {
-      square(Large{}, std::false_type{}, cur, pa, mp);
-      square(Large{}, std::true_type{}, pa, pb, np);
+    uint16_t* cur_low = wide ? pw + (k & 1) * xs : nullptr;
+    uint16_t* a_low = wide ? pa + 2 * as : nullptr;
+    uint16_t* b_low = wide ? pa + 3 * as : nullptr;
+    if (wide) {
+      square(Thin{}, No{}, Yes{}, cur, pa, cur_low, a_low, mp);
+      square(Thin{}, Yes{}, Yes{}, pa, pb, a_low, b_low, np);
+    } else if (large_square) {
+      square(Large{}, No{}, No{}, cur, pa, nullptr, nullptr, mp);
+      square(Large{}, Yes{}, No{}, pa, pb, nullptr, nullptr, np);
     } else {
-      square(Small{}, std::false_type{}, cur, pa, mp);
-      square(Small{}, std::true_type{}, pa, pb, np);
+      square(Small{}, No{}, No{}, cur, pa, nullptr, nullptr, mp);
+      square(Small{}, Yes{}, No{}, pa, pb, nullptr, nullptr, np);
     }
-    // the last two X that are multiplied have no low part
-    const NsUpdate u{pb, cur, k + 2 < steps ? pl + (k & 1) * xs : nullptr, nxt,
-                     k + 3 < steps ? pl + ((k + 1) & 1) * xs : nullptr,
+    // the last two X that are multiplied have no low part (but a wide one)
+    const bool in_low = !wide && k + 2 < steps, to_low = !wide && k + 3 < steps;
+    const NsUpdate u{pb, cur, in_low ? pl + (k & 1) * xs : nullptr, nxt,
+                     to_low ? pl + ((k + 1) & 1) * xs : nullptr, b_low, cur_low,
+                     wide ? pw + ((k + 1) & 1) * xs : nullptr,
                      static_cast<uint16_t*>(out.data_ptr()), (int)np, (int)mp,
                      (int)rows, (int)cols, rows > cols};
     const bool last = k + 1 == steps;
-    if (large)
-      last ? update(Large{}, std::true_type{}, u)
-           : update(Large{}, std::false_type{}, u);
-    else
-      last ? update(Small{}, std::true_type{}, u)
-           : update(Small{}, std::false_type{}, u);
+    if (wide) update(Thin{}, Yes{}, last, u);
+    else if (large) update(Large{}, No{}, last, u);
+    else update(Small{}, No{}, last, u);
   }
   return out;
 }

@@ -62,6 +62,23 @@ def test_sizes(n, m):
     _check(_matrix(3, n, m, "flat"))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,m", [
+    (1, 5), (2, 2), (2, 9), (3, 3), (5, 6), (17, 9), (16, 16), (40, 64),
+    (64, 200), (1, 300), (4, 400), (2100, 3), (40, 1000), (64, 257)])
+def test_few_singular_values(n, m, dtype):
+    """Up to 64 rows X, A and B have 22 bits.  Rounding the result costs at
+    most 2^-8 of each element, so of the norm.  A step adds at most four
+    roundings of 2^-22, and a step multiplies what is there already by at
+    most |s p'(s) / p(s)| <= 5 for the s up to 1.21 that come up, so that
+    five leave 4 * 2^-22 (1 + 5 + 25 + 125 + 625) = 7.5e-4."""
+    g = _matrix(32, n, m, "flat", seed=3).to(dtype)
+    want = _exact(g)
+    off = (_f().newton_schulz(g).double() - want).flatten(-2).norm(dim=-1)
+    rel = off / want.flatten(-2).norm(dim=-1)
+    assert (rel <= 2 ** -8 + 7.5e-4).all(), rel.max().item()
+
+
 @pytest.mark.parametrize("b,n,m", [
     (24, 512, 1100), (24, 1100, 512), (60, 500, 500), (23, 700, 768),
     (200, 130, 250)])
