@@ -18,11 +18,12 @@
 // P^T are at once operand B of O^T = V^T P^T (mfma_tile.h).  The gradient of
 // keys and values takes S = Q K^T instead, a lane holding one key.  P is
 // rounded to the inputs' type for the second product, as its other operand
-// is, and so is ds; maxima, sums and all accumulators are fp32.  D takes o in
-// twice the bits (a training forward writes what rounding leaves of it): with
-// the rounded o alone, gradients in short documents are off by up to 1.57
-// times what rounding the exact ones costs, so by 1.41.  A pass over 16384
-// packed tokens takes 185 us instead of 181; with that part in a byte, 190.
+// is, and so is ds (in two parts where documents are short, kFine); maxima,
+// sums and all accumulators are fp32.  D takes o in twice the bits (a training
+// forward writes what rounding leaves of it): with the rounded o alone,
+// gradients are off by up to 1.57 times what rounding the exact ones costs, so
+// by 1.41.  A pass over 16384 packed tokens takes 185 us instead of 181; with
+// that part in a byte, 190.
 //
 // No atomics: dq comes from a pass over keys, dk and dv from a pass over
 // queries, each with its own recomputation of P (two products of seven).
@@ -45,6 +46,14 @@ constexpr float kLog2e = 1.4426950408889634f;
 // 273 / 269, 919 / 857, of the narrow ones 141 / 176, 231 / 255, 744 / 745,
 // which stay with four.
 constexpr int kWide = 1024;
+// Tokens of a document up to which P and dS are taken in two parts of the
+// inputs' type, and tokens of a call up to which they are in all of it (where
+// launches, not products, take the time).  In one part, with few terms to even
+// out its rounding, it leaves dq and dk off by 1.5 (at worst 2.3) times what
+// rounding the exact ones costs, in two by 1.0; in long documents one leaves
+// 1.41.  The second part costs 32 x 128 and 16384 packed tokens nothing that
+// shows (14 -> 14.7 us of the forward's 32 x 128).
+constexpr int kFine = 64, kFineAll = 1024;
 constexpr float kLazy = 8.f;          // P stays under 2^8
 
 __device__ const uint4 g_zero16 = {0, 0, 0, 0};
@@ -58,6 +67,7 @@ struct AttnArgs {
   View q, k, v, o, dout, dq, dk, dv;
   uint16_t* low;                      // [tokens, heads, dim]: what o leaves
   float* lse;                         // [heads, tokens], base 2
+  int fine;                           // tokens: P and dS in two parts
   float* delta;                       // [heads, tokens]
   const int* cu;
   const float* slopes;                // [heads] or none
@@ -213,6 +223,10 @@ DLX_DEV f32x16 bias(float sl, int k0, int wave_row, int shift) {
 // ---------------------------------------------------------------------------
 // forward: a wave owns 32 queries, a block NW waves; keys and values pass in
 // tiles of 64, the next one on its way while this one is worked on.
+// Bound by exp and the rest of the softmax, which take about as many cycles of
+// a SIMD as the matrix instructions and run beside them only in part: 2 x 8192
+// tokens, 12 heads of 64, slopes: 530 us (0.78 PFLOP/s); 16384 packed tokens
+// in documents up to 512: 52 us; 8192 tokens of 16 heads of 128: 275 us.
 // ---------------------------------------------------------------------------
 
 template <typename T, int DP, int NW, bool BIAS>
@@ -256,7 +270,8 @@ __global__ __launch_bounds__(NW * 64, DP == 64 ? 4 : 2) void doc_attn_fwd_kernel
   float m = -INFINITY, ms = 0.f, l = 0.f;
   f32x16 acc[DP / 32] = {};
 
-  auto body = [&](int t, auto half_) {
+  auto body = [&](int t, auto half_, auto fine_) {
+    constexpr bool FINE = decltype(fine_)::value;
     constexpr int LK = decltype(half_)::value * 2 * TS, LV = LK + TS;
     uint16_t* nx = lds + (2 * TS - LK);
     __builtin_amdgcn_s_waitcnt(0);
@@ -319,13 +334,23 @@ __global__ __launch_bounds__(NW * 64, DP == 64 ? 4 : 2) void doc_attn_fwd_kernel
 #pragma unroll
       for (int db = 0; db < DP / 32; ++db)
         acc[db] = mfma32<T>(vf[db], pf, acc[db]);
+      if constexpr (FINE) {
+        const s16x8 rest = pack_rest<T>(p, pf);
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+          acc[db] = mfma32<T>(vf[db], rest, acc[db]);
+      }
     });
   };
   // two tiles a turn, so that each half of LDS has its own addresses
-  for (int t = 0; t < nt; t += 2) {
-    body(t, std::integral_constant<int, 0>{});
-    if (t + 1 < nt) body(t + 1, std::integral_constant<int, 1>{});
-  }
+  auto walk = [&](auto fine) {
+    for (int t = 0; t < nt; t += 2) {
+      body(t, std::integral_constant<int, 0>{}, fine);
+      if (t + 1 < nt) body(t + 1, std::integral_constant<int, 1>{}, fine);
+    }
+  };
+  if (NW == 4 && tl.len <= a.fine) walk(std::true_type{});
+  else walk(std::false_type{});
   l += __shfl_xor(l, 32, kWave);
   if (!real) return;
   store_rows<T, DP>(a.o.p + token * a.o.token + head * a.o.head, acc, 1.f / l,
@@ -339,7 +364,9 @@ __global__ __launch_bounds__(NW * 64, DP == 64 ? 4 : 2) void doc_attn_fwd_kernel
 
 // ---------------------------------------------------------------------------
 // gradient of the queries: the forward's walk over the keys, a third product.
-// Also writes delta, which the next kernel reads.
+// Also writes delta, which the next kernel reads.  The same packed tokens:
+// 60 us; the same 16 heads of 128 on four key heads: 370 us, registers leaving
+// two waves to a SIMD.
 // ---------------------------------------------------------------------------
 
 template <typename T, int DP, int NW, bool BIAS>
@@ -399,8 +426,9 @@ __global__ __launch_bounds__(NW * 64, DP == 64 ? 3 : 2) void doc_attn_dq_kernel(
 #pragma unroll
   for (int i = 0; i < 16; ++i) less[i] = -delta;
 
-  auto body = [&](int t, auto half_) {
+  auto body = [&](int t, auto half_, auto fine_) {
     constexpr int LK = decltype(half_)::value * 2 * TS, LV = LK + TS;
+    constexpr bool FINE = decltype(fine_)::value;
     uint16_t* nx = lds + (2 * TS - LK);
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
@@ -435,16 +463,26 @@ __global__ __launch_bounds__(NW * 64, DP == 64 ? 3 : 2) void doc_attn_dq_kernel(
 #pragma unroll
         for (int db = 0; db < DP / 32; ++db)
           acc[db] = mfma32<T>(kf[db], df, acc[db]);
+        if constexpr (FINE) {
+          const s16x8 rest = pack_rest<T>(&ds[st * 8], df);
+#pragma unroll
+          for (int db = 0; db < DP / 32; ++db)
+            acc[db] = mfma32<T>(kf[db], rest, acc[db]);
+        }
       });
     });
   };
-  for (int t = 0; t < nt; t += 2) {
-    body(t, std::integral_constant<int, 0>{});
-    if (t + 1 < nt) body(t + 1, std::integral_constant<int, 1>{});
-  }
-  if (real)
+  auto walk = [&](auto fine) {
+    for (int t = 0; t < nt; t += 2) {
+      body(t, std::integral_constant<int, 0>{}, fine);
+      if (t + 1 < nt) body(t + 1, std::integral_constant<int, 1>{}, fine);
+    }
+  };
+  if (NW == 4 && tl.len <= a.fine) walk(std::true_type{});
+  else walk(std::false_type{});
+  if (real)             // of one score p is 1: nothing depends on q or k
     store_rows<T, DP>(a.dq.p + token * a.dq.token + head * a.dq.head, acc,
-                      a.scale, a.dim, lane);
+                      tl.len == 1 ? 0.f : a.scale, a.dim, lane);
 }
 
 // ---------------------------------------------------------------------------
@@ -452,10 +490,11 @@ __global__ __launch_bounds__(NW * 64, DP == 64 ? 3 : 2) void doc_attn_dq_kernel(
 // queries of every head that shares it pass in tiles of 64.  Shared heads
 // leave few such waves and give each a long walk: then the walk is split, its
 // parts' sums stay in fp32 and doc_attn_join_kernel adds them, in their order.
+// The same packed tokens: 77 us; the same 16 heads: 485 us and 23 to join.
 // ---------------------------------------------------------------------------
 
 template <typename T, int DP, int NW, bool BIAS>
-__global__ __launch_bounds__(NW * 64, 2) void doc_attn_dkv_kernel(AttnArgs a) {
+__global__ __launch_bounds__(NW * 64, DP == 64 ? 3 : 2) void doc_attn_dkv_kernel(AttnArgs a) {
   constexpr int NT = NW * 64, ROWS = NW * 32, TS = kKeys * DP;
   __shared__ __attribute__((aligned(16))) uint16_t lds[4 * TS];
   __shared__ __attribute__((aligned(16))) float stat[2][2][kKeys];
@@ -518,18 +557,19 @@ __global__ __launch_bounds__(NW * 64, 2) void doc_attn_dkv_kernel(AttnArgs a) {
   const Frags<DP> fr(lds, lane);
   f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
 
-  auto body = [&](int n, auto half_) {
+  // REST: what rounding P and dS has left, in a turn of its own over the same
+  // tile (in the first one it would need registers that are not there)
+  auto turn = [&](int n, auto half_, auto rest_) {
     constexpr int H = decltype(half_)::value;
+    constexpr bool REST = decltype(rest_)::value;
     constexpr int LQ = H * 2 * TS, LG = LQ + TS;
     const float (*st_)[kKeys] = stat[H];
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    if (n + 1 < n1) stage(n + 1, lds + (2 * TS - LQ), stat[1 - H]);
-    if (!mine) return;
+    int place = kpos;                  // nothing of the first turn is kept
+    if (REST) asm volatile("" : "+v"(place)::"memory");
     const float sl = BIAS ? a.slopes[kvh * a.group + n / nt] / a.scale : 0.f;
     unroll<2>([&](auto b) {
       const int q0 = b * 32 + half * 4;
-      const float d0 = (float)((n % nt) * kKeys + q0 - kpos);
+      const float d0 = (float)((n % nt) * kKeys + q0 - place);
       f32x16 s, dp;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
@@ -554,8 +594,11 @@ __global__ __launch_bounds__(NW * 64, 2) void doc_attn_dkv_kernel(AttnArgs a) {
           p[e] = __builtin_amdgcn_exp2f(s[st * 8 + e] * sc);
           ds[e] = p[e] * dp[st * 8 + e];
         }
-        const s16x8 pf = pack_step<T>(p);
-        const s16x8 df = pack_step<T>(ds);
+        s16x8 pf = pack_step<T>(p), df = pack_step<T>(ds);
+        if (REST) {
+          pf = pack_rest<T>(p, pf);
+          df = pack_rest<T>(ds, df);
+        }
         constexpr int at = (b * 2 + st) * 16 * DP;
         unroll<DP / 64>([&](auto h) {           // two operands at a time
           s16x8 f[2];
@@ -569,11 +612,24 @@ __global__ __launch_bounds__(NW * 64, 2) void doc_attn_dkv_kernel(AttnArgs a) {
       });
     });
   };
+  auto body = [&](int n, auto half_) {
+    constexpr int H = decltype(half_)::value;
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (n + 1 < n1) stage(n + 1, lds + (1 - H) * 2 * TS, stat[1 - H]);
+    if (!mine) return;
+    turn(n, half_, std::false_type{});
+    if (NW == 4 && tl.len <= a.fine) turn(n, half_, std::true_type{});
+  };
   for (int n = n0; n < n1; n += 2) {
     body(n, std::integral_constant<int, 0>{});
     if (n + 1 < n1) body(n + 1, std::integral_constant<int, 1>{});
   }
   if (!real) return;
+  if (tl.len == 1) {    // of one score p is 1: nothing depends on q or k
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b) dk[b] *= 0.f;
+  }
   if (a.splits > 1) {
     float* row = part_row(token);
 #pragma unroll
@@ -591,8 +647,8 @@ __global__ __launch_bounds__(NW * 64, 2) void doc_attn_dkv_kernel(AttnArgs a) {
       }
     return;
   }
-  store_rows<T, DP>(a.dk.p + token * a.dk.token + kvh * a.dk.head, dk, a.scale,
-                    a.dim, lane);
+  store_rows<T, DP>(a.dk.p + token * a.dk.token + kvh * a.dk.head, dk,
+                    a.scale, a.dim, lane);
   store_rows<T, DP>(a.dv.p + token * a.dv.token + kvh * a.dv.head, dv, 1.f,
                     a.dim, lane);
 }
@@ -694,6 +750,7 @@ void fill(AttnArgs& a, const at::Tensor& q, const at::Tensor& k,
   a.group = (int)(q.size(1) / k.size(1));
   a.dim = (int)q.size(2);
   a.scale = (float)scale;
+  a.fine = a.tokens <= kFineAll ? kFineAll : kFine;
 }
 
 unsigned blocks_of(const AttnArgs& a, int rows_, int heads) {

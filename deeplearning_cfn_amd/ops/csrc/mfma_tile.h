@@ -68,6 +68,14 @@ template <typename T> DLX_DEV s16x8 pack_step(const float* p) {
                    pack2<T>(p[4], p[5]), pack2<T>(p[6], p[7])});
 }
 
+// what pack_step's rounding leaves of them
+template <typename T> DLX_DEV s16x8 pack_rest(const float* p, s16x8 high) {
+  float rest[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) rest[e] = p[e] - to_f32<T>(T{(uint16_t)high[e]});
+  return pack_step<T>(rest);
+}
+
 template <int DP> DLX_DEV constexpr int swizzle(int r) {
   if (DP == 32) return ((r >> 2) & 1) | (((r >> 3) ^ (r >> 1)) & 1) << 1;
   if (DP == 64)

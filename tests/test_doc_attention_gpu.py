@@ -467,3 +467,52 @@ def test_two_calls_at_once():
     for n in range(2):
         for a, b, c in zip(want[n], got[n], graphs[n][1]):
             assert torch.equal(a, b) and torch.equal(a, c)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads,kv", [(4, 4), (8, 2)])
+@pytest.mark.parametrize("dim", [16, 64, 128])
+@pytest.mark.parametrize("lengths", [
+    [2], [1, 2, 2, 1], [3, 9, 1, 5], [17, 2, 30], [64, 63], [65, 200, 7],
+    [33] * 40])
+def test_short_documents_round_once(lengths, dim, heads, kv, dtype):
+    """Few terms even nothing out, so P and dS keep twice the type's bits: a
+    term is off by u^2, the terms' sizes add up to at most 16 times the
+    result's (sqrt(n) for n terms of random sign, n <= 200), and fp16's
+    subnormals leave 2^-25 of a p where typical ones are 2^-6 or more.  What
+    is left is the rounding of the result."""
+    more = 2.0 ** -12 if dtype == torch.bfloat16 else 2.0 ** -15
+    for seed in range(4):
+        q, k, v, do = _inputs(sum(lengths), heads, kv, dim, dtype, seed=seed)
+        ends = [0]
+        for n in lengths:
+            ends.append(ends[-1] + n)
+        cu = torch.tensor(ends, dtype=torch.int32, device="cuda")
+        for t in (q, k, v):
+            t.requires_grad_(True)
+        y = _f().document_attention(q, k, v, cu)
+        got = [y, *torch.autograd.grad(y, [q, k, v], do)]
+        with torch.no_grad():
+            want = _reference(q, k, v, do, ends, dim ** -0.5, None)[0]
+            for g, w in zip(got, want):
+                size = w.norm()
+                least = (w.to(dtype).double() - w).norm()
+                assert (g.double() - w).norm() <= least + more * size
+
+
+@pytest.mark.parametrize("heads,kv", [(4, 4), (8, 1)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_single_tokens_have_no_gradient_of_scores(heads, kv, dim):
+    """Of one score the softmax is 1, whatever q and k are."""
+    q, k, v, do = _inputs(100, heads, kv, dim, torch.bfloat16)
+    cu = torch.arange(101, dtype=torch.int32, device="cuda")
+    for t in (q, k, v):
+        t.requires_grad_(True)
+    y = _f().document_attention(q, k, v, cu)
+    dq, dk, dv = torch.autograd.grad(y, [q, k, v], do)
+    group = heads // kv
+    assert (y == v.repeat_interleave(group, 1)).all()
+    assert not dq.any() and not dk.any()
+    want = do.double().unflatten(1, (kv, group)).sum(2)
+    assert ((dv.double() - want).abs()
+            <= want.abs() * 2.0 ** -8 + 2.0 ** -20 * group).all()
