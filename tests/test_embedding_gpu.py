@@ -248,3 +248,20 @@ def test_many_short_rows():
     for n in (4095, 4096, 4097, 70000):
         ids = torch.randint(0, 3000, (n,), device="cuda")
         _check([ids], _tables([3000], 3, torch.float32), [1.0])
+
+
+def test_backward_again():
+    """With its graph kept a second pass gives the same; without it raises,
+    and so does a graph whose ids were written to in between."""
+    w = torch.randn(20, 8, device="cuda", requires_grad=True)
+    ids = torch.randint(0, 20, (30,), device="cuda")
+    y = _f().embedding_sum([ids], [w])
+    first, = torch.autograd.grad(y.sum(), w, retain_graph=True)
+    again, = torch.autograd.grad(y.sum(), w)
+    assert torch.equal(first, again)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y.sum(), w)
+    y = _f().embedding_sum([ids], [w])
+    ids.add_(0)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y.sum(), w)
