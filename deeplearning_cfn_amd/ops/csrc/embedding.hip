@@ -789,9 +789,10 @@ std::vector<at::Tensor> embed_sum_bwd_impl(const at::Tensor& dy_in,
     for (auto& o : out) o.zero_();
     return out;
   }
-  const auto work = at::empty({ints}, dy.options().dtype(at::kInt));
-  const auto part = at::empty({(long)nt * slots * width},
-                              dy.options().dtype(at::kFloat));
+  // the lists, then the pieces' sums
+  const auto work = at::empty({ints + (long)nt * slots * width},
+                              dy.options().dtype(at::kInt));
+  float* part = reinterpret_cast<float*>(work.data_ptr<int>() + ints);
   const bool direct = n <= kDirect;
   for (size_t j = 0; j < nt; ++j) {
     GradTable& t = a.t[j];
@@ -803,7 +804,7 @@ std::vector<at::Tensor> embed_sum_bwd_impl(const at::Tensor& dy_in,
     t.first = t.start + g + 1;
     t.slot_row = t.first + ((long)t.own << t.lg) + 1;
     t.join_row = t.slot_row + slots;
-    t.part = part.data_ptr<float>() + (long)j * slots * width;
+    t.part = part + (long)j * slots * width;
   }
   const long blocks = (long)nt * slots + light_blocks;
   // a grid has under 2^32 threads in x

@@ -45,6 +45,30 @@ void refuse_graph(const char* name) {
               ": its gradient has no gradient (create_graph)");
 }
 
+// What functional.embedding_sum checks elsewhere, for 4 us less of host time
+void check_lookup(at::TensorList ids, at::TensorList tables,
+                  at::ArrayRef<double> scales) {
+  const size_t n = tables.size();
+  TORCH_CHECK_VALUE(n >= 1 && n <= 4, "embedding_sum: 1 to 4 tables, got ", n);
+  TORCH_CHECK_VALUE(ids.size() == n && scales.size() == n,
+                    "embedding_sum: as many ids and scales as tables");
+  const at::Tensor& w0 = tables[0];
+  for (size_t j = 0; j < n; ++j) {
+    const at::Tensor &i = ids[j], &w = tables[j];
+    TORCH_CHECK_VALUE(
+        i.scalar_type() == at::kInt || i.scalar_type() == at::kLong,
+        "embedding_sum: ids are int32 or int64, got ", i.scalar_type());
+    TORCH_CHECK_VALUE(i.sizes() == ids[0].sizes(),
+                      "embedding_sum: the ids differ in shape");
+    TORCH_CHECK_VALUE(w.dim() == 2 && w.size(1) == w0.size(1) &&
+                          w.scalar_type() == w0.scalar_type(),
+                      "embedding_sum: tables are [rows, width], of one width "
+                      "and type");
+    TORCH_CHECK_VALUE(i.device() == w0.device() && w.device() == w0.device(),
+                      "embedding_sum: ids and tables are on different devices");
+  }
+}
+
 at::Tensor lookup(at::TensorList ids, at::TensorList tables,
                   at::ArrayRef<double> scales) {
   auto y = embed_sum_fwd_impl(ids, tables, scales);
@@ -165,7 +189,7 @@ bool wants_grad(at::TensorList ts) {
 // ids of one shape, tables [rows, width] -> [*shape, width]
 at::Tensor embedding_sum(at::TensorList ids, at::TensorList tables,
                          at::ArrayRef<double> scales) {
-  TORCH_CHECK(!ids.empty() && !tables.empty(), "embedding_sum: no tables");
+  check_lookup(ids, tables, scales);
   std::shared_ptr<EmbeddingSumBackward> node;
   if (wants_grad(tables)) {
     node.reset(new EmbeddingSumBackward, torch::autograd::deleteNode);

@@ -645,6 +645,9 @@ def embedding_sum(ids: Sequence[torch.Tensor], tables: Sequence[torch.Tensor],
     ids, tables = list(ids), list(tables)
     scales = [1.0] * len(tables) if scales is None else [float(c)
                                                          for c in scales]
+    if tables and _use_native(tables[0]) and tables[0].dtype in (
+            torch.bfloat16, torch.float16, torch.float32):
+        return native().embedding_sum(ids, tables, scales)  # checks the same
     if not 1 <= len(tables) <= 4:
         raise ValueError(f"embedding_sum: 1 to 4 tables, got {len(tables)}")
     if len(ids) != len(tables) or len(scales) != len(tables):
@@ -662,9 +665,6 @@ def embedding_sum(ids: Sequence[torch.Tensor], tables: Sequence[torch.Tensor],
         if i.device != w0.device or w.device != w0.device:
             raise ValueError("embedding_sum: ids and tables are on different "
                              "devices")
-    if _use_native(w0) and w0.dtype in (torch.bfloat16, torch.float16,
-                                        torch.float32):
-        return native().embedding_sum(ids, tables, scales)
     acc = sum(F.embedding(i, w).float() * c
               for i, w, c in zip(ids, tables, scales))
     return acc.to(w0.dtype)

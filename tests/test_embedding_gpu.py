@@ -265,3 +265,18 @@ def test_backward_again():
     ids.add_(0)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(y.sum(), w)
+
+
+def test_refusals_on_the_device():
+    """The same errors as on the CPU."""
+    f = _f().embedding_sum
+    w, w2 = (torch.randn(4, n, device="cuda") for n in (8, 9))
+    i = torch.zeros(3, dtype=torch.long, device="cuda")
+    for ids, tables, scales in (
+            ([i] * 5, [w] * 5, None), ([i], [w, w], None),
+            ([i, i], [w, w], [1.0]), ([i.float()], [w], None),
+            ([i, i[:2]], [w, w], None), ([i, i], [w, w2], None),
+            ([i, i], [w, w.half()], None), ([i], [w[0]], None),
+            ([i.cpu()], [w], None), ([i, i], [w, w.cpu()], None)):
+        with pytest.raises(ValueError, match="embedding_sum"):
+            f(ids, tables, scales)
