@@ -9,6 +9,7 @@
 // The gradients have no gradient of their own: asking for a graph of them
 // (create_graph) raises.  Saved inputs are checked for changes in place.
 #include <torch/extension.h>
+#include <limits>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 
@@ -67,6 +68,39 @@ void check_lookup(at::TensorList ids, at::TensorList tables,
     TORCH_CHECK_VALUE(i.device() == w0.device() && w.device() == w0.device(),
                       "embedding_sum: ids and tables are on different devices");
   }
+}
+
+// The same for document attention; borders as contiguous int32 (what lies
+// outside is cut off like what lies outside the tokens), slopes as fp32.
+std::pair<at::Tensor, c10::optional<at::Tensor>> attention_args(
+    const char* name, const at::Tensor& q, int64_t heads, int64_t kv_heads,
+    const at::Tensor& cu, const c10::optional<at::Tensor>& slopes,
+    double scale) {
+  TORCH_CHECK_VALUE(cu.dim() == 1 && cu.numel() >= 1 &&
+                        (cu.scalar_type() == at::kInt ||
+                         cu.scalar_type() == at::kLong),
+                    name, ": cu_seqlens is a vector of int32 or int64");
+  TORCH_CHECK_VALUE(kv_heads >= 1 && heads % kv_heads == 0, name,
+                    ": query heads have to be a multiple of key heads, got ",
+                    heads, " and ", kv_heads);
+  TORCH_CHECK_VALUE(cu.device() == q.device(), name,
+                    ": cu_seqlens is on another device");
+  TORCH_CHECK_VALUE(scale >= 1e-30 && scale <= 1e30, name,
+                    ": scale has to lie between 1e-30 and 1e30");
+  at::AutoDispatchBelowADInplaceOrView below;
+  c10::optional<at::Tensor> s;
+  if (slopes) {
+    TORCH_CHECK_VALUE(!slopes->requires_grad(), name,
+                      ": slopes are constants, they get no gradient");
+    TORCH_CHECK_VALUE(slopes->dim() == 1 && slopes->size(0) == heads &&
+                          slopes->device() == q.device(),
+                      name, ": slopes has one number a query head, on the same "
+                      "device");
+    s = slopes->to(at::kFloat).contiguous();
+  }
+  if (cu.scalar_type() == at::kInt && cu.is_contiguous()) return {cu, s};
+  return {cu.clamp(-1, std::numeric_limits<int>::max())
+              .to(at::kInt).contiguous(), s};
 }
 
 at::Tensor lookup(at::TensorList ids, at::TensorList tables,
@@ -208,20 +242,35 @@ at::Tensor embedding_sum(at::TensorList ids, at::TensorList tables,
 }
 
 at::Tensor doc_attention(const at::Tensor& q, const at::Tensor& k,
-                         const at::Tensor& v, const at::Tensor& cu,
-                         const c10::optional<at::Tensor>& slopes,
+                         const at::Tensor& v, const at::Tensor& cu_in,
+                         const c10::optional<at::Tensor>& slopes_in,
                          double scale) {
+  TORCH_CHECK_VALUE(
+      q.dim() == 3 && k.dim() == 3 && k.sizes() == v.sizes() &&
+          k.size(0) == q.size(0) && k.size(2) == q.size(2),
+      "document_attention: q is [tokens, heads, dim], k and v [tokens, "
+      "kv_heads, dim], got ", q.sizes(), ", ", k.sizes(), ", ", v.sizes());
+  TORCH_CHECK_VALUE(q.scalar_type() == k.scalar_type() &&
+                        q.scalar_type() == v.scalar_type(),
+                    "document_attention: q, k and v differ in type");
+  const auto [cu, slopes] =
+      attention_args("document_attention", q, q.size(1), k.size(1), cu_in,
+                     slopes_in, scale);
   if (wants_grad({q, k, v}))
     return DocAttention::apply(q, k, v, cu, slopes, scale);
   at::AutoDispatchBelowADInplaceOrView below;
   return std::get<0>(doc_attn_fwd_impl(q, k, v, cu, slopes, scale, false));
 }
 
-at::Tensor doc_attention_qkv(const at::Tensor& qkv, const at::Tensor& cu,
-                             const c10::optional<at::Tensor>& slopes,
+at::Tensor doc_attention_qkv(const at::Tensor& qkv, const at::Tensor& cu_in,
+                             const c10::optional<at::Tensor>& slopes_in,
                              double scale) {
-  TORCH_CHECK(qkv.dim() == 4 && qkv.size(1) == 3,
-              "document_attention_qkv: [tokens, 3, heads, dim] expected");
+  TORCH_CHECK_VALUE(qkv.dim() == 4 && qkv.size(1) == 3,
+                    "document_attention_qkv: [tokens, 3, heads, dim] expected, "
+                    "got ", qkv.sizes());
+  const auto [cu, slopes] =
+      attention_args("document_attention_qkv", qkv, qkv.size(2), qkv.size(2),
+                     cu_in, slopes_in, scale);
   if (wants_grad({qkv})) return DocAttentionQKV::apply(qkv, cu, slopes, scale);
   at::AutoDispatchBelowADInplaceOrView below;
   return std::get<0>(doc_attn_fwd_impl(qkv.select(1, 0), qkv.select(1, 1),

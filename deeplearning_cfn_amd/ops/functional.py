@@ -752,6 +752,9 @@ def document_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     Fused CDNA4 kernels for bf16 and fp16 with dim a multiple of 8 up to 128;
     anything else runs document by document in torch, in fp32.
     """
+    if q.dim() == 3 and _doc_attention_native(q):
+        scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+        return native().doc_attention(q, k, v, cu_seqlens, slopes, scale)
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or \
             k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
         raise ValueError(
@@ -763,8 +766,6 @@ def document_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     cu, scale, slopes = _doc_attention_args(
         "document_attention", q, q.shape[1], k.shape[1], cu_seqlens, scale,
         slopes)
-    if _doc_attention_native(q):
-        return native().doc_attention(q, k, v, cu, slopes, scale)
     return _doc_attention_composed(q, k, v, cu, scale, slopes)
 
 
@@ -785,14 +786,15 @@ def document_attention_qkv(qkv: torch.Tensor, cu_seqlens: torch.Tensor,
                            ) -> torch.Tensor:
     """``document_attention`` of one projection's output [tokens, 3, heads,
     dim]; its gradient comes in the same layout."""
+    if qkv.dim() == 4 and _doc_attention_native(qkv):
+        scale = qkv.shape[-1] ** -0.5 if scale is None else float(scale)
+        return native().doc_attention_qkv(qkv, cu_seqlens, slopes, scale)
     if qkv.dim() != 4 or qkv.shape[1] != 3:
         raise ValueError("document_attention_qkv: [tokens, 3, heads, dim] "
                          f"expected, got {tuple(qkv.shape)}")
     heads = qkv.shape[2]
     cu, scale, slopes = _doc_attention_args(
         "document_attention_qkv", qkv, heads, heads, cu_seqlens, scale, slopes)
-    if _doc_attention_native(qkv):
-        return native().doc_attention_qkv(qkv, cu, slopes, scale)
     return _doc_attention_composed(*qkv.unbind(1), cu, scale, slopes)
 
 
@@ -811,7 +813,7 @@ def newton_schulz(g: torch.Tensor, steps: int = 5,
 
     ``g`` is fp32, bf16 or fp16.  Matrices of a batch share their launches.
     The products take fp16 operands with fp32 sums; X itself is carried in 15
-    bits.  A zero matrix stays zero.  Gives no gradient.
+    bits (up to 64 rows: all operands in 22).  A zero matrix stays zero.  Gives no gradient.
     """
     if g.dim() < 2 or not g.is_floating_point():
         raise ValueError("newton_schulz: a floating [..., rows, cols] "

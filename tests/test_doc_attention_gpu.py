@@ -516,3 +516,37 @@ def test_single_tokens_have_no_gradient_of_scores(heads, kv, dim):
     want = do.double().unflatten(1, (kv, group)).sum(2)
     assert ((dv.double() - want).abs()
             <= want.abs() * 2.0 ** -8 + 2.0 ** -20 * group).all()
+
+
+def test_refusals_on_the_device():
+    """The same errors as on the CPU."""
+    F_amd = _f()
+    q, k, v, _ = _inputs(10, 4, 2, 64, torch.bfloat16)
+    cu = torch.tensor([0, 10], dtype=torch.int32, device="cuda")
+    s = _slopes(4)
+    for args, kw in (
+            ((q, k[:5], v, cu), {}), ((q, k, v[..., :32], cu), {}),
+            ((q, k.half(), v, cu), {}), ((q, k, v, cu.float()), {}),
+            ((q, k, v, cu[None]), {}), ((q, k, v, cu[:0]), {}),
+            ((q, k, v, cu.cpu()), {}), ((q[:, :3], k, v, cu), {}),
+            ((q, k, v, cu), {"scale": 0.0}),
+            ((q, k, v, cu), {"scale": float("nan")}),
+            ((q, k, v, cu), {"slopes": s[:3]}),
+            ((q, k, v, cu), {"slopes": s.cpu()}),
+            ((q, k, v, cu), {"slopes": s.clone().requires_grad_(True)})):
+        with pytest.raises(ValueError, match="document_attention"):
+            F_amd.document_attention(*args, **kw)
+    with pytest.raises(ValueError, match="document_attention_qkv"):
+        F_amd.document_attention_qkv(torch.stack([q, q], 1), cu)
+
+
+def test_borders_and_slopes_of_other_types():
+    F_amd = _f()
+    q, k, v, _ = _inputs(30, 4, 2, 64, torch.bfloat16)
+    ends = [0, 7, 30]
+    cu = torch.tensor(ends, dtype=torch.int32, device="cuda")
+    s = _slopes(4)
+    want = F_amd.document_attention(q, k, v, cu, slopes=s)
+    wide = torch.tensor([[0, 1], [7, 1], [2 ** 40, 1]], device="cuda")[:, 0]
+    got = F_amd.document_attention(q, k, v, wide, slopes=s.double())
+    assert torch.equal(got, want)
