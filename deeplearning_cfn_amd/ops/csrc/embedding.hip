@@ -307,10 +307,11 @@ DLX_DEV int2 token_at(const GradTable& t, int i, int end, int me, int& less) {
 
 // A bucket's tokens by id / G.  DIRECT: few tokens; every block looks at all
 // of them, and those of lower buckets, counted on the way, are the place where
-// its own begin, which saves the launches that make the buckets (three tables, 4096 tokens of
-// 768: 37 us for a whole gradient, 41 with buckets).
-// Bound by the same chain: 16384 tokens in three tables 11.8 us, 65536 in one
-// 15.5 us; two tables of 3001 tokens, without buckets, 10 us.
+// its own begin, which saves the launches that make the buckets (three tables,
+// 4096 tokens of 768: 37 us for a whole gradient, 41 with buckets).
+// Bound by its chain of reads, counts, a scan and a second walk: 16384 tokens
+// in three tables 12 us, 65536 in one 15.5 us; two tables of 3001 tokens,
+// without buckets, 10 us.
 // LDS: counts [wave][own], then scratch.
 template <bool DIRECT>
 __global__ __launch_bounds__(kSortThreads) void embed_order_kernel(GradArgs a,
