@@ -692,8 +692,12 @@ bool loadable(const at::Tensor& t) {
          reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
 }
 
+// A contiguous tensor that begins off a 16-byte border (cut out of a flat
+// buffer) is its own contiguous(): only a copy has a place that fits.
 at::Tensor rows(const at::Tensor& t) {
-  return loadable(t) ? t : t.contiguous();
+  if (loadable(t)) return t;
+  const auto c = t.contiguous();
+  return loadable(c) ? c : c.clone(at::MemoryFormat::Contiguous);
 }
 
 View view(const at::Tensor& t) {
@@ -850,6 +854,7 @@ void doc_attn_bwd_impl(const at::Tensor& dout_in, const at::Tensor& q_in,
                   && loadable(o) && lse.numel() == q_in.size(0) * q_in.size(1)
                   && lse.scalar_type() == at::kFloat && lse.is_contiguous() &&
                   low.sizes() == o.sizes() && low.is_contiguous() &&
+                  reinterpret_cast<uintptr_t>(low.data_ptr()) % 16 == 0 &&
                   low.scalar_type() == o.scalar_type() &&
                   o.device() == q_in.device() &&
                   lse.device() == q_in.device() &&
