@@ -13,6 +13,10 @@ all_reduce and replays it) — but the multi-GPU default stays eager
 (``DLX_GRAPHS=1`` to force) until an 8-GPU box can validate multi-rank
 capture; at the bench's batch sizes the step is not launch-bound, so
 eager costs little there.
+
+What a step takes from host numbers (an optimizer's lr, betas, weight decay)
+stays what it was at capture; what it counts (Adam's steps) lives on the
+device and goes on with every replay.
 """
 
 from __future__ import annotations

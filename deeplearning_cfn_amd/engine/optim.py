@@ -126,7 +126,55 @@ class FlatSGD(_FlatOptimBase):
         self.nesterov = sd["nesterov"]
 
 
-class FlatAdam(_FlatOptimBase):
+class _FlatAdamBase(_FlatOptimBase):
+    """Counts steps on the parameters' device, so that a captured step that
+    is replayed counts (and corrects its moments' bias) like an eager one."""
+
+    def __init__(self, engine: DataParallel):
+        super().__init__(engine)
+        device = self.flat_params[0].device if self.flat_params else "cpu"
+        self._steps = torch.zeros((), dtype=torch.int64, device=device)
+        # 1 / (1 - beta ** t) of both betas
+        self._inverse = torch.ones(2, dtype=torch.float32, device=device)
+
+    @property
+    def t(self) -> int:
+        """Steps taken (on the GPU: waits for them)."""
+        return int(self._steps)
+
+    @t.setter
+    def t(self, value: int) -> None:
+        self._steps.fill_(int(value))
+
+    def _count(self) -> Tuple[float, float]:
+        """One step more; the corrections where the torch form asks."""
+        b1, b2 = self.betas
+        if self._steps.is_cuda and native_available():
+            native().adam_count(self._steps, self._inverse, b1, b2)
+            return 1.0, 1.0               # not read: _inverse is
+        self._steps.add_(1)
+        t = self.t
+        return 1 - b1 ** t, 1 - b2 ** t
+
+    def _adamw(self, fp, g, m, v, master, lr, bc1, bc2) -> None:
+        b1, b2 = self.betas
+        if fp.is_cuda and native_available():
+            native().adamw_flat_counted(fp, g, m, v, master, lr, b1, b2,
+                                        self.eps, self.weight_decay,
+                                        self._inverse)
+            return
+        g32 = g.float()
+        m.mul_(b1).add_(g32, alpha=1 - b1)
+        v.mul_(b2).addcmul_(g32, g32, value=1 - b2)
+        p32 = master if master is not None else fp.float()
+        p32 = p32 - lr * self.weight_decay * p32
+        p32 = p32 - lr * (m / bc1) / ((v / bc2).sqrt() + self.eps)
+        if master is not None:
+            master.copy_(p32)
+        fp.copy_(p32.to(fp.dtype))
+
+
+class FlatAdam(_FlatAdamBase):
     """AdamW over flat buckets (BERT path; fused adamw_flat on HIP)."""
 
     def __init__(self, engine: DataParallel, lr: float = 1e-4,
@@ -135,38 +183,16 @@ class FlatAdam(_FlatOptimBase):
         super().__init__(engine)
         self.lr, self.betas, self.eps = lr, betas, eps
         self.weight_decay = weight_decay
-        self.t = 0
         self.m = [torch.zeros(fp.numel(), dtype=torch.float32,
                               device=fp.device) for fp in self.flat_params]
         self.v = [torch.zeros_like(mm) for mm in self.m]
 
     @torch.no_grad()
     def step(self) -> None:
-        self.t += 1
-        b1, b2 = self.betas
-        bc1 = 1 - b1 ** self.t
-        bc2 = 1 - b2 ** self.t
+        bc1, bc2 = self._count()
         for fp, b, m, v, master in zip(self.flat_params, self.buckets,
                                        self.m, self.v, self.masters):
-            g = b.flat
-            if fp.is_cuda and native_available():
-                if master is not None:
-                    native().adamw_flat_master(fp, g, m, v, master, self.lr,
-                                               b1, b2, self.eps,
-                                               self.weight_decay, bc1, bc2)
-                else:
-                    native().adamw_flat(fp, g, m, v, self.lr, b1, b2,
-                                        self.eps, self.weight_decay, bc1, bc2)
-                continue
-            g32 = g.float()
-            m.mul_(b1).add_(g32, alpha=1 - b1)
-            v.mul_(b2).addcmul_(g32, g32, value=1 - b2)
-            p32 = master if master is not None else fp.float()
-            p32 = p32 - self.lr * self.weight_decay * p32
-            p32 = p32 - self.lr * (m / bc1) / ((v / bc2).sqrt() + self.eps)
-            if master is not None:
-                master.copy_(p32)
-            fp.copy_(p32.to(fp.dtype))
+            self._adamw(fp, b.flat, m, v, master, self.lr, bc1, bc2)
 
     def state_dict(self) -> dict:
         return {"m": self.m, "v": self.v, "masters": self.masters,
@@ -188,7 +214,7 @@ class FlatAdam(_FlatOptimBase):
         self.weight_decay = sd.get("weight_decay", self.weight_decay)
 
 
-class FlatMuon(_FlatOptimBase):
+class FlatMuon(_FlatAdamBase):
     """Muon for hidden matrices, AdamW for the other parameters.
 
     A hidden matrix is the weight of an ``nn.Linear`` with at least 16 rows
@@ -213,7 +239,6 @@ class FlatMuon(_FlatOptimBase):
         self.ns_steps, self.ns_eps = ns_steps, ns_eps
         self.weight_decay = weight_decay
         self.adam_lr, self.betas, self.eps = adam_lr, betas, eps
-        self.t = 0
         hidden = {id(m.weight) for m in engine.module.modules()
                   if isinstance(m, torch.nn.Linear)
                   and min(m.weight.shape) >= self.MIN_SIDE}
@@ -284,34 +309,15 @@ class FlatMuon(_FlatOptimBase):
     def _step_rest(self, span, v: torch.Tensor, bc1: float,
                    bc2: float) -> None:
         bi, a, e = span
-        b1, b2 = self.betas
-        fp, g = self.flat_params[bi][a:e], self.buckets[bi].flat[a:e]
-        m = self.m[bi][a:e]
         master = self.masters[bi]
-        master = None if master is None else master[a:e]
-        if fp.is_cuda and native_available():
-            args = (self.adam_lr, b1, b2, self.eps, self.weight_decay, bc1,
-                    bc2)
-            if master is not None:
-                native().adamw_flat_master(fp, g, m, v, master, *args)
-            else:
-                native().adamw_flat(fp, g, m, v, *args)
-            return
-        g32 = g.float()
-        m.mul_(b1).add_(g32, alpha=1 - b1)
-        v.mul_(b2).addcmul_(g32, g32, value=1 - b2)
-        p32 = master if master is not None else fp.float()
-        p32 = p32 - self.adam_lr * self.weight_decay * p32
-        p32 = p32 - self.adam_lr * (m / bc1) / ((v / bc2).sqrt() + self.eps)
-        if master is not None:
-            master.copy_(p32)
-        fp.copy_(p32.to(fp.dtype))
+        self._adamw(self.flat_params[bi][a:e], self.buckets[bi].flat[a:e],
+                    self.m[bi][a:e], v,
+                    None if master is None else master[a:e], self.adam_lr,
+                    bc1, bc2)
 
     @torch.no_grad()
     def step(self) -> None:
-        self.t += 1
-        bc1 = 1 - self.betas[0] ** self.t
-        bc2 = 1 - self.betas[1] ** self.t
+        bc1, bc2 = self._count()
         for (rows, cols, _, _), spans in self.groups.items():
             self._step_matrices(rows, cols, spans)
         for span, v in zip(self.rest, self.v):

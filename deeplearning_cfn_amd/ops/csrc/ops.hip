@@ -23,7 +23,10 @@ void launch_sgd_flat(at::Tensor& p, const at::Tensor& g, at::Tensor& m,
 void launch_adamw_flat(at::Tensor& p, const at::Tensor& g, at::Tensor& m,
                        at::Tensor& v, const at::Tensor* master, double lr,
                        double b1, double b2, double eps, double wd,
-                       double bc1, double bc2, hipStream_t s);
+                       double bc1, double bc2, const float* inverse,
+                       hipStream_t s);
+void launch_adam_count(at::Tensor& steps, at::Tensor& inverse, double b1,
+                       double b2, hipStream_t s);
 
 // softmax_ce.hip
 std::tuple<at::Tensor, at::Tensor> softmax_ce_fwd_impl(
@@ -263,14 +266,38 @@ void adamw_flat(at::Tensor p, at::Tensor g, at::Tensor m, at::Tensor v,
                 double lr, double b1, double b2, double eps, double wd,
                 double bc1, double bc2) {
   launch_adamw_flat(p, g, m, v, nullptr, lr, b1, b2, eps, wd, bc1, bc2,
-                    cur_stream());
+                    nullptr, cur_stream());
 }
 
 void adamw_flat_master(at::Tensor p, at::Tensor g, at::Tensor m, at::Tensor v,
                        at::Tensor master, double lr, double b1, double b2,
                        double eps, double wd, double bc1, double bc2) {
   launch_adamw_flat(p, g, m, v, &master, lr, b1, b2, eps, wd, bc1, bc2,
-                    cur_stream());
+                    nullptr, cur_stream());
+}
+
+// steps: one number; inverse: two, what adamw_flat_counted multiplies by
+void adam_count(at::Tensor steps, at::Tensor inverse, double b1, double b2) {
+  TORCH_CHECK(steps.scalar_type() == at::kLong && steps.numel() == 1 &&
+                  inverse.scalar_type() == at::kFloat &&
+                  inverse.numel() == 2 && inverse.is_contiguous() &&
+                  inverse.device() == steps.device(),
+              "adam_count: steps is one int64, inverse two float32");
+  const c10::DeviceGuard guard(steps.device());
+  launch_adam_count(steps, inverse, b1, b2, cur_stream());
+}
+
+// adamw_flat (master: adamw_flat_master) with adam_count's corrections
+void adamw_flat_counted(at::Tensor p, at::Tensor g, at::Tensor m, at::Tensor v,
+                        const c10::optional<at::Tensor>& master, double lr,
+                        double b1, double b2, double eps, double wd,
+                        const at::Tensor& inverse) {
+  TORCH_CHECK(inverse.scalar_type() == at::kFloat && inverse.numel() == 2 &&
+                  inverse.is_contiguous() && inverse.device() == p.device(),
+              "adamw: inverse is two float32");
+  const c10::DeviceGuard guard(p.device());
+  launch_adamw_flat(p, g, m, v, master ? &*master : nullptr, lr, b1, b2, eps,
+                    wd, 1.0, 1.0, inverse.data_ptr<float>(), cur_stream());
 }
 
 std::tuple<at::Tensor, at::Tensor> softmax_ce_fwd(const at::Tensor& logits,
@@ -311,6 +338,8 @@ TORCH_LIBRARY(dlx_hip, m) {
   m.def("sgd_momentum_flat_master(Tensor(a!) p, Tensor g, Tensor(b!) m, Tensor(c!) master, float lr, float momentum, float wd, bool nesterov) -> ()");
   m.def("adamw_flat(Tensor(a!) p, Tensor g, Tensor(b!) m, Tensor(c!) v, float lr, float b1, float b2, float eps, float wd, float bc1, float bc2) -> ()");
   m.def("adamw_flat_master(Tensor(a!) p, Tensor g, Tensor(b!) m, Tensor(c!) v, Tensor(d!) master, float lr, float b1, float b2, float eps, float wd, float bc1, float bc2) -> ()");
+  m.def("adam_count(Tensor(a!) steps, Tensor(b!) inverse, float b1, float b2) -> ()");
+  m.def("adamw_flat_counted(Tensor(a!) p, Tensor g, Tensor(b!) m, Tensor(c!) v, Tensor(d!)? master, float lr, float b1, float b2, float eps, float wd, Tensor inverse) -> ()");
   m.def("softmax_ce_fwd(Tensor logits, Tensor target) -> (Tensor, Tensor)");
   m.def("softmax_ce_bwd(Tensor probs, Tensor target, Tensor grad, bool out_bf16) -> Tensor");
   m.def("bn_fwd_train(Tensor x, Tensor w, Tensor b, Tensor(a!) rmean, Tensor(b!) rvar, float momentum, float eps, bool relu) -> (Tensor, Tensor, Tensor, Tensor)");
@@ -364,6 +393,8 @@ TORCH_LIBRARY_IMPL(dlx_hip, CUDA, m) {
   m.impl("sgd_momentum_flat_master", dlx::sgd_momentum_flat_master);
   m.impl("adamw_flat", dlx::adamw_flat);
   m.impl("adamw_flat_master", dlx::adamw_flat_master);
+  m.impl("adam_count", dlx::adam_count);
+  m.impl("adamw_flat_counted", dlx::adamw_flat_counted);
   m.impl("softmax_ce_fwd", dlx::softmax_ce_fwd);
   m.impl("softmax_ce_bwd", dlx::softmax_ce_bwd);
   m.impl("bn_fwd_train", dlx::bn_fwd_train_impl);

@@ -84,7 +84,12 @@ __global__ void adamw_kernel(T* __restrict__ p, const T* __restrict__ g,
                              float* __restrict__ m, float* __restrict__ v,
                              float* __restrict__ master, long n, float lr,
                              float b1, float b2, float eps, float wd,
-                             float inv_bc1, float inv_bc2) {
+                             float inv_bc1, float inv_bc2,
+                             const float* __restrict__ inverse) {
+  if (inverse) {              // counted on the device (adam_count_kernel)
+    inv_bc1 = inverse[0];
+    inv_bc2 = inverse[1];
+  }
   const long stride = (long)gridDim.x * blockDim.x;
   const long nvec = n / kW;
   for (long i = blockIdx.x * (long)blockDim.x + threadIdx.x; i < nvec;
@@ -163,7 +168,8 @@ template <typename T>
 static void adamw_launch_t(at::Tensor& p, const at::Tensor& g, at::Tensor& m,
                            at::Tensor& v, const at::Tensor* master, double lr,
                            double b1, double b2, double eps, double wd,
-                           double bc1, double bc2, hipStream_t s) {
+                           double bc1, double bc2, const float* inverse,
+                           hipStream_t s) {
   long n = p.numel();
   int grid = grid_for(n / kW + 1);
   T* pp = reinterpret_cast<T*>(p.data_ptr());
@@ -174,24 +180,46 @@ static void adamw_launch_t(at::Tensor& p, const at::Tensor& g, at::Tensor& m,
   float ib1 = 1.0 / bc1, ib2 = 1.0 / bc2;
   if (master)
     adamw_kernel<T, true><<<grid, kBlock, 0, s>>>(pp, gp, mp, vp, ms, n, lr,
-                                                  b1, b2, eps, wd, ib1, ib2);
+                                                  b1, b2, eps, wd, ib1, ib2,
+                                                  inverse);
   else
     adamw_kernel<T, false><<<grid, kBlock, 0, s>>>(pp, gp, mp, vp, ms, n, lr,
-                                                   b1, b2, eps, wd, ib1, ib2);
+                                                   b1, b2, eps, wd, ib1, ib2,
+                                                   inverse);
 }
 
 void launch_adamw_flat(at::Tensor& p, const at::Tensor& g, at::Tensor& m,
                        at::Tensor& v, const at::Tensor* master, double lr,
                        double b1, double b2, double eps, double wd,
-                       double bc1, double bc2, hipStream_t s) {
+                       double bc1, double bc2, const float* inverse,
+                       hipStream_t s) {
   TORCH_CHECK(m.scalar_type() == at::kFloat && v.scalar_type() == at::kFloat,
               "adamw: m/v must be fp32");
   if (p.scalar_type() == at::kBFloat16)
-    adamw_launch_t<uint16_t>(p, g, m, v, master, lr, b1, b2, eps, wd, bc1, bc2, s);
+    adamw_launch_t<uint16_t>(p, g, m, v, master, lr, b1, b2, eps, wd, bc1, bc2,
+                             inverse, s);
   else if (p.scalar_type() == at::kFloat)
-    adamw_launch_t<float>(p, g, m, v, master, lr, b1, b2, eps, wd, bc1, bc2, s);
+    adamw_launch_t<float>(p, g, m, v, master, lr, b1, b2, eps, wd, bc1, bc2,
+                          inverse, s);
   else
     TORCH_CHECK(false, "adamw: unsupported dtype ", p.scalar_type());
+}
+
+// One step more, and what the moments' bias corrections multiply by after it:
+// 1 / (1 - b ** steps), in 64 bits.  On the device, so that a captured step
+// counts its replays; one thread, 3 us a step (a launch).
+__global__ void adam_count_kernel(long* steps, float* inverse, double b1,
+                                  double b2) {
+  const long t = *steps + 1;
+  *steps = t;
+  inverse[0] = (float)(1.0 / (1.0 - pow(b1, (double)t)));
+  inverse[1] = (float)(1.0 / (1.0 - pow(b2, (double)t)));
+}
+
+void launch_adam_count(at::Tensor& steps, at::Tensor& inverse, double b1,
+                       double b2, hipStream_t s) {
+  adam_count_kernel<<<1, 1, 0, s>>>(steps.data_ptr<int64_t>(),
+                                    inverse.data_ptr<float>(), b1, b2);
 }
 
 }  // namespace dlx
