@@ -7,7 +7,7 @@
 // C++ about 20.
 //
 // The gradients have no gradient of their own: asking for a graph of them
-// (create_graph) raises.  Saved inputs are checked for changes in place.
+// (create_graph) raises, and so does an input with a forward-mode tangent.  Saved inputs are checked for changes in place.
 #include <torch/extension.h>
 #include <limits>
 #include <torch/csrc/autograd/custom_function.h>
@@ -46,6 +46,12 @@ void refuse_graph(const char* name) {
               ": its gradient has no gradient (create_graph)");
 }
 
+// A tangent that no formula here takes on would be lost without a word.
+void refuse_tangent(const char* name, const at::Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(/*level=*/0).defined(), name,
+                              ": no forward-mode gradient");
+}
+
 // What functional.embedding_sum checks elsewhere, for 4 us less of host time
 void check_lookup(at::TensorList ids, at::TensorList tables,
                   at::ArrayRef<double> scales) {
@@ -67,6 +73,7 @@ void check_lookup(at::TensorList ids, at::TensorList tables,
                       "and type");
     TORCH_CHECK_VALUE(i.device() == w0.device() && w.device() == w0.device(),
                       "embedding_sum: ids and tables are on different devices");
+    refuse_tangent("embedding_sum", w);
   }
 }
 
@@ -96,6 +103,7 @@ std::pair<at::Tensor, c10::optional<at::Tensor>> attention_args(
                           slopes->device() == q.device(),
                       name, ": slopes has one number a query head, on the same "
                       "device");
+    refuse_tangent(name, *slopes);
     s = slopes->to(at::kFloat).contiguous();
   }
   if (cu.scalar_type() == at::kInt && cu.is_contiguous()) return {cu, s};
@@ -256,6 +264,7 @@ at::Tensor doc_attention(const at::Tensor& q, const at::Tensor& k,
   const auto [cu, slopes] =
       attention_args("document_attention", q, q.size(1), k.size(1), cu_in,
                      slopes_in, scale);
+  for (const auto* t : {&q, &k, &v}) refuse_tangent("document_attention", *t);
   if (wants_grad({q, k, v}))
     return DocAttention::apply(q, k, v, cu, slopes, scale);
   at::AutoDispatchBelowADInplaceOrView below;
@@ -271,6 +280,7 @@ at::Tensor doc_attention_qkv(const at::Tensor& qkv, const at::Tensor& cu_in,
   const auto [cu, slopes] =
       attention_args("document_attention_qkv", qkv, qkv.size(2), qkv.size(2),
                      cu_in, slopes_in, scale);
+  refuse_tangent("document_attention_qkv", qkv);
   if (wants_grad({qkv})) return DocAttentionQKV::apply(qkv, cu, slopes, scale);
   at::AutoDispatchBelowADInplaceOrView below;
   return std::get<0>(doc_attn_fwd_impl(qkv.select(1, 0), qkv.select(1, 1),
