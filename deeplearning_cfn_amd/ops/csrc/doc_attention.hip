@@ -349,7 +349,7 @@ __global__ __launch_bounds__(NW * 64, DP == 64 ? 4 : 2) void doc_attn_fwd_kernel
       if (t + 1 < nt) body(t + 1, std::integral_constant<int, 1>{}, fine);
     }
   };
-  if (NW == 4 && tl.len <= a.fine) walk(std::true_type{});
+  if (tl.len <= a.fine) walk(std::true_type{});
   else walk(std::false_type{});
   l += __shfl_xor(l, 32, kWave);
   if (!real) return;
@@ -478,7 +478,7 @@ __global__ __launch_bounds__(NW * 64, DP == 64 ? 3 : 2) void doc_attn_dq_kernel(
       if (t + 1 < nt) body(t + 1, std::integral_constant<int, 1>{}, fine);
     }
   };
-  if (NW == 4 && tl.len <= a.fine) walk(std::true_type{});
+  if (tl.len <= a.fine) walk(std::true_type{});
   else walk(std::false_type{});
   if (real)             // of one score p is 1: nothing depends on q or k
     store_rows<T, DP>(a.dq.p + token * a.dq.token + head * a.dq.head, acc,
@@ -619,7 +619,7 @@ __global__ __launch_bounds__(NW * 64, DP == 64 ? 3 : 2) void doc_attn_dkv_kernel
     if (n + 1 < n1) stage(n + 1, lds + (1 - H) * 2 * TS, stat[1 - H]);
     if (!mine) return;
     turn(n, half_, std::false_type{});
-    if (NW == 4 && tl.len <= a.fine) turn(n, half_, std::true_type{});
+    if (tl.len <= a.fine) turn(n, half_, std::true_type{});
   };
   for (int n = n0; n < n1; n += 2) {
     body(n, std::integral_constant<int, 0>{});
