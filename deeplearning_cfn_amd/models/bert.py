@@ -147,7 +147,13 @@ class BertForPretraining(nn.Module):
                          cu_seqlens: torch.Tensor,
                          token_type: torch.Tensor | None = None
                          ) -> torch.Tensor:
-        """Packed documents: [*input_ids.shape, hidden]."""
+        """Packed documents: [*input_ids.shape, hidden].
+
+        With a table of positions a document has at most ``max_seq`` tokens:
+        the positions behind that are outside the table, which raises on the
+        CPU and gives NaN for that document on the GPU (where the lengths are
+        not known on the host).
+        """
         from ..ops import functional as F_amd
         ids = input_ids.reshape(-1)
         cu = cu_seqlens.to(torch.int32)
@@ -159,8 +165,7 @@ class BertForPretraining(nn.Module):
             slopes = self.slope_bits.view(torch.float32)
         else:
             tables.append(self.pos.weight)
-            index.append(F_amd.document_positions(cu, ids.numel())
-                         .clamp_(max=self.cfg.max_seq - 1))
+            index.append(F_amd.document_positions(cu, ids.numel()))
         x = self.ln(F_amd.embedding_sum(index, tables))
         for blk in self.blocks:
             x = blk(x, cu, slopes)
