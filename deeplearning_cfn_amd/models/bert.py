@@ -156,7 +156,8 @@ class BertForPretraining(nn.Module):
         """
         from ..ops import functional as F_amd
         ids = input_ids.reshape(-1)
-        cu = cu_seqlens.to(torch.int32)
+        # once, not in every layer; cut off at the tokens before it is narrowed
+        cu = cu_seqlens.clamp(0, ids.numel()).to(torch.int32)
         typ = (token_type.reshape(-1) if token_type is not None
                else torch.zeros_like(ids))
         tables, index = [self.tok.weight, self.typ.weight], [ids, typ]

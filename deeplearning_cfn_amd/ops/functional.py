@@ -743,8 +743,8 @@ def document_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     ``q`` [tokens, heads, dim], ``k`` and ``v`` [tokens, kv_heads, dim] (heads
     a multiple of kv_heads; neighbouring query heads share one).
     ``cu_seqlens`` [documents + 1]: document i is the tokens from
-    ``cu_seqlens[i]`` to ``cu_seqlens[i + 1]``, in rising order; empty ones
-    are allowed.  Tokens in no document get zeros, and zero gradients.
+    ``cu_seqlens[i]`` to ``cu_seqlens[i + 1]``, in rising order (borders
+    outside the tokens are cut off at them); empty ones are allowed.  Tokens in no document get zeros, and zero gradients.
     ``scale`` (default dim ** -0.5) lies between 1e-30 and
     1e30.  ``slopes`` [heads] takes
     ``slopes[h] * |i - j|`` off the scores; it gets no gradient.
@@ -770,9 +770,10 @@ def document_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 
 
 def document_positions(cu_seqlens: torch.Tensor, tokens: int) -> torch.Tensor:
-    """Each token's place in its document (0 for tokens in none): int64."""
+    """Each token's place in its document (0 for tokens in none): int64.
+    Borders outside the tokens are cut off at them, as attention does."""
     at = torch.arange(tokens, device=cu_seqlens.device)
-    cu = cu_seqlens.long()
+    cu = cu_seqlens.long().clamp(0, tokens)
     # the last border that is not behind the token
     doc = torch.searchsorted(cu, at, right=True) - 1
     start = cu[doc.clamp(0, cu.numel() - 1)]

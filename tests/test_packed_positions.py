@@ -49,3 +49,19 @@ def test_document_longer_than_the_table_is_nan():
             [0, 16, 32, 40], dtype=torch.int32, device="cuda")).reshape(40, -1)
         assert fits.isfinite().all() and torch.equal(fits[:16], x[:16])
         assert model(ids, ids, cu_seqlens=cu).isnan()
+
+
+def test_borders_outside_the_tokens():
+    """They are cut off at the tokens: positions, and the whole model."""
+    from deeplearning_cfn_amd.ops import functional as F_amd
+    want = [0, 1, 2, 3, 0, 1, 2, 3, 4, 5]
+    for ends in ([0, 4, 10], [-3, 4, 12], [-2 ** 40, 4, 2 ** 40],
+                 [-1, 0, 4, 10, 10, 11]):
+        assert F_amd.document_positions(torch.tensor(ends), 10).tolist() \
+            == want
+    for alibi in (False, True):
+        model, ids = _model(alibi), _ids(1, 10)
+        x = model.encode(ids, cu_seqlens=torch.tensor([0, 4, 10]))
+        for ends in ([-3, 4, 12], [-2 ** 32 - 6, 4, 2 ** 32 + 5]):
+            assert torch.equal(
+                model.encode(ids, cu_seqlens=torch.tensor(ends)), x)
