@@ -126,6 +126,18 @@ DLX_DEV double ns_sum(const double* part, int parts, double* red) {
   return red[0] + red[1] + red[2] + red[3];
 }
 
+// What X_0 is of G: times 2^e first, then times f, so that neither leaves fp32
+// (a norm of 1e-37 asks for 4e40).  Nothing but zeros has norm and eps of 0.
+struct NsScale {
+  float f;
+  int e;
+  DLX_DEV NsScale(double sum, double eps) {
+    const double norm = sqrt(sum) + eps;
+    f = (float)frexp(norm == 0.0 ? 0.0 : (double)kXScale / norm, &e);
+  }
+  DLX_DEV float of(float x) const { return ldexpf(x, e) * f; }
+};
+
 // G to X_0: scaled, split in two, padded with zeros, a tall one transposed.
 // A block writes a 64 x 64 tile of X.  WIDE: low parts of 16 bits.  Bound by
 // memory: the same 24, 403 MB read and 302 written in 123 us (5.7 TB/s).
@@ -133,12 +145,12 @@ template <typename T, int V, bool WIDE>
 __global__ __launch_bounds__(256) void ns_split_kernel(
     const T* __restrict__ g, const double* __restrict__ part, int parts,
     uint16_t* __restrict__ xh, void* __restrict__ xl, int rows, int cols,
-    bool tall, int np, int mp, float eps) {
+    bool tall, int np, int mp, double eps) {
   __shared__ float t[64][65];
   __shared__ double red[4];
   const int b = blockIdx.z;
   const double sum = ns_sum(part + (long)b * parts, parts, red);
-  const float by = (float)(kXScale / (sqrt(sum) + (double)eps));
+  const NsScale by(sum, eps);
   const int i0 = blockIdx.y * 64, j0 = blockIdx.x * 64;   // in X
   const int r0 = tall ? j0 : i0, c0 = tall ? i0 : j0;     // in G
   const T* gb = g + (long)b * rows * cols;
@@ -150,7 +162,7 @@ __global__ __launch_bounds__(256) void ns_split_kernel(
     if (r0 + r < rows && c0 + x < cols)
       load_vec<T, V>(gb + (long)(r0 + r) * cols + c0 + x, v);
 #pragma unroll
-    for (int e = 0; e < V; ++e) t[r][x + e] = v[e] * by;
+    for (int e = 0; e < V; ++e) t[r][x + e] = by.of(v[e]);
   }
   __syncthreads();
   const int xj = (threadIdx.x & 15) * 4;
@@ -514,7 +526,7 @@ ns_update_kernel(NsUpdate a) {
 template <typename T, int NP, int MP, int WAVES>
 __global__ __launch_bounds__(WAVES* kWave) void ns_small_kernel(
     const T* __restrict__ g, uint16_t* __restrict__ out, int rows, int cols,
-    int steps, float eps) {
+    int steps, double eps) {
   constexpr int TI = NP / 32, TJ = MP / 32;
   constexpr int MINE = (TI * TJ + WAVES - 1) / WAVES;
   constexpr int SQ = (TI * TI + WAVES - 1) / WAVES;
@@ -556,11 +568,11 @@ __global__ __launch_bounds__(WAVES* kWave) void ns_small_kernel(
   __syncthreads();
   sum = 0;
   for (int i = 0; i < WAVES; ++i) sum += red[i];
-  const float by = (float)(kXScale / (sqrt(sum) + (double)eps));
+  const NsScale by(sum, eps);
 #pragma unroll
   for (int u = 0; u < MINE; ++u)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) x[u][r] *= by;
+    for (int r = 0; r < 16; ++r) x[u][r] = by.of(x[u][r]);
 
   auto put = [&](uint16_t* tile, auto dp, auto low, int row, int col,
                  const float* v) {
@@ -704,7 +716,7 @@ __global__ __launch_bounds__(WAVES* kWave) void ns_small_kernel(
 
 template <typename T>
 void launch_small(const at::Tensor& g, at::Tensor& out, int batch, int rows,
-                  int cols, int steps, float eps, hipStream_t s) {
+                  int cols, int steps, double eps, hipStream_t s) {
   const int n = std::min(rows, cols), m = std::max(rows, cols);
   auto go = [&](auto kernel, int waves) {
     kernel<<<batch, waves * kWave, 0, s>>>(
@@ -722,7 +734,7 @@ void launch_small(const at::Tensor& g, at::Tensor& out, int batch, int rows,
 template <typename T, int V>
 void launch_start(const at::Tensor& g, double* part, int parts, uint16_t* xh,
                   void* xl, bool wide, int batch, int rows, int cols, int np, int mp,
-                  float eps, hipStream_t s) {
+                  double eps, hipStream_t s) {
   const T* p = static_cast<const T*>(g.data_ptr());
   ns_norm_kernel<T, V><<<dim3(parts, batch), 256, 0, s>>>(p, part,
                                                           (long)rows * cols);
@@ -930,7 +942,7 @@ at::Tensor newton_schulz_impl(const at::Tensor& g_in, int64_t steps,
   if (std::min(rows, cols) <= 128 && std::max(rows, cols) <= 256) {
     auto small = [&](auto tag) {
       launch_small<decltype(tag)>(g, out, (int)batch, (int)rows, (int)cols,
-                                  (int)steps, (float)eps, s);
+                                  (int)steps, eps, s);
     };
     switch (g.scalar_type()) {
       case at::kFloat: small(float{}); break;
@@ -965,7 +977,7 @@ at::Tensor newton_schulz_impl(const at::Tensor& g_in, int64_t steps,
     (v4 ? launch_start<T, 4> : launch_start<T, 1>)(
         g, part.data_ptr<double>(), (int)parts, px,
         wide || steps > 2 ? low.data_ptr() : nullptr, wide, (int)batch,
-        (int)rows, (int)cols, (int)np, (int)mp, (float)eps, s);
+        (int)rows, (int)cols, (int)np, (int)mp, eps, s);
   };
   switch (g.scalar_type()) {
     case at::kFloat: start(float{}); break;

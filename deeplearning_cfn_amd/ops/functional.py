@@ -833,7 +833,7 @@ def newton_schulz(g: torch.Tensor, steps: int = 5,
     tall = x.shape[1] > x.shape[2]
     x = (x.transpose(1, 2) if tall else x).float().contiguous()
     norm = x.double().square().sum((1, 2), keepdim=True).sqrt() + eps
-    x = (x / norm).float()
+    x = torch.where(norm == 0, 0.0, x / norm).float()
     for _ in range(steps):
         s = x @ x.transpose(1, 2).contiguous()
         x = a * x + (b * s + c * (s @ s)) @ x
