@@ -9,16 +9,19 @@
 //
 // Precision.  The products take fp16 operands (11 bits; bf16's 8 would leave
 // an error of 1e-2) and add in fp32.  Small singular values grow about 3.4
-// times a step, and what X loses to rounding grows with them, so X is kept as
-// an fp16 number and an fp8 one (e4m3) for what that leaves, 15 bits: the
-// products take the first, the term a X both, the first by way of a's place
-// on B's diagonal.  The last two X that are multiplied are fp16 alone,
-// for what they lose has no time to grow.  B X's rounding lies in the
-// directions where B is large, which are those that no longer grow.  Against
-// 64 bits that leaves 7e-4 to 2.9e-3 relative (CPU model of these roundings,
-// four spectra, sizes 64 to 1024), next to bf16's own 1.7e-3 in the result.
+// times a step, and so does what X loses to rounding in directions without
+// signal, so X_0 is two fp16 numbers, 22 bits, and the next ones an fp16 and an
+// fp8 one (e4m3) for what that leaves, 15: the products take the first, the
+// term a X both.  The last X that is multiplied is fp16 alone, for what it
+// loses has no time to grow.  a X takes the fp16 number exactly, by a product
+// of its own (ns_update_kernel): on B's diagonal a's rounding, 2^-10, is one of
+// every row, and in a matrix of few directions nothing evens that out.  Off by
+// so many times what rounding the result costs, for rank 1 / 4 / 64 / full:
+// 768 x 2304 1.32 / 1.28 / 1.21 / 1.31, 300 x 300 1.30 / 1.27 / 1.21 / 1.35
+// (X_0 in 15 bits, the last two X in 11 and a on the diagonal: 3.31 / 2.35 /
+// 2.01 / 1.20, for 4 % less time).
 // With up to 64 rows, where few directions share a step's rounding, X, A and
-// B are two fp16 numbers each: 1.7e-3, the rounding of the result.
+// B are two fp16 numbers each: 1.00, the rounding of the result.
 // X is stored times 2^12: its entries stay under 2 and its small ones clear
 // of fp16's subnormals.
 #include <torch/extension.h>
@@ -37,6 +40,7 @@ constexpr int kTile = 128;            // the smaller output tile
 constexpr int kDepth = 64;            // of a stage along k
 constexpr float kXScale = 4096.f;
 constexpr float kNsA = 3.4445f, kNsB = -4.7750f, kNsC = 2.0315f;
+constexpr float kNsDiag = 3.4453125f;   // a, rounded to fp16
 constexpr int kNormChunk = 1 << 14;   // elements of a partial norm
 
 // k within 16 as operand B wants it next to Frags::tr: quads 0, 2, 1, 3
@@ -138,13 +142,14 @@ struct NsScale {
   DLX_DEV float of(float x) const { return ldexpf(x, e) * f; }
 };
 
-// G to X_0: scaled, split in two, padded with zeros, a tall one transposed.
-// A block writes a 64 x 64 tile of X.  WIDE: low parts of 16 bits.  Bound by
-// memory: the same 24, 403 MB read and 302 written in 123 us (5.7 TB/s).
-template <typename T, int V, bool WIDE>
+// G to X_0: scaled, split in two fp16 numbers, padded with zeros, a tall one
+// transposed.  A block writes a 64 x 64 tile of X.  Bound by memory: the same
+// 24, 403 MB read and 403 written in 135 us
+// (6.0 TB/s).
+template <typename T, int V>
 __global__ __launch_bounds__(256) void ns_split_kernel(
     const T* __restrict__ g, const double* __restrict__ part, int parts,
-    uint16_t* __restrict__ xh, void* __restrict__ xl, int rows, int cols,
+    uint16_t* __restrict__ xh, uint16_t* __restrict__ xl, int rows, int cols,
     bool tall, int np, int mp, double eps) {
   __shared__ float t[64][65];
   __shared__ double red[4];
@@ -177,12 +182,7 @@ __global__ __launch_bounds__(256) void ns_split_kernel(
       h.v[e] = from_f32<FP16>(v[e]).v;
     }
     *reinterpret_cast<Pack<uint16_t, 4>*>(xh + o) = h;
-    if (WIDE)
-      *reinterpret_cast<Pack<uint16_t, 4>*>(static_cast<uint16_t*>(xl) + o) =
-          low_halves(v, h);
-    else if (xl)
-      *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(xl) + o) =
-          low_parts(v, h.v);
+    if (xl) *reinterpret_cast<Pack<uint16_t, 4>*>(xl + o) = low_halves(v, h);
   }
 }
 
@@ -195,7 +195,8 @@ template <> struct Shape<128> { static constexpr int WM = 2, WN = 2; };
 template <> struct Shape<256> { static constexpr int WM = 2, WN = 4; };
 
 // out = by (in in^T)              POLY false: A from X
-// out = a I + b in + c (in in^T)  POLY true: B from A, columns quad-swapped
+// out = a I + b in + c (in in^T)  POLY true: B from A, columns quad-swapped;
+//                                 not SPLIT: less kNsDiag I (ns_update_kernel)
 // SPLIT: in and out are two fp16 numbers each (all but the product of the low
 // ones is taken), and a matrix has one tile.
 // Bound by the main loop where tiles fill the card: 24 of 1024 x 4096, tiles of
@@ -298,7 +299,7 @@ ns_square_kernel(const uint16_t* __restrict__ in, uint16_t* __restrict__ out,
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             x[e] += kNsB * (SPLIT ? h2f(o.v[e]) + h2f(l.v[e]) : h2f(o.v[e])) +
-                    (i == j + e ? kNsA : 0.f);
+                    (i == j + e ? (SPLIT ? kNsA : kNsA - kNsDiag) : 0.f);
         }
         Pack<uint16_t, 4> y;
 #pragma unroll
@@ -319,7 +320,7 @@ ns_square_kernel(const uint16_t* __restrict__ in, uint16_t* __restrict__ out,
 
 struct NsUpdate {
   const uint16_t *b, *xh;             // b: columns quad-swapped
-  const uint8_t* xl;                  // or none
+  const void* xl;                     // X's low part: kFirst fp16, kNext fp8
   uint16_t* yh;                       // the next X, or
   uint8_t* yl;                        // (or none)
   const uint16_t *bw, *xw;            // SPLIT: the low halves
@@ -329,18 +330,27 @@ struct NsUpdate {
   bool tall;
 };
 
-// B X, and a times the low part of X
+enum { kFirst, kNext, kLast };          // steps; one alone is kLast
+
+// B X, and a times the low part of X (the last step's X has none).
+// a X takes X's fp16 part exactly: on B's diagonal a would leave every row an
+// error of up to 2^-10 of its own, so what lies there is what kNsDiag leaves of
+// a, and kNsDiag X is a product more with a diagonal operand, for the 64 rows
+// of a wave where the walk over k passes them: 2 FM in FM FN np / 16.
 // SPLIT: all but the product of the low halves (a lies on B's diagonal)
-// Bound by the main loop: 24 of 1024 x 4096 in 260 us (0.79 PFLOP/s, at best
-// 0.94); 12 of 768 x 2304 in 63 us, 324 tiles on 256 CUs, and 92 where the
+// Bound by the main loop: 24 of 1024 x 4096 in 270 us (0.76 PFLOP/s, at best
+// 0.84); 12 of 768 x 2304 in 68 us, 324 tiles on 256 CUs, and 80 where the
 // result is stored transposed, in pieces of 2 bytes.
-template <int TILE, bool LAST, bool SPLIT>
+template <int TILE, int STEP, bool SPLIT>
 __global__ __launch_bounds__(Shape<TILE>::WM* Shape<TILE>::WN* kWave) void
 ns_update_kernel(NsUpdate a) {
   constexpr int WM = Shape<TILE>::WM, WN = Shape<TILE>::WN;
   constexpr int NT = WM * WN * kWave, TS = TILE * kDepth;
   constexpr int FM = TILE / WM / 32, FN = TILE / WN / 32;
   constexpr int BUF = (SPLIT ? 4 : 2) * TS;   // of one turn
+  constexpr bool LAST = STEP == kLast;
+  constexpr bool LOW8 = !SPLIT && STEP == kNext, LOW16 = !SPLIT && STEP == kFirst;
+  static_assert(SPLIT || FN * 32 == kDepth, "a wave's rows are a stage of k");
   __shared__ __attribute__((aligned(16))) uint16_t lds[2 * BUF];
   const int nbi = a.np / TILE, nbj = a.mp / TILE;
   int blk = xcd_block(blockIdx.x, gridDim.x);
@@ -369,6 +379,7 @@ ns_update_kernel(NsUpdate a) {
     }
   };
   stage(lds, 0);
+  const int own = bi * (TILE / kDepth) + wc;   // the stage of this wave's rows
   auto step = [&](int t, auto half) {
     constexpr int LX = decltype(half)::value * BUF, LB = LX + TS;
     __builtin_amdgcn_s_waitcnt(0);
@@ -402,6 +413,24 @@ ns_update_kernel(NsUpdate a) {
         }
       }
     });
+    if constexpr (!SPLIT) {
+      if (t == own) {
+        unroll<kDepth / 16>([&](auto st) {
+          // columns 16 st.. of rows 32 (st / 2) + (lane & 31), in tr's order
+          s16x8 fa[FM], d;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            d[e] = (st & 1) * 16 + (e >> 2) * 8 + (lane >> 5) * 4 + (e & 3) ==
+                           (lane & 31)
+                       ? (short)from_f32<FP16>(kNsDiag).v
+                       : (short)0;
+          fx.template tr<FM, st * 16 * TILE>(fa, LX * 2);
+#pragma unroll
+          for (int u = 0; u < FM; ++u)
+            acc[u][st / 2] = mfma32<FP16>(fa[u], d, acc[u][st / 2]);
+        });
+      }
+    }
   };
   for (int t = 0; t < nt; t += 2) {
     step(t, std::integral_constant<int, 0>{});
@@ -428,10 +457,16 @@ ns_update_kernel(NsUpdate a) {
 #pragma unroll
   for (int v = 0; v < FN; ++v) {
     uint2 low[TURNS] = {};                     // on their way meanwhile
-    if (!SPLIT && a.xl) {
+    P8 half_low[TURNS] = {};
 #pragma unroll
-      for (int n = 0; n < TURNS; ++n)
-        low[n] = *reinterpret_cast<const uint2*>(a.xl + place_of(v, row_of(n)));
+    for (int n = 0; n < TURNS; ++n) {
+      const long o = place_of(v, row_of(n));
+      if (LOW8)
+        low[n] = *reinterpret_cast<const uint2*>(
+            static_cast<const uint8_t*>(a.xl) + o);
+      if (LOW16)
+        half_low[n] = *reinterpret_cast<const P8*>(
+            static_cast<const uint16_t*>(a.xl) + o);
     }
     __syncthreads();
 #pragma unroll
@@ -457,9 +492,13 @@ ns_update_kernel(NsUpdate a) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) x[e * 4 + k] = y.v[k];
       }
-      if (!SPLIT && a.xl) {
+      if (LOW8) {
         add_low(x, low[n].x, kNsA / kLowScale);
         add_low(x + 4, low[n].y, kNsA / kLowScale);
+      }
+      if (LOW16) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] += kNsA * h2f(half_low[n].v[e]);
       }
       if (!LAST) {
         P8 yh;
@@ -733,18 +772,14 @@ void launch_small(const at::Tensor& g, at::Tensor& out, int batch, int rows,
 
 template <typename T, int V>
 void launch_start(const at::Tensor& g, double* part, int parts, uint16_t* xh,
-                  void* xl, bool wide, int batch, int rows, int cols, int np, int mp,
+                  uint16_t* xl, int batch, int rows, int cols, int np, int mp,
                   double eps, hipStream_t s) {
   const T* p = static_cast<const T*>(g.data_ptr());
   ns_norm_kernel<T, V><<<dim3(parts, batch), 256, 0, s>>>(p, part,
                                                           (long)rows * cols);
   const dim3 grid(mp / 64, np / 64, batch);
-  if (wide)
-    ns_split_kernel<T, V, true><<<grid, 256, 0, s>>>(
-        p, part, parts, xh, xl, rows, cols, rows > cols, np, mp, eps);
-  else
-    ns_split_kernel<T, V, false><<<grid, 256, 0, s>>>(
-        p, part, parts, xh, xl, rows, cols, rows > cols, np, mp, eps);
+  ns_split_kernel<T, V><<<grid, 256, 0, s>>>(
+      p, part, parts, xh, xl, rows, cols, rows > cols, np, mp, eps);
 }
 
 // ---------------------------------------------------------------------------
@@ -957,8 +992,10 @@ at::Tensor newton_schulz_impl(const at::Tensor& g_in, int64_t steps,
 
   const auto half = g.options().dtype(at::kHalf);
   auto x = at::empty({2, batch, np, mp}, half);       // X twice
-  auto low = at::empty({2, batch, np, mp},
-                       wide ? half : g.options().dtype(at::kByte));
+  // X's low parts: two fp16 (wide); or X_0's fp16, in whose place every second
+  // fp8 one follows, and the others' fp8: three bytes an element
+  auto low = at::empty({wide ? 4 : 3, batch, np, mp},
+                       g.options().dtype(at::kByte));
   auto sq = at::empty({wide ? 4 : 2, batch, np, np}, half);   // A, B
   auto part = at::empty({batch, parts}, g.options().dtype(at::kDouble));
   auto* px = static_cast<uint16_t*>(x.data_ptr());
@@ -976,8 +1013,8 @@ at::Tensor newton_schulz_impl(const at::Tensor& g_in, int64_t steps,
                     reinterpret_cast<uintptr_t>(g.data_ptr()) % 16 == 0;
     (v4 ? launch_start<T, 4> : launch_start<T, 1>)(
         g, part.data_ptr<double>(), (int)parts, px,
-        wide || steps > 2 ? low.data_ptr() : nullptr, wide, (int)batch,
-        (int)rows, (int)cols, (int)np, (int)mp, eps, s);
+        wide || steps > 1 ? pw : nullptr, (int)batch, (int)rows, (int)cols,
+        (int)np, (int)mp, eps, s);
   };
   switch (g.scalar_type()) {
     case at::kFloat: start(float{}); break;
@@ -1001,15 +1038,17 @@ at::Tensor newton_schulz_impl(const at::Tensor& g_in, int64_t steps,
         <<<(unsigned)(batch * pairs), NT, 0, s>>>(
             in, to, in_low, to_low, (int)np, (int)depth, (int)pairs);
   };
-  auto update = [&](auto tile, auto split, bool last, const NsUpdate& u) {
+  auto update = [&](auto tile, auto split, int step, const NsUpdate& u) {
     constexpr int TILE = decltype(tile)::value;
     constexpr int NT = Shape<TILE>::WM * Shape<TILE>::WN * kWave;
     const unsigned blocks = (unsigned)(batch * (np / TILE) * (mp / TILE));
-    if (last)
-      ns_update_kernel<TILE, true, decltype(split)::value>
-          <<<blocks, NT, 0, s>>>(u);
-    else
-      ns_update_kernel<TILE, false, decltype(split)::value>
+    constexpr bool SPLIT = decltype(split)::value;
+    if (step == kLast)
+      ns_update_kernel<TILE, kLast, SPLIT><<<blocks, NT, 0, s>>>(u);
+    else if (step == kNext)
+      ns_update_kernel<TILE, kNext, SPLIT><<<blocks, NT, 0, s>>>(u);
+    else                               // SPLIT: the first is like the next
+      ns_update_kernel<TILE, SPLIT ? kNext : kFirst, SPLIT>
           <<<blocks, NT, 0, s>>>(u);
   };
   for (int64_t k = 0; k < steps; ++k) {
@@ -1028,17 +1067,18 @@ at::Tensor newton_schulz_impl(const at::Tensor& g_in, int64_t steps,
       square(Small{}, No{}, No{}, cur, pa, nullptr, nullptr, mp);
       square(Small{}, Yes{}, No{}, pa, pb, nullptr, nullptr, np);
     }
-    // the last two X that are multiplied have no low part (but a wide one)
-    const bool in_low = !wide && k + 2 < steps, to_low = !wide && k + 3 < steps;
-    const NsUpdate u{pb, cur, in_low ? pl + (k & 1) * xs : nullptr, nxt,
-                     to_low ? pl + ((k + 1) & 1) * xs : nullptr, b_low, cur_low,
+    // what the last X loses has no time to grow: it has no low part
+    auto low_of = [&](int64_t i) { return pl + (i & 1) * 2 * xs; };
+    const bool to_low = !wide && k + 2 < steps;
+    const NsUpdate u{pb, cur, low_of(k), nxt,
+                     to_low ? low_of(k + 1) : nullptr, b_low, cur_low,
                      wide ? pw + ((k + 1) & 1) * xs : nullptr,
                      static_cast<uint16_t*>(out.data_ptr()), (int)np, (int)mp,
                      (int)rows, (int)cols, rows > cols};
-    const bool last = k + 1 == steps;
-    if (wide) update(Thin{}, Yes{}, last, u);
-    else if (large) update(Large{}, No{}, last, u);
-    else update(Small{}, No{}, last, u);
+    const int which = k + 1 == steps ? kLast : k ? kNext : kFirst;
+    if (wide) update(Thin{}, Yes{}, which, u);
+    else if (large) update(Large{}, No{}, which, u);
+    else update(Small{}, No{}, which, u);
   }
   return out;
 }

@@ -813,8 +813,12 @@ def newton_schulz(g: torch.Tensor, steps: int = 5,
     ``X = g / (|g| + eps)``; the result, in bf16, has singular values near 1.
 
     ``g`` is fp32, bf16 or fp16.  Matrices of a batch share their launches.
-    The products take fp16 operands with fp32 sums; X itself is carried in 15
-    bits (up to 64 rows: all operands in 22).  A zero matrix stays zero.  Gives no gradient.
+    The products take fp16 operands with fp32 sums; X itself is carried in 22
+    bits, then 15, and the last one in 11 (up to 64 rows: all operands in 22).
+    What is rounded in a direction without signal grows 3.4 times a step: five
+    steps leave 1.4 times the rounding of the result, many more of a matrix
+    that is not of full rank leave noise.  A zero matrix stays zero.  Gives no
+    gradient.
     """
     if g.dim() < 2 or not g.is_floating_point():
         raise ValueError("newton_schulz: a floating [..., rows, cols] "
