@@ -148,8 +148,10 @@ struct EmbeddingSumBackward : Node {
         want_scales.push_back(scales[i]);
       }
     if (want.empty() || !dy.defined()) return out;
-    const auto got = embed_sum_bwd_impl(dy.reshape({-1, dy.size(-1)}), want,
-                                        want_rows, want_scales);
+    // -1 in place of the tokens would be ambiguous for rows of no width
+    const auto got =
+        embed_sum_bwd_impl(dy.reshape({want[0].numel(), dy.size(-1)}), want,
+                           want_rows, want_scales);
     for (size_t i = 0, k = 0; i < ids.size(); ++i)
       if (task_should_compute_output(i)) out[i] = got[k++];
     return out;

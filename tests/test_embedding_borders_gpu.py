@@ -1,0 +1,38 @@
+"""Embedding lookup (embedding.hip) at the borders of what it takes."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _f():
+    from deeplearning_cfn_amd.ops import functional
+    return functional
+
+
+@pytest.mark.parametrize("shape", [(), (0,), (3,), (2, 0), (2, 3)])
+@pytest.mark.parametrize("width", [0, 5])
+@pytest.mark.parametrize("rows", [0, 4])
+def test_nothing_of_something(rows, width, shape):
+    """No tokens, no width, no rows: outputs and gradients have their shapes,
+    as on the CPU."""
+    tokens = 1
+    for n in shape:
+        tokens *= n
+    if rows == 0 and tokens and width:
+        return                            # ids outside a table: NaN, not 0
+    got = []
+    for device in ("cuda", "cpu"):
+        if device == "cpu" and rows == 0 and tokens:
+            continue                      # raises there
+        w = torch.ones(rows, width, device=device, requires_grad=True)
+        v = torch.ones(7, width, device=device, requires_grad=True)
+        i = torch.zeros(shape, dtype=torch.int64, device=device)
+        y = _f().embedding_sum([i, i], [w, v], [1.0, 2.0])
+        assert y.shape == (*shape, width)
+        d = torch.autograd.grad(y, [w, v], torch.ones_like(y))
+        assert d[0].shape == w.shape and d[1].shape == v.shape
+        got.append([t.cpu() for t in (y, *d)])
+    for a, b in zip(*got) if len(got) == 2 else ():
+        assert torch.equal(a, b)
