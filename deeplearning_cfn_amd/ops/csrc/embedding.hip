@@ -733,6 +733,44 @@ at::Tensor embed_sum_fwd_impl(at::TensorList ids_in, at::TensorList tables_in,
   return y;
 }
 
+namespace {
+
+// The buckets of a table of so many rows (log2), and the ids of each: 256
+// buckets, more where a bucket's counts would not fit a block's LDS.
+struct Buckets {
+  int lg;
+  long own;
+  explicit Buckets(long rows) : lg(0) {
+    while ((1l << lg) < rows && (lg < 8 || (rows >> lg) >= kMaxOwn)) ++lg;
+    own = std::max<long>((rows + (1l << lg) - 1) >> lg, 1);
+  }
+  long places() const { return own << lg; }
+  long light_blocks() const {
+    return (places() + 4 * kLightRows - 1) / (4 * kLightRows);
+  }
+};
+
+}  // namespace
+
+// Whether the gradient of such a lookup can be taken: what the lookup itself
+// has no reason to refuse is refused before it, not in the backward pass.
+void embed_check_grad(int64_t n, int64_t width, at::IntArrayRef rows) {
+  TORCH_CHECK_VALUE(width <= (1 << 21) && n <= (1 << 30),
+                    "embedding_sum: a gradient of ", n, " tokens of ", width,
+                    " is too large");
+  long blocks = (long)rows.size() * (n / kSlotUnit + 1);
+  for (const int64_t r : rows) {
+    TORCH_CHECK_VALUE(r >= 0 && r < (1l << (2 * kMaxSplit)),
+                      "embedding_sum: a table with a gradient has under 2^22 "
+                      "rows, got ", r);
+    blocks += Buckets(r).light_blocks();
+  }
+  // a grid has under 2^32 threads in x
+  TORCH_CHECK_VALUE(blocks < (1l << 24),
+                    "embedding_sum: too many tokens, or too large tables, for "
+                    "a gradient");
+}
+
 // dy: [n, width]; rows: of each table -> the tables' gradients in dy's type
 std::vector<at::Tensor> embed_sum_bwd_impl(const at::Tensor& dy_in,
                                            at::TensorList ids_in,
@@ -746,8 +784,7 @@ std::vector<at::Tensor> embed_sum_bwd_impl(const at::Tensor& dy_in,
   const c10::DeviceGuard guard(dy_in.device());
   const auto dy = dy_in.contiguous();
   const long n = dy.size(0), width = dy.size(1);
-  TORCH_CHECK(width <= (1 << 21) && n <= (1 << 30),
-              "embedding: the gradient is too large");
+  embed_check_grad(n, width, rows);
   const long slots = n / kSlotUnit + 1;
   const long joins = n / kPiece + 1;
   std::vector<at::Tensor> hold, out;
@@ -758,22 +795,18 @@ std::vector<at::Tensor> embed_sum_bwd_impl(const at::Tensor& dy_in,
   long buckets = 0, light_blocks = 0, most = 1, ints = 0, at[kMaxTables];
   for (size_t j = 0; j < nt; ++j) {
     check_ids(ids_in[j], dy, n);
-    TORCH_CHECK(rows[j] >= 0 && rows[j] < (1l << (2 * kMaxSplit)),
-                "embedding: a table has too many rows");
     out.push_back(at::empty({rows[j], width}, dy.options()));
     GradTable& t = a.t[j];
     t.rows = (int)rows[j];
-    // 256 buckets, more where a bucket's counts would not fit a block's LDS
-    int lg = 0;
-    while ((1l << lg) < rows[j] && (lg < 8 || (rows[j] >> lg) >= kMaxOwn)) ++lg;
-    const long own = std::max<long>((rows[j] + (1l << lg) - 1) >> lg, 1);
-    most = std::max(most, std::max(own, 1l << lg));
-    t.own = (int)own;
+    const Buckets split(rows[j]);
+    const int lg = split.lg;
+    most = std::max(most, std::max(split.own, 1l << lg));
+    t.own = (int)split.own;
     t.lg = lg;
     t.bucket0 = (int)buckets;
     buckets += 1l << lg;
     t.light0 = (int)light_blocks;
-    light_blocks += ((own << lg) + 4 * kLightRows - 1) / (4 * kLightRows);
+    light_blocks += split.light_blocks();
     if (!ids_in[j].is_contiguous()) hold.push_back(ids_in[j].contiguous());
     t.ids = (ids_in[j].is_contiguous() ? ids_in[j] : hold.back()).data_ptr();
     t.ids64 = ids_in[j].scalar_type() == at::kLong;
@@ -782,8 +815,8 @@ std::vector<at::Tensor> embed_sum_bwd_impl(const at::Tensor& dy_in,
     // all tables' lists in one piece of memory, each from a 16-byte border
     const long g = n > kDirect ? 1l << lg : 0, m = n > kDirect ? n : 0;
     at[j] = ints;
-    ints += (g * kChunks + 2 * m + n + g + 1 + (own << lg) + 1 + slots + joins +
-             3) / 4 * 4;
+    ints += (g * kChunks + 2 * m + n + g + 1 + split.places() + 1 + slots +
+             joins + 3) / 4 * 4;
   }
   if (width == 0) return out;
   if (n == 0) {
@@ -808,9 +841,6 @@ std::vector<at::Tensor> embed_sum_bwd_impl(const at::Tensor& dy_in,
     t.part = part + (long)j * slots * width;
   }
   const long blocks = (long)nt * slots + light_blocks;
-  // a grid has under 2^32 threads in x
-  TORCH_CHECK(blocks < (1l << 24),
-              "embedding: too many tokens, or too large tables");
   auto s = at::cuda::getCurrentCUDAStream();
   const size_t lds = ((size_t)kSortWaves * (most + 2)) * sizeof(int);
   if (direct) {

@@ -21,6 +21,7 @@ std::vector<at::Tensor> embed_sum_bwd_impl(const at::Tensor& dy,
                                            at::TensorList ids,
                                            at::IntArrayRef rows,
                                            at::ArrayRef<double> scales);
+void embed_check_grad(int64_t n, int64_t width, at::IntArrayRef rows);
 std::tuple<at::Tensor, at::Tensor, at::Tensor> doc_attn_fwd_impl(
     const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
     const at::Tensor& cu, const c10::optional<at::Tensor>& slopes,
@@ -236,6 +237,10 @@ at::Tensor embedding_sum(at::TensorList ids, at::TensorList tables,
   check_lookup(ids, tables, scales);
   std::shared_ptr<EmbeddingSumBackward> node;
   if (wants_grad(tables)) {
+    std::vector<int64_t> wanted;
+    for (const auto& w : tables)
+      if (w.requires_grad()) wanted.push_back(w.size(0));
+    embed_check_grad(ids[0].numel(), tables[0].size(1), wanted);
     node.reset(new EmbeddingSumBackward, torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(tables));
     for (const auto& i : ids) node->ids.emplace_back(i, false);

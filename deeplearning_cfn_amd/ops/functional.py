@@ -640,7 +640,8 @@ def embedding_sum(ids: Sequence[torch.Tensor], tables: Sequence[torch.Tensor],
     of one type (bf16, fp16, fp32).  The sum is taken in fp32 and rounded
     once.  A table's gradient adds its tokens in their order in fp32, so it
     is the same from run to run.  On the GPU an id outside its table gives a
-    row of NaN and takes no part in the gradient (on the CPU it raises).
+    row of NaN and takes no part in the gradient (on the CPU it raises), and
+    a table that wants a gradient has under 2^22 rows.
     """
     ids, tables = list(ids), list(tables)
     scales = [1.0] * len(tables) if scales is None else [float(c)

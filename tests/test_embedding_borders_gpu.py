@@ -36,3 +36,29 @@ def test_nothing_of_something(rows, width, shape):
         got.append([t.cpu() for t in (y, *d)])
     for a, b in zip(*got) if len(got) == 2 else ():
         assert torch.equal(a, b)
+
+
+def test_large_tables_are_refused_before_the_lookup():
+    """What has no gradient kernel raises in the forward pass, if a gradient
+    is wanted of it; without one it is looked up."""
+    rows = 2 ** 22
+    big = torch.zeros(rows, 1, device="cuda", dtype=torch.bfloat16)
+    big[-1] = 3
+    small = torch.ones(5, 1, device="cuda", dtype=torch.bfloat16)
+    i = torch.tensor([rows - 1, 0], device="cuda")
+    j = torch.tensor([4, 4], device="cuda")
+    f = _f().embedding_sum
+    assert f([i], [big]).flatten().tolist() == [3, 0]
+    y = f([i, j], [big, small.requires_grad_(True)])
+    d, = torch.autograd.grad(y, [small], torch.ones_like(y))
+    assert d.flatten().tolist() == [0, 0, 0, 0, 2]
+    big.requires_grad_(True)
+    for ids, tables in (([i], [big]), ([j, i], [small, big])):
+        with pytest.raises(ValueError, match="embedding_sum.*2\\^22"):
+            f(ids, tables)
+        with torch.no_grad():
+            assert f(ids, tables).isfinite().all()
+    less = torch.zeros(rows - 1, 1, device="cuda", requires_grad=True)
+    y = f([i - 1], [less])
+    d, = torch.autograd.grad(y[:1], [less], torch.ones(1, 1, device="cuda"))
+    assert d[rows - 2] == 1 and d.sum() == 1
