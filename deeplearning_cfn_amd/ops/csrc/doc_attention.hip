@@ -200,6 +200,14 @@ DLX_DEV void zero_rows(const View& v, long token, int head, int dim, int lane) {
 // register i of a result: its row of 32
 DLX_DEV constexpr int reg_row(int i) { return 8 * (i >> 2) + (i & 3); }
 
+// A head's slope in units of the scores before their scale.  A finite one stays
+// finite: infinity times a distance of 0 would be NaN, where nothing is taken
+// off.
+DLX_DEV float slope_of(const AttnArgs& a, int head) {
+  const float s = a.slopes[head], x = s / a.scale;
+  return isinf(x) && !isinf(s) ? copysignf(3.402823466e38f, s) : x;
+}
+
 // What a block of scores begins at: -sl |key - query|, keys k0 + .., queries
 // wave_row ..+31, shift = 4 * (lane >> 5) - query.  Where the block lies on
 // one side of the diagonal the sign is known, and a register takes one fma.
@@ -263,7 +271,7 @@ __global__ __launch_bounds__(NW * 64, DP == 64 ? 4 : 2) void doc_attn_fwd_kernel
 
   const Frags<DP> fr(lds, lane);
   const float sc = a.scale * kLog2e;
-  const float sl = BIAS ? a.slopes[head] / a.scale : 0.f;
+  const float sl = BIAS ? slope_of(a, head) : 0.f;
   // m: what the row's exponents are taken next to; it follows the row's
   // maximum only when that is past it by 2^kLazy, which spares the products
   // their rescaling in nearly every tile.  ms: m, or 0 in a row of -inf.
@@ -420,7 +428,7 @@ __global__ __launch_bounds__(NW * 64, DP == 64 ? 3 : 2) void doc_attn_dq_kernel(
   const float lse = a.lse[(long)head * a.tokens + token];
   const Frags<DP> fr(lds, lane);
   const float sc = a.scale * kLog2e;
-  const float sl = BIAS ? a.slopes[head] / a.scale : 0.f;
+  const float sl = BIAS ? slope_of(a, head) : 0.f;
   f32x16 acc[DP / 32] = {};
   f32x16 less;                        // what dP begins at: dP - D for nothing
 #pragma unroll
@@ -566,7 +574,7 @@ __global__ __launch_bounds__(NW * 64, DP == 64 ? 3 : 2) void doc_attn_dkv_kernel
     const float (*st_)[kKeys] = stat[H];
     int place = kpos;                  // nothing of the first turn is kept
     if (REST) asm volatile("" : "+v"(place)::"memory");
-    const float sl = BIAS ? a.slopes[kvh * a.group + n / nt] / a.scale : 0.f;
+    const float sl = BIAS ? slope_of(a, kvh * a.group + n / nt) : 0.f;
     unroll<2>([&](auto b) {
       const int q0 = b * 32 + half * 4;
       const float d0 = (float)((n % nt) * kKeys + q0 - place);
