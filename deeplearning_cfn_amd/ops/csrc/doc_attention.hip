@@ -55,6 +55,17 @@ constexpr int kWide = 1024;
 // shows (14 -> 14.7 us of the forward's 32 x 128).
 constexpr int kFine = 64, kFineAll = 1024;
 constexpr float kLazy = 8.f;          // P stays under 2^8
+// fp16 ends at 6e-8.  dS is about gradient / tokens, so gradients of 1e-3 over
+// 4096 tokens left dq and dk off by 8 times what rounding the exact ones costs
+// (gradients of 1: 1.4), a dS past 65504 was infinite, and of 60000 tokens P
+// itself is down there.  So fp16's gradients take P, which is at most 1, times
+// 2^14, and dP - D times a power of two (`up`) that each query (key) holds on
+// to until one grows past it.  That costs 4 to 6 % (16384 tokens in documents
+// of 512, 12 heads of 64, slopes: 196 -> 205 us; 8192 of 16 heads of 128 on
+// four: 1230 -> 1300).
+constexpr int kPUp = 14;
+constexpr float kPDown = 1.f / (1 << kPUp);
+constexpr float kUp0 = 0x1p46f;       // where `up` begins: it only falls
 
 __device__ const uint4 g_zero16 = {0, 0, 0, 0};
 
@@ -370,6 +381,34 @@ __global__ __launch_bounds__(NW * 64, DP == 64 ? 4 : 2) void doc_attn_fwd_kernel
   }
 }
 
+template <typename T> constexpr bool kHalf = std::is_same_v<T, FP16>;
+
+// Whether one of a wave's dP - D, times its `up`, is past 1, and what up and all
+// that was summed are multiplied by then to have 2^6 of room again (1 in lanes
+// that need none): times a P of at most 2^14 it stays in fp16.  Lanes l and
+// l ^ 32 hold one query (key).
+DLX_DEV bool lower(const f32x16& dp, float up, float& f) {
+  float mx = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) mx = fmaxf(mx, fabsf(dp[i]));
+  mx *= up;
+  if (!__ballot(mx > 1.f)) return false;
+  const uint32_t x = __builtin_bit_cast(uint32_t, mx);
+  const auto both = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  const uint32_t top = both[0] > both[1] ? both[0] : both[1];  // not negative
+  // to 2^-6 .. 2^-5; infinity stays what it is
+  f = top > 0x3f800000u && top < 0x7f800000u
+          ? __builtin_bit_cast(float, (127u - 6u + 127u - (top >> 23)) << 23)
+          : 1.f;
+  return true;
+}
+
+// What exp2 takes off for P times 2^kPUp and up.
+DLX_DEV float scaled(float lse, float up) {
+  return lse -
+         (float)(kPUp - 127 + (int)(__builtin_bit_cast(uint32_t, up) >> 23));
+}
+
 // ---------------------------------------------------------------------------
 // gradient of the queries: the forward's walk over the keys, a third product.
 // Also writes delta, which the next kernel reads.  The same packed tokens:
@@ -425,7 +464,9 @@ __global__ __launch_bounds__(NW * 64, DP == 64 ? 3 : 2) void doc_attn_dq_kernel(
     delta += __shfl_xor(delta, 32, kWave);
   }
   if (real && half == 0) a.delta[(long)head * a.tokens + token] = delta;
-  const float lse = a.lse[(long)head * a.tokens + token];
+  const float lse0 = a.lse[(long)head * a.tokens + token];
+  float up = kHalf<T> ? kUp0 : 1.f;
+  float lse = kHalf<T> ? scaled(lse0, up) : lse0;   // P comes out times both
   const Frags<DP> fr(lds, lane);
   const float sc = a.scale * kLog2e;
   const float sl = BIAS ? slope_of(a, head) : 0.f;
@@ -453,6 +494,15 @@ __global__ __launch_bounds__(NW * 64, DP == 64 ? 3 : 2) void doc_attn_dq_kernel(
       for (int st = 0; st < DP / 16; ++st) {
         s = mfma32<T>(fr.row(LK + b * 32 * DP, st), qf[st], s);
         dp = mfma32<T>(fr.row(LV + b * 32 * DP, st), gf[st], dp);
+      }
+      if constexpr (kHalf<T>) {
+        float f;
+        if (lower(dp, up, f)) {
+          up *= f;
+          lse = scaled(lse0, up);
+#pragma unroll
+          for (int db = 0; db < DP / 32; ++db) acc[db] *= f;
+        }
       }
       float ds[16];
 #pragma unroll
@@ -490,7 +540,9 @@ __global__ __launch_bounds__(NW * 64, DP == 64 ? 3 : 2) void doc_attn_dq_kernel(
   else walk(std::false_type{});
   if (real)             // of one score p is 1: nothing depends on q or k
     store_rows<T, DP>(a.dq.p + token * a.dq.token + head * a.dq.head, acc,
-                      tl.len == 1 ? 0.f : a.scale, a.dim, lane);
+                      tl.len == 1 ? 0.f
+                                  : a.scale * (kHalf<T> ? kPDown : 1.f) / up,
+                      a.dim, lane);
 }
 
 // ---------------------------------------------------------------------------
@@ -554,7 +606,8 @@ __global__ __launch_bounds__(NW * 64, DP == 64 ? 3 : 2) void doc_attn_dkv_kernel
       // what S and dP begin at; behind the document's end exp2(-inf) is 0
       const int r = row0 + threadIdx.x;
       const long i = (long)head * a.tokens + tl.start + r;
-      st[0][threadIdx.x] = r < tl.len ? a.lse[i] * -unit : -INFINITY;
+      st[0][threadIdx.x] =
+          r < tl.len ? (a.lse[i] - (kHalf<T> ? kPUp : 0)) * -unit : -INFINITY;
       st[1][threadIdx.x] = r < tl.len ? -a.delta[i] : 0.f;
     }
   };
@@ -564,6 +617,7 @@ __global__ __launch_bounds__(NW * 64, DP == 64 ? 3 : 2) void doc_attn_dkv_kernel
   load_rows<DP>(vf, a.v.p + token * a.v.token + kvh * a.v.head, a.dim, lane);
   const Frags<DP> fr(lds, lane);
   f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
+  float up = kUp0;                      // fp16's
 
   // REST: what rounding P and dS has left, in a turn of its own over the same
   // tile (in the first one it would need registers that are not there)
@@ -595,12 +649,22 @@ __global__ __launch_bounds__(NW * 64, DP == 64 ? 3 : 2) void doc_attn_dkv_kernel
         s = mfma32<T>(fr.row(LQ + b * 32 * DP, st), kf[st], s);
         dp = mfma32<T>(fr.row(LG + b * 32 * DP, st), vf[st], dp);
       }
+      if constexpr (kHalf<T>) {
+        float f;
+        // the second turn finds what the first has made room for
+        if (!REST && lower(dp, up, f)) {
+          up *= f;
+#pragma unroll
+          for (int db = 0; db < DP / 32; ++db) dk[db] *= f;
+        }
+      }
       unroll<2>([&](auto st) {
         float p[8], ds[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           p[e] = __builtin_amdgcn_exp2f(s[st * 8 + e] * sc);
           ds[e] = p[e] * dp[st * 8 + e];
+          if (kHalf<T>) ds[e] *= up;
         }
         s16x8 pf = pack_step<T>(p), df = pack_step<T>(ds);
         if (REST) {
@@ -634,6 +698,14 @@ __global__ __launch_bounds__(NW * 64, DP == 64 ? 3 : 2) void doc_attn_dkv_kernel
     if (n + 1 < n1) body(n + 1, std::integral_constant<int, 1>{});
   }
   if (!real) return;
+  if (kHalf<T>) {
+    const float less = kPDown / up;
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b) {
+      dk[b] *= less;
+      dv[b] *= kPDown;
+    }
+  }
   if (tl.len == 1) {    // of one score p is 1: nothing depends on q or k
 #pragma unroll
     for (int b = 0; b < DP / 32; ++b) dk[b] *= 0.f;
