@@ -27,6 +27,8 @@
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 
+#include <algorithm>
+
 #include "seq_common.h"
 
 namespace dlx {
@@ -308,19 +310,16 @@ DLX_DEV int2 token_at(const GradTable& t, int i, int end, int me, int& less) {
 // A bucket's tokens by id / G.  DIRECT: few tokens; every block looks at all
 // of them, and those of lower buckets, counted on the way, are the place where
 // its own begin, which saves the launches that make the buckets (three tables,
-// 4096 tokens of 768: 37 us for a whole gradient, 41 with buckets).
+// 4096 tokens of 768: 32 us for a whole gradient, more with buckets).
 // Bound by its chain of reads, counts, a scan and a second walk: 16384 tokens
-// in three tables 12 us, 65536 in one 15.5 us; two tables of 3001 tokens,
+// in three tables 11 us, 65536 in one 15.5 us; two tables of 3001 tokens,
 // without buckets, 10 us.
 // LDS: counts [wave][own], then scratch.
 template <bool DIRECT>
 __global__ __launch_bounds__(kSortThreads) void embed_order_kernel(GradArgs a,
                                                                    int n) {
   extern __shared__ int lds[];
-  // the last table's buckets first: a small table, whose buckets are long,
-  // often follows a large one (16384 tokens in three tables: 13.4 -> 11.8 us)
-  const int blk =
-      DIRECT ? (int)blockIdx.x : (int)(gridDim.x - 1 - blockIdx.x);
+  const int blk = (int)blockIdx.x;
   int j = 0;
   while (j + 1 < a.n && blk >= a.t[j + 1].bucket0) ++j;
   const GradTable& tb = a.t[j];
@@ -793,10 +792,23 @@ std::vector<at::Tensor> embed_sum_bwd_impl(const at::Tensor& dy_in,
   a.slots = (int)slots;
   a.joins = (int)joins;
   long buckets = 0, light_blocks = 0, most = 1, ints = 0, at[kMaxTables];
+  // Tables of few rows first, whatever their order in the call: they have the
+  // longest buckets, whose blocks should not begin last.  embed_order of 16384
+  // tokens in tables of 30528, 512 and 2 rows: 10.6 to 11.1 us in any order of
+  // the call, by the call's own 10.3 to 13.3; the whole gradient of 4096 tokens
+  // in them 32 us, in the call's order 35 to 36.5.
+  size_t by_rows[kMaxTables];
   for (size_t j = 0; j < nt; ++j) {
     check_ids(ids_in[j], dy, n);
     out.push_back(at::empty({rows[j], width}, dy.options()));
-    GradTable& t = a.t[j];
+    by_rows[j] = j;
+  }
+  std::sort(by_rows, by_rows + nt, [&](size_t x, size_t y) {
+    return rows[x] != rows[y] ? rows[x] < rows[y] : x < y;
+  });
+  for (size_t k = 0; k < nt; ++k) {
+    const size_t j = by_rows[k];
+    GradTable& t = a.t[k];
     t.rows = (int)rows[j];
     const Buckets split(rows[j]);
     const int lg = split.lg;
@@ -811,10 +823,10 @@ std::vector<at::Tensor> embed_sum_bwd_impl(const at::Tensor& dy_in,
     t.ids = (ids_in[j].is_contiguous() ? ids_in[j] : hold.back()).data_ptr();
     t.ids64 = ids_in[j].scalar_type() == at::kLong;
     t.scale = (float)scales[j];
-    t.out = out.back().data_ptr();
+    t.out = out[j].data_ptr();
     // all tables' lists in one piece of memory, each from a 16-byte border
     const long g = n > kDirect ? 1l << lg : 0, m = n > kDirect ? n : 0;
-    at[j] = ints;
+    at[k] = ints;
     ints += (g * kChunks + 2 * m + n + g + 1 + split.places() + 1 + slots +
              joins + 3) / 4 * 4;
   }

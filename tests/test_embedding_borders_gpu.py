@@ -62,3 +62,23 @@ def test_large_tables_are_refused_before_the_lookup():
     y = f([i - 1], [less])
     d, = torch.autograd.grad(y[:1], [less], torch.ones(1, 1, device="cuda"))
     assert d[rows - 2] == 1 and d.sum() == 1
+
+
+@pytest.mark.parametrize("n", [900, 6000])
+def test_any_order_of_the_tables(n):
+    """A table's gradient has the same bits wherever it stands in the call."""
+    rows, width = [3000, 2, 512, 2], 40
+    g = torch.Generator(device="cuda").manual_seed(n)
+    ids = [torch.randint(0, r, (n,), generator=g, device="cuda") for r in rows]
+    tables = [torch.randn(r, width, generator=g, device="cuda")
+              .requires_grad_(True) for r in rows]
+    scales = [1.0, 0.5, 2.0, -1.0]
+    grad = torch.randn(n, width, generator=g, device="cuda")
+    want = None
+    for order in ((0, 1, 2, 3), (3, 2, 1, 0), (1, 3, 0, 2), (2, 0, 3, 1)):
+        pick = lambda x: [x[k] for k in order]  # noqa: E731
+        y = _f().embedding_sum(pick(ids), pick(tables), pick(scales))
+        d = dict(zip(order, torch.autograd.grad(y, pick(tables), grad)))
+        want = want or d
+        for k in range(4):
+            assert torch.equal(d[k], want[k])
