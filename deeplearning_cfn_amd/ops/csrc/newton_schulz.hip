@@ -949,16 +949,27 @@ at::Tensor newton_schulz_impl(const at::Tensor& g_in, int64_t steps,
   if (g.numel() == 0) return out;
   TORCH_CHECK(rows <= (1 << 20) && cols <= (1 << 20) && batch <= 65535,
               "newton_schulz: the matrices are too large or too many");
-  // The larger tile where it pads little and leaves about a tile a CU.  us, of
-  // 128 / 256: update of 24 1024x4096 in one part 305 / 246, of 12 768x2304
-  // 60 / 62; X X^T of the first 150 / 128, of the second, 72 tiles, 31 / 64.
+  // The larger tile where it pads little and its last round of 256 CUs is
+  // nearly full: at most 56 of them, or a sixth of all tiles, without one.  us
+  // of five steps, all of 128 / update of 256 / square too:
+  //   768 x 768      x 32 684 / 731 / 745   x 56 1095 / 1079 / 1216
+  //                  x 48 904 / 900 / 1122  x 128 2489 / 2452 / 2418
+  //   768 x 2304     x 8 429 / 414 / 691    x 12 546 / 592 / 853
+  //   1024 x 1024    x 17 733 / 828 / 838   x 48 1857 / 1769 / 1752
+  //   1024 x 4096    x 4 562 / 544 / 949    x 5 643 / 714 / 1120
+  //                  x 12 1379 / 1284 / 1542  x 24 2784 / 2582 / 2504
+  //   256 x 256      x 200 388 / 385 / 360
   const long lo = std::min(rows, cols), hi = std::max(rows, cols);
   auto pad = [](long x, long t) { return (x + t - 1) / t * t; };
   const long n256 = pad(lo, 256) / 256, m256 = pad(hi, 256) / 256;
+  auto fills = [](long tiles) {
+    const long idle = (tiles + 255) / 256 * 256 - tiles;
+    return idle <= 56 || idle * 6 <= tiles;
+  };
   const bool large = pad(lo, 256) * pad(hi, 256) * 8 <=
                          pad(lo, kTile) * pad(hi, kTile) * 9 &&
-                     batch * n256 * m256 >= 200;
-  const bool large_square = large && batch * n256 * (n256 + 1) / 2 >= 200;
+                     fills(batch * n256 * m256);
+  const bool large_square = large && fills(batch * n256 * (n256 + 1) / 2);
   // Few singular values: nothing evens out what they lose to a step, so X, A
   // and B are two fp16 numbers each, in tiles of 64 (with the parts that more
   // rows get, 40 x 1000 is off by 2.0 times what rounding the result costs,

@@ -73,3 +73,17 @@ def test_transpose_and_batch():
     y = F_amd.newton_schulz(g)
     assert torch.equal(F_amd.newton_schulz(g.mT), y.mT)
     assert torch.equal(F_amd.newton_schulz(g[3:4]), y[3:4])
+
+
+@pytest.mark.parametrize("b,n,m", [
+    (8, 768, 2304), (9, 768, 2304), (16, 1024, 1024), (17, 1024, 1024),
+    (43, 768, 768), (56, 768, 768), (200, 256, 256), (43, 500, 500)])
+def test_any_tile_gives_the_same_bits(b, n, m):
+    """Batches on both sides of where the tiles change, of update and square:
+    a matrix alone takes tiles of 128, and every tile adds in the order of k."""
+    from deeplearning_cfn_amd.ops import functional as F_amd
+    g = torch.randn(b, n, m, generator=torch.Generator(device="cuda")
+                    .manual_seed(b), device="cuda")
+    y = F_amd.newton_schulz(g)
+    for k in (0, b // 2, b - 1):
+        assert torch.equal(F_amd.newton_schulz(g[k]), y[k])
