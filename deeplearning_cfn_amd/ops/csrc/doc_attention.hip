@@ -18,10 +18,11 @@
 // P^T are at once operand B of O^T = V^T P^T (mfma_tile.h).  The gradient of
 // keys and values takes S = Q K^T instead, a lane holding one key.  P is
 // rounded to the inputs' type for the second product, as its other operand
-// is, and so is ds (in two parts where documents are short, kFine); maxima,
-// sums and all accumulators are fp32.  D takes o in twice the bits (a training
-// forward writes what rounding leaves of it): with the rounded o alone,
-// gradients are off by up to 1.57 times what rounding the exact ones costs, so
+// is, and so is ds (in two parts where documents are short, kFine; scaled in
+// fp16, kPUp); maxima, sums and all accumulators are fp32.  D takes o in twice
+// the bits (a training forward writes what rounding leaves of it): with the
+// rounded o alone, gradients are off by up to 1.57 times what rounding the
+// exact ones costs (where values have a large part in common by much more), so
 // by 1.41.  A pass over 16384 packed tokens takes 185 us instead of 181; with
 // that part in a byte, 190.
 //
@@ -60,9 +61,9 @@ constexpr float kLazy = 8.f;          // P stays under 2^8
 // (gradients of 1: 1.4), a dS past 65504 was infinite, and of 60000 tokens P
 // itself is down there.  So fp16's gradients take P, which is at most 1, times
 // 2^14, and dP - D times a power of two (`up`) that each query (key) holds on
-// to until one grows past it.  That costs 4 to 6 % (16384 tokens in documents
-// of 512, 12 heads of 64, slopes: 196 -> 205 us; 8192 of 16 heads of 128 on
-// four: 1230 -> 1300).
+// to until one grows past it.  That costs 3 to 7 % (16384 tokens in documents
+// of 512, 12 heads of 64, slopes: 194 -> 202 us; 8192 of 16 heads of 128 on
+// four: 1235 -> 1316).
 constexpr int kPUp = 14;
 constexpr float kPDown = 1.f / (1 << kPUp);
 constexpr float kUp0 = 0x1p46f;       // where `up` begins: it only falls
@@ -550,7 +551,8 @@ __global__ __launch_bounds__(NW * 64, DP == 64 ? 3 : 2) void doc_attn_dq_kernel(
 // queries of every head that shares it pass in tiles of 64.  Shared heads
 // leave few such waves and give each a long walk: then the walk is split, its
 // parts' sums stay in fp32 and doc_attn_join_kernel adds them, in their order.
-// The same packed tokens: 77 us; the same 16 heads: 485 us and 23 to join.
+// The same packed tokens: 77 us; the same 16 heads, in
+// fp16 (kPUp): 570 us and 23 to join.
 // ---------------------------------------------------------------------------
 
 template <typename T, int DP, int NW, bool BIAS>

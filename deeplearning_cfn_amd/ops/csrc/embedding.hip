@@ -7,8 +7,10 @@
 // Both directions are bound by memory.  The lookup reads each row and
 // writes y once, in one launch for all tables.
 //
-// The gradient sorts the tokens by id and sums each row's tokens in that
-// order, so every bit is the same from run to run (no float atomics).
+// The gradient sorts the tokens by id and sums each row's tokens in a fixed
+// order, so every bit is the same from run to run (no float atomics).  It is
+// the tokens' own up to 65536 of them; of more, a chunk's waves come one after
+// the other, each with its tokens.
 //   1. Tokens into buckets, id % G (frequent ids are neighbours in a
 //      vocabulary, so this spreads them): embed_count counts each of up to
 //      64 chunks of the tokens, embed_scatter turns the counts into places

@@ -638,7 +638,7 @@ def embedding_sum(ids: Sequence[torch.Tensor], tables: Sequence[torch.Tensor],
 
     ``ids``: int32 or int64 tensors of one shape; ``tables``: [rows_j, width]
     of one type (bf16, fp16, fp32).  The sum is taken in fp32 and rounded
-    once.  A table's gradient adds its tokens in their order in fp32, so it
+    once.  A table's gradient adds its tokens in a fixed order in fp32, so it
     is the same from run to run.  On the GPU an id outside its table gives a
     row of NaN and takes no part in the gradient (on the CPU it raises), and
     a table that wants a gradient has under 2^22 rows.
@@ -751,7 +751,12 @@ def document_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     ``slopes[h] * |i - j|`` off the scores; it gets no gradient.
 
     Fused CDNA4 kernels for bf16 and fp16 with dim a multiple of 8 up to 128;
-    anything else runs document by document in torch, in fp32.
+    anything else runs document by document in torch, in fp32, and reads the
+    borders on the host (it cannot be captured).  The kernels round P and dS
+    to the inputs' type, in two parts in documents of up to 64 tokens and in
+    calls of up to 1024: a document's last bits may hang on the size of the
+    call (as shared heads' sums over queries do), not on what its neighbours
+    hold.  They have no forward-mode gradient.
     """
     if q.dim() == 3 and _doc_attention_native(q):
         scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
