@@ -951,7 +951,7 @@ at::Tensor newton_schulz_impl(const at::Tensor& g_in, int64_t steps,
   if (g.numel() == 0) return out;
   TORCH_CHECK(rows <= (1 << 20) && cols <= (1 << 20) && batch <= 65535,
               "newton_schulz: the matrices are too large or too many");
-  // The larger tile where it pads little and its last round of 256 CUs is
+  // The larger tile where it pads little and its last turn of 256 CUs is
   // nearly full: at most 56 of them, or a sixth of all tiles, without one.  us
   // of five steps, all of 128 / update of 256 / square too:
   //   768 x 768      x 32 684 / 731 / 745   x 56 1095 / 1079 / 1216
